@@ -165,6 +165,61 @@ size_t shvk_gdn_chunked_workspace_bytes(int B, int T, int H);
 int shvk_gdn_chunked(const void* q, const void* k, const void* v, const float* g, const float* beta, void* o, int o_dtype,
                      int B, int T, int H, int DK, int DV, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The gated delta rule with states that are kept between calls, over packed sequences.  Rows of all sequences lie one behind the
+ * other: sequence n has the rows seq_start[n] .. seq_start[n + 1] - 1 (device, [n_seq + 1], not falling, at most n_tokens); a sequence
+ * may have no rows, and rows behind the last sequence are neither read nor written.  q, k, v, o in `dtype` with row pitches in
+ * elements, head h at h * DK (q, k) or h * DV (v, o) of its row; HK query / key heads, HV value heads, value head h uses key head
+ * h / (HV / HK).  g (log decay) and beta fp32, row pitch ldgb.  l2norm != 0: q and k are divided by sqrt(x.x + 1e-6) first; q is
+ * multiplied by `scale` either way.
+ *     S <- exp(g) S + k u^T,  u = beta (v - exp(g) S^T k),  o = S^T q
+ * States are fp32 [n_slots][HV][DK][DV].  Sequence n starts from slot slot_in[n] and leaves its last state in slot slot_out[n]; a
+ * value outside [0, n_slots), or a NULL array, means a zero state and a state that is not kept.  The two may name the same slot.  A
+ * slot is written by one sequence of a call at most, and read by no other sequence of that call then (what is left there or read
+ * from there is unspecified otherwise).  A sequence without rows copies its state.  DK 64 or 128; DV a multiple of 32, 32 .. 256;
+ * q, k, v, o and states 16-byte aligned, row pitches of q, k, v, o multiples of 16 bytes.  Launched on the current device.
+ * Extends the reference's recurrence (engine/cuda/seq.cu:107-195: one sequence length, a zero initial state, none left). */
+typedef struct shvk_gdn_seq_args {
+    int n_seq, HK, HV, DK, DV;
+    int dtype;
+    int l2norm;
+    float scale;
+    long long n_tokens;
+    const void* q; long long ldq;
+    const void* k; long long ldk;
+    const void* v; long long ldv;
+    const float* g; const float* beta; long long ldgb;
+    void* o; long long ldo;
+    const int32_t* seq_start;
+    float* states; long long n_slots;
+    const int32_t* slot_in; const int32_t* slot_out;
+} shvk_gdn_seq_args;
+/* Token by token in fp32, any storage type: new tokens of live sequences (one, or a few), and the exact tier's form of any length. */
+int shvk_gdn_step(const shvk_gdn_seq_args* a, void* stream);
+
+/* What stands between two blocks, in one pass over rows of D values (1 .. 16384): the norm, gate and scale of a block's output, the
+ * residual sum, the norm in front of the next block:
+ *     y = x;  y = rmsnorm(y) * post_w  (post_w given);  y = y * act(gate)  (gate given);  h = scale * y (+ h_in, if given)
+ *     h_out = h  (if given);  xn = rmsnorm(h) * pre_w  (pre_w given, and xn with it)
+ * with rmsnorm(z) = z / sqrt(mean(z^2) + eps) in fp32 over the D values, xn from h before it is rounded.  act: 0 none, 1 SiLU, 2
+ * sigmoid.  Row r of an array lies at r * ld (elements); with heads > 1 it holds `heads` groups of D values, each normalised by
+ * itself, post_w and pre_w shared by them (the gated norm behind the delta rule: D = DV).  ldgate = 0: one gate row for all rows.
+ * x, gate and xn in x_dtype (gate_dtype and xn_dtype say the same), h_in and h_out in h_dtype (fp32 or x_dtype).  h_out may be h_in,
+ * and xn or h_out may be x, with the same pitch and type; else outputs overlap nothing.  Extends shvk_rmsnorm (rows of 384, no gate,
+ * no residual; engine/cuda/seq.cu:44-69, and the gated norm of seq.cu:197-214). */
+typedef struct shvk_block_norm_args {
+    long long rows; int heads; int D;
+    const void* x; long long ldx; int x_dtype;
+    const float* post_w;
+    const void* gate; long long ldgate; int gate_dtype; int gate_act;
+    float scale;
+    const void* h_in; long long ldh_in;
+    void* h_out; long long ldh_out; int h_dtype;
+    const float* pre_w;
+    void* xn; long long ldxn; int xn_dtype;
+    float eps;
+} shvk_block_norm_args;
+int shvk_block_norm(const shvk_block_norm_args* a, void* stream);
+
 /* SISA attention of the readout row per (clip, head): -softplus(alpha), logsigmoid(forget), theta prefix sums in
  * double rounded to fp32, pair rotation of B (all rows) and C (row 320), scores, softmax over 321 keys, y = P V.
  * S: [B*321][1072] fp32; QC: [B][576] fp32; Y: [B][384] fp32.

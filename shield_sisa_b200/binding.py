@@ -44,6 +44,25 @@ class ReadoutWeights(C.Structure):
                                           "head_w2", "head_b2")]
 
 
+class GdnSeqArgs(C.Structure):
+    """shvk_gdn_seq_args: packed sequences of the delta rule with kept states."""
+    _fields_ = [("n_seq", C.c_int), ("HK", C.c_int), ("HV", C.c_int), ("DK", C.c_int), ("DV", C.c_int), ("dtype", C.c_int),
+                ("l2norm", C.c_int), ("scale", C.c_float), ("n_tokens", C.c_longlong), ("q", C.c_void_p),
+                ("ldq", C.c_longlong), ("k", C.c_void_p), ("ldk", C.c_longlong), ("v", C.c_void_p), ("ldv", C.c_longlong),
+                ("g", C.c_void_p), ("beta", C.c_void_p), ("ldgb", C.c_longlong), ("o", C.c_void_p), ("ldo", C.c_longlong),
+                ("seq_start", C.c_void_p), ("states", C.c_void_p), ("n_slots", C.c_longlong), ("slot_in", C.c_void_p),
+                ("slot_out", C.c_void_p)]
+
+
+class BlockNormArgs(C.Structure):
+    """shvk_block_norm_args: norm, gate, scale, residual and norm between two blocks."""
+    _fields_ = [("rows", C.c_longlong), ("heads", C.c_int), ("D", C.c_int), ("x", C.c_void_p), ("ldx", C.c_longlong),
+                ("x_dtype", C.c_int), ("post_w", C.c_void_p), ("gate", C.c_void_p), ("ldgate", C.c_longlong),
+                ("gate_dtype", C.c_int), ("gate_act", C.c_int), ("scale", C.c_float), ("h_in", C.c_void_p),
+                ("ldh_in", C.c_longlong), ("h_out", C.c_void_p), ("ldh_out", C.c_longlong), ("h_dtype", C.c_int),
+                ("pre_w", C.c_void_p), ("xn", C.c_void_p), ("ldxn", C.c_longlong), ("xn_dtype", C.c_int), ("eps", C.c_float)]
+
+
 LOAD_FN = C.CFUNCTYPE(C.c_void_p, C.c_char_p, C.c_char_p, C.c_int, C.POINTER(Options))
 FREE_FN = C.CFUNCTYPE(None, C.c_void_p)
 SUBMIT_FN = C.CFUNCTYPE(C.c_void_p, C.c_void_p, C.POINTER(Request))
@@ -158,6 +177,8 @@ def load_library(experimental: bool = True) -> C.CDLL:
         "shvk_gdn_scan_status": (i32, [C.POINTER(i32)]),
         "shvk_gdn_chunked_workspace_bytes": (sz, [i32, i32, i32]),
         "shvk_gdn_chunked": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, C.c_float, vp, sz, vp]),
+        "shvk_gdn_step": (i32, [C.POINTER(GdnSeqArgs), vp]),
+        "shvk_block_norm": (i32, [C.POINTER(BlockNormArgs), vp]),
         "shvk_sisa_attn": (i32, [vp, vp, vp, vp, i32, vp]),
         "shvk_sisa_attn_h16": (i32, [vp, vp, vp, vp, vp, i32, vp]),
         "shvk_readout_qc": (i32, [vp, C.c_longlong, vp, vp, vp, i32, vp]),

@@ -1,0 +1,294 @@
+// What stands between two blocks of a layer, in one pass over the rows:
+//
+//   y = x;  y = y rstd(y) post_w;  y = y act(gate);  h = h_in + scale y;  h_out = h;  xn = h rstd(h) pre_w
+// with rstd(z) = 1 / sqrt(mean(z^2) + eps), every step in float32 and each output rounded once.  HBM binds: a row's arrays are read
+// once into registers, its two sums of squares are reductions over the threads that hold the row.
+//
+// A thread has NV groups of eight consecutive values (16-byte accesses): 16 threads, a warp or a whole CTA to a row, by its length.
+// Rows whose pitch is no multiple of eight start anywhere in such a group.  All arrays of a call then start at the same place of it (or
+// the call goes to block_norm_any_kernel), and the place repeats every eight rows at most: a CTA walks rows of one class, which are
+// cut at the same places, so that its copy of the weights in shared memory, shifted as its rows are, serves them all with 16-byte
+// reads.  A group that reaches over a row's end is read and written value by value.
+#include "device_utils.cuh"
+#include "shv_seq_kernels.h"
+
+#include <type_traits>
+
+namespace sb {
+namespace {
+
+constexpr int BN_MAXD = 16384;
+
+template <typename T> __device__ __forceinline__ void get8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
+    }
+}
+template <typename T> __device__ __forceinline__ void put8(T* p, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint4 w;
+        T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = from_float<T>(v[i]);
+        *reinterpret_cast<uint4*>(p) = w;
+    }
+}
+
+// act(g): SiLU and sigmoid from one exponential
+template <typename T> __device__ __forceinline__ float gate_of(float g, int act) {
+    if (act == 0) return g;
+    const float s = sizeof(T) == 4 ? 1.0f / (1.0f + expf(-g)) : __fdividef(1.0f, 1.0f + __expf(-g));
+    return act == 1 ? g * s : s;
+}
+
+// ROWT: threads of a row: 16, 32, or 0 = the whole CTA.  P: classes of rows (1 where every row starts on a group).
+template <typename T, typename TH, int NV, int ROWT>
+__global__ void __launch_bounds__(ROWT ? 128 : 512)
+block_norm_kernel(const shvk_block_norm_args a, int P) {
+    extern __shared__ __align__(16) float bn_w[];                // post_w | pre_w | gate row, each `span` floats
+    __shared__ float red[2][2][32];                              // [row parity][which sum][warp]
+    const int tid = threadIdx.x, rt = ROWT ? ROWT : blockDim.x, span = rt * NV * 8;
+    const int groups = ROWT ? blockDim.x / ROWT : 1, grp = ROWT ? tid / ROWT : 0, j = ROWT ? tid % ROWT : tid;
+    const int cls = blockIdx.x % P;
+    const long long cta = blockIdx.x / P, ctas = gridDim.x / P, total = a.rows * a.heads;
+    const int off = int(cls * (a.ldx & 7) & 7);                  // where the class's rows start in a group (0 where P is 1)
+    const bool post = a.post_w, pre = a.pre_w, one_gate = a.gate && a.ldgate == 0 && a.heads == 1;
+    const float inv_d = 1.0f / float(a.D);
+    int lo[NV], hi[NV];                                          // the values of each group that belong to the row: [lo, hi)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (j + i * rt) * 8 - off;                    // column of the group's first value
+        lo[i] = c < 0 ? min(-c, 8) : 0;
+        hi[i] = max(min(a.D - c, 8), 0);
+    }
+    auto load = [&](const auto* p, int i, float (&v)[8]) {            // p: the group's first value
+        if (hi[i] - lo[i] == 8) {
+            get8(p, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = e >= lo[i] && e < hi[i] ? to_float(p[e]) : 0.0f;
+        }
+    };
+    auto store = [&](auto* p, int i, const float (&v)[8]) {
+        if (hi[i] - lo[i] == 8) {
+            put8(p, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e >= lo[i] && e < hi[i]) p[e] = from_float<std::remove_pointer_t<decltype(p)>>(v[e]);
+        }
+    };
+    bool staged = false;
+    int par = 0;
+    // whole CTAs walk the rows in step: a group without a row of its own goes along without touching memory
+    for (long long at = cta * groups; P * at + cls < total; at += ctas * groups, par ^= 1) {
+        const long long R = P * (at + grp) + cls;
+        const bool on = R < total;
+        const long long row = on ? (a.heads == 1 ? R : R / a.heads) : 0;
+        const long long base = (on ? R - row * a.heads : 0) * a.D - off + j * 8;
+        float x[NV][8], h[NV][8], ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const long long c = base + i * rt * 8;
+            const bool any = on && hi[i] > lo[i];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] = h[i][e] = 0.0f;
+            float gt[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
+            if (any) {
+                load(static_cast<const T*>(a.x) + row * a.ldx + c, i, x[i]);
+                if (a.h_in) load(static_cast<const TH*>(a.h_in) + row * a.ldh_in + c, i, h[i]);
+                if (a.gate && !one_gate) {
+                    load(static_cast<const T*>(a.gate) + row * a.ldgate + c, i, gt);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) gt[e] = gate_of<T>(gt[e], a.gate_act);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {                        // the row's rstd is one factor of all its values: the gate may go first
+                ss = fmaf(x[i][e], x[i][e], ss);
+                x[i][e] *= gt[e];
+            }
+        }
+        if (!staged) {                                           // behind the first row's loads
+            for (int e = tid; e < span; e += blockDim.x) {
+                const int c = e - off;
+                const bool in = c >= 0 && c < a.D;
+                if (post) bn_w[e] = in ? a.post_w[c] : 0.0f;
+                if (pre) bn_w[span + e] = in ? a.pre_w[c] : 0.0f;
+                if (one_gate) bn_w[2 * span + e] = in ? gate_of<T>(to_float(static_cast<const T*>(a.gate)[c]), a.gate_act) : 0.0f;
+            }
+            __syncthreads();
+            staged = true;
+        }
+        auto row_sum = [&](float v, int which) {
+#pragma unroll
+            for (int o = ROWT == 16 ? 8 : 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if constexpr (ROWT == 0) {
+                if ((tid & 31) == 0) red[par][which][tid >> 5] = v;
+                __syncthreads();
+                const int nw = blockDim.x >> 5;
+                v = (tid & 31) < nw ? red[par][which][tid & 31] : 0.0f;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            }
+            return v;
+        };
+        if (post) {
+            const float r = 1.0f / sqrtf(row_sum(ss, 0) * inv_d + a.eps);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float w[8];
+                get8<float>(bn_w + (j + i * rt) * 8, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[i][e] = x[i][e] * r * w[e];
+            }
+        }
+        ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (one_gate) {
+                float w[8];
+                get8<float>(bn_w + 2 * span + (j + i * rt) * 8, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[i][e] *= w[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[i][e] = a.h_in ? fmaf(x[i][e], a.scale, h[i][e]) : x[i][e] * a.scale;
+            const bool any = on && hi[i] > lo[i];
+            if (any && a.h_out) store(static_cast<TH*>(a.h_out) + row * a.ldh_out + base + i * rt * 8, i, h[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+        }
+        if (pre) {
+            const float r = 1.0f / sqrtf(row_sum(ss, 1) * inv_d + a.eps);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float w[8];
+                get8<float>(bn_w + span + (j + i * rt) * 8, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = h[i][e] * r * w[e];
+                if (on && hi[i] > lo[i]) store(static_cast<T*>(a.xn) + row * a.ldxn + base + i * rt * 8, i, w);
+            }
+        }
+    }
+}
+
+// Any pitch and alignment: a CTA per row, value by value, the row's h in shared memory (h_out may be h_in, so h is not made twice).
+template <typename T, typename TH>
+__global__ void __launch_bounds__(256) block_norm_any_kernel(const shvk_block_norm_args a) {
+    extern __shared__ float bn_h[];
+    __shared__ float red[2][8];
+    const int tid = threadIdx.x;
+    const long long row = blockIdx.x / a.heads, base = blockIdx.x % a.heads * (long long)a.D;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx + base;
+    const T* gate = a.gate ? static_cast<const T*>(a.gate) + row * a.ldgate + base : nullptr;
+    const TH* h_in = a.h_in ? static_cast<const TH*>(a.h_in) + row * a.ldh_in + base : nullptr;
+    auto row_sum = [&](float v, int which) {
+        v = warp_sum(v);
+        if ((tid & 31) == 0) red[which][tid >> 5] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v += red[which][w];
+        return v;
+    };
+    float r = 1.0f, ss = 0.0f;
+    if (a.post_w) {
+        for (int c = tid; c < a.D; c += 256) {
+            const float v = to_float(x[c]);
+            ss = fmaf(v, v, ss);
+        }
+        r = 1.0f / sqrtf(row_sum(ss, 0) / float(a.D) + a.eps);
+    }
+    ss = 0.0f;
+    for (int c = tid; c < a.D; c += 256) {
+        float v = to_float(x[c]);
+        if (a.post_w) v = v * r * a.post_w[c];
+        if (gate) v *= gate_of<T>(to_float(gate[c]), a.gate_act);
+        v = h_in ? fmaf(v, a.scale, to_float(h_in[c])) : v * a.scale;
+        if (a.h_out) static_cast<TH*>(a.h_out)[row * a.ldh_out + base + c] = from_float<TH>(v);
+        ss = fmaf(v, v, ss);
+        bn_h[c] = v;                                             // read back by this thread alone
+    }
+    if (a.pre_w) {
+        r = 1.0f / sqrtf(row_sum(ss, 1) / float(a.D) + a.eps);
+        for (int c = tid; c < a.D; c += 256) static_cast<T*>(a.xn)[row * a.ldxn + base + c] = from_float<T>(bn_h[c] * r * a.pre_w[c]);
+    }
+}
+
+template <typename T, typename TH, int NV, int ROWT>
+int launch_rows(const shvk_block_norm_args& a, int P, int threads, cudaStream_t s) {
+    const int groups = ROWT ? threads / ROWT : 1, span = (ROWT ? ROWT : threads) * NV * 8;
+    const int smem = 3 * span * int(sizeof(float));
+    static_assert(3 * 4 * 512 * 8 * sizeof(float) <= 200 * 1024, "the longest row's weights fit");
+    const cudaError_t e = cudaFuncSetAttribute(block_norm_kernel<T, TH, NV, ROWT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return int(e);
+    const long long need = ((a.rows * a.heads + P - 1) / P + groups - 1) / groups * P;     // CTAs of one pass over the rows
+    const int resident = 1024 / threads;
+    const long long most = (long long)device_sms() * resident / P * P;
+    const long long ctas = need < most ? need : (most > 0 ? most : P);
+    block_norm_kernel<T, TH, NV, ROWT><<<unsigned(ctas), threads, smem, s>>>(a, P);
+    return int(cudaGetLastError());
+}
+
+inline bool on_group(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T, typename TH> int launch_block_norm(const shvk_block_norm_args& a, cudaStream_t s) {
+    // the vector form: every array starts on 16 bytes, and a row starts at the same place of a group of eight in all of them
+    const int ld = int(a.ldx & 7);
+    const bool gate_rows = a.gate && (a.ldgate || a.heads > 1);
+    const bool vec = on_group(a.x) && on_group(a.h_in) && on_group(a.h_out) && on_group(a.xn) && (!gate_rows || on_group(a.gate)) &&
+                     (!a.h_in || (a.ldh_in & 7) == ld) && (!a.h_out || (a.ldh_out & 7) == ld) && (!a.xn || (a.ldxn & 7) == ld) &&
+                     (!gate_rows || (a.ldgate & 7) == ld) && (a.heads == 1 || (ld == 0 && a.D % 8 == 0));
+    const int P = a.rows == 1 ? 1 : ld == 0 ? 1 : ld % 2 ? 8 : ld % 4 ? 4 : 2, nvec = (a.D + (P > 1 ? 7 : 0) + 7) / 8;
+    if (!vec || nvec > 2048) {
+        if (a.rows * a.heads > 0x7fffffff) return int(cudaErrorInvalidValue);
+        const int smem = a.D * int(sizeof(float));
+        const cudaError_t e = cudaFuncSetAttribute(block_norm_any_kernel<T, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return int(e);
+        block_norm_any_kernel<T, TH><<<unsigned(a.rows * a.heads), 256, smem, s>>>(a);
+        return int(cudaGetLastError());
+    }
+    if (nvec <= 16) return launch_rows<T, TH, 1, 16>(a, P, 128, s);
+    if (nvec <= 32) return launch_rows<T, TH, 1, 32>(a, P, 128, s);
+    if (nvec <= 64) return launch_rows<T, TH, 2, 32>(a, P, 128, s);
+    if (nvec <= 1024) return launch_rows<T, TH, 2, 0>(a, P, ((nvec + 1) / 2 + 31) / 32 * 32, s);
+    return launch_rows<T, TH, 4, 0>(a, P, ((nvec + 3) / 4 + 31) / 32 * 32, s);
+}
+
+inline bool on_type(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == DT_F32 ? 3 : 1)) == 0; }
+
+}  // namespace
+}  // namespace sb
+
+extern "C" int shvk_block_norm(const shvk_block_norm_args* a, void* stream) {
+    using namespace sb;
+    constexpr int bad = int(cudaErrorInvalidValue);
+    if (!a || a->rows < 0 || a->heads < 1 || a->heads > 4096 || a->D < 1 || a->D > BN_MAXD) return bad;
+    const int t = a->x_dtype;
+    if (t != DT_F32 && t != DT_BF16 && t != DT_F16) return bad;
+    if (a->h_dtype != DT_F32 && a->h_dtype != t) return bad;
+    if ((a->gate && (a->gate_dtype != t || a->gate_act < 0 || a->gate_act > 2)) || (a->xn && a->xn_dtype != t)) return bad;
+    if (!!a->pre_w != !!a->xn || (!a->h_out && !a->xn)) return bad;
+    if (a->rows == 0) return 0;
+    if (!a->x) return bad;
+    const long long width = (long long)a->heads * a->D;
+    if (a->ldx < 0 || (a->h_in && a->ldh_in < 0) || (a->gate && a->ldgate < 0)) return bad;
+    if (a->rows > 1 && ((a->h_out && a->ldh_out < width) || (a->xn && a->ldxn < width))) return bad;
+    if (!on_type(a->x, t) || !on_type(a->gate, t) || !on_type(a->xn, t) || !on_type(a->h_in, a->h_dtype) || !on_type(a->h_out, a->h_dtype) ||
+        !on_type(a->post_w, DT_F32) || !on_type(a->pre_w, DT_F32))
+        return bad;
+    cudaStream_t s = cudaStream_t(stream);
+    if (t == DT_F32) return launch_block_norm<float, float>(*a, s);
+    if (t == DT_BF16) return a->h_dtype == DT_F32 ? launch_block_norm<__nv_bfloat16, float>(*a, s) : launch_block_norm<__nv_bfloat16, __nv_bfloat16>(*a, s);
+    return a->h_dtype == DT_F32 ? launch_block_norm<__half, float>(*a, s) : launch_block_norm<__half, __half>(*a, s);
+}

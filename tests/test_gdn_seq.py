@@ -1,0 +1,367 @@
+"""The delta rule with kept states over packed sequences (shvk_gdn_step, shvk_gdn_prefill) against the rule in float64, and what it
+refuses.
+
+Tolerances.  An output in a 16-bit type is off by half a step of its type, eps / 2 of its value.  Everything else is float32
+arithmetic: a product with the state sums DK terms, whose partial sums are rounded up to DK times, and a token adds a dozen roundings
+to a state entry; errors carried by the state do not grow, because I - beta k k^T with |k| <= 1 and beta <= 1, and a decay below one,
+are contractions.  So an output is within (DK + 16 T) 2^-24 of the largest sum of magnitudes that enters one, |q| |S|, and a state
+within the same factor of the largest state column.  The prefill form's pieces are held in 22 bits, which adds two steps of 2^-22
+(8 x 2^-24) a chunk: its factor is (DK + 24 T) 2^-24.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from shield_sisa_b200 import binding
+
+CODES = {"fp32": 0, "bf16": 1, "fp16": 2}
+INVALID = 1                                                     # cudaErrorInvalidValue
+
+
+@pytest.fixture(scope="module")
+def L():
+    from shield_sisa_b200 import build
+    build.build()
+    return binding.load_library(True)
+
+
+def call(L, form, a, ws=None, stream=None):
+    if form == "step":
+        return L.shvk_gdn_step(C.byref(a), stream)
+    return L.shvk_gdn_prefill(C.byref(a), ws, L.shvk_gdn_prefill_workspace_bytes(C.byref(a)) if ws else 0, stream)
+
+
+# ---------------------------------------------------------------------------------------------- refusals (no GPU)
+def good(**kw):
+    p = 0x100000                                                # never dereferenced: every call below ends on the host
+    a = dict(n_seq=2, HK=2, HV=4, DK=64, DV=128, dtype=1, l2norm=1, scale=0.125, n_tokens=9, q=p, ldq=128, k=p, ldk=128, v=p,
+             ldv=512, g=p, beta=p, ldgb=4, o=p, ldo=512, seq_start=p, states=p, n_slots=4, slot_in=p, slot_out=p)
+    a.update(kw)
+    return binding.GdnSeqArgs(**a)
+
+
+BAD = [dict(n_seq=-1), dict(n_tokens=-1), dict(n_tokens=1 << 31), dict(dtype=3), dict(dtype=-1), dict(DK=96), dict(DK=32),
+       dict(DK=256), dict(DV=0), dict(DV=48), dict(DV=288), dict(HK=0), dict(HV=0), dict(HV=5), dict(HK=3), dict(HV=8192),
+       dict(seq_start=None), dict(q=None), dict(k=None), dict(v=None), dict(g=None), dict(beta=None), dict(o=None),
+       dict(q=0x100008), dict(k=0x100002), dict(v=0x100004), dict(o=0x100008), dict(ldq=129), dict(ldk=132), dict(ldv=514),
+       dict(ldo=513), dict(ldo=504), dict(ldq=-128), dict(ldgb=-1), dict(states=None), dict(states=0x100004), dict(n_slots=-1)]
+
+
+@pytest.mark.parametrize("kw", BAD, ids=lambda d: "-".join(f"{k}={v}" for k, v in d.items()))
+def test_step_refuses(L, kw):
+    assert call(L, "step", good(**kw)) == INVALID
+
+
+def test_step_of_nothing_launches_nothing(L):
+    assert L.shvk_gdn_step(None, None) == INVALID
+    assert call(L, "step", good(n_seq=0)) == 0
+    assert call(L, "step", good(n_seq=0, seq_start=None, q=None)) == 0
+
+
+# ---------------------------------------------------------------------------------------------- GPU
+gpu = pytest.mark.gpu
+LAYOUTS = [(6, 6, 64, 128), (2, 6, 128, 128), (1, 4, 64, 64), (2, 2, 128, 256), (3, 3, 64, 32), (1, 1, 128, 96)]
+
+
+def make(kind, lens, hk, hv, dk, dv, seed, tail=3, fused=False, unit=False, slots=None):
+    """A call's buffers: packed rows (separate, or slices of one fused row), states, slots."""
+    import torch
+    t = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}[kind]
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
+    n, rows = len(lens), sum(lens) + tail
+    x = {"n": n, "lens": lens, "hk": hk, "hv": hv, "dk": dk, "dv": dv, "kind": kind, "rows": rows, "l2norm": not unit, "scale": dk ** -0.5}
+    widths = [hk * dk, hk * dk, hv * dv]
+    if fused:                                                   # q | k | v | something else
+        row = rn(rows, sum(widths) + 40).to(t)
+        parts = list(row.split(widths + [40], 1)[:3])
+    else:
+        parts = [rn(rows, w).to(t) for w in widths]
+    if unit:
+        for i in range(2):
+            p = parts[i].float().reshape(rows, hk, dk)
+            parts[i] = (p / p.norm(dim=-1, keepdim=True).clamp_min(1e-3)).reshape(rows, -1).to(t)
+    x["q"], x["k"], x["v"] = parts
+    x["g"] = -torch.exp(rn(rows, hv) - 2.0)
+    x["beta"] = torch.sigmoid(rn(rows, hv))
+    x["o"] = torch.full((rows, hv, dv), 7.0, device="cuda").to(t)
+    starts = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    x["seq_start"] = torch.from_numpy(starts).cuda()
+    x["n_slots"] = 2 * n + 1
+    x["states"] = rn(x["n_slots"], hv, dk, dv)
+    x["slot_in"] = torch.arange(n, device="cuda", dtype=torch.int32) if slots is None else slots[0]
+    x["slot_out"] = (n + torch.randperm(n, device="cuda", generator=gen)).to(torch.int32) if slots is None else slots[1]
+    return x
+
+
+def args(x):
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    return binding.GdnSeqArgs(n_seq=x["n"], HK=x["hk"], HV=x["hv"], DK=x["dk"], DV=x["dv"], dtype=CODES[x["kind"]],
+                              l2norm=int(x["l2norm"]), scale=x["scale"], n_tokens=x["rows"], q=ptr(x["q"]), ldq=x["q"].stride(0),
+                              k=ptr(x["k"]), ldk=x["k"].stride(0), v=ptr(x["v"]), ldv=x["v"].stride(0), g=ptr(x["g"]),
+                              beta=ptr(x["beta"]), ldgb=x["g"].stride(0), o=ptr(x["o"]), ldo=x["o"].stride(0),
+                              seq_start=ptr(x["seq_start"]), states=ptr(x["states"]), n_slots=x["n_slots"], slot_in=ptr(x["slot_in"]),
+                              slot_out=ptr(x["slot_out"]))
+
+
+def launch(L, form, x, stream=None):
+    """The call on the current (or the given) stream; the prefill form's workspace is poisoned: it must not rely on its contents."""
+    import torch
+    s = torch.cuda.current_stream() if stream is None else stream
+    a, ws = args(x), None
+    if form == "prefill":
+        need = L.shvk_gdn_prefill_workspace_bytes(C.byref(a))
+        if "ws" not in x or x["ws"].numel() < need:
+            x["ws"] = torch.full((max(need, 16),), 0xff, device="cuda", dtype=torch.uint8)
+        ws = x["ws"].data_ptr()
+    rc = call(L, form, a, ws, s.cuda_stream)
+    assert rc == 0, rc
+
+
+def rule(x, state0):
+    """o [rows, hv, dv] (7 where no sequence has a row), the state behind each sequence, |q| |S| at most, in float64."""
+    import torch
+    hk, hv, dk, dv, group = x["hk"], x["hv"], x["dk"], x["dv"], x["hv"] // x["hk"]
+    q = x["q"].double().reshape(x["rows"], hk, dk)
+    k = x["k"].double().reshape(x["rows"], hk, dk)
+    v = x["v"].double().reshape(x["rows"], hv, dv)
+    if x["l2norm"]:
+        q, k = (z / torch.sqrt((z * z).sum(-1, keepdim=True) + 1e-6) for z in (q, k))
+    q = q * float(np.float32(x["scale"]))
+    q, k = q.repeat_interleave(group, 1), k.repeat_interleave(group, 1)
+    o = torch.full((x["rows"], hv, dv), 7.0, device="cuda", dtype=torch.float64)
+    out, big = [], 0.0
+    row = 0
+    for n, ln in enumerate(x["lens"]):
+        S = state0[n].double().clone()
+        for _ in range(ln):
+            S = S * torch.exp(x["g"][row].double())[:, None, None]
+            u = x["beta"][row].double()[:, None] * (v[row] - torch.einsum("hk,hkv->hv", k[row], S))
+            S = S + k[row][:, :, None] * u[:, None, :]
+            o[row] = torch.einsum("hk,hkv->hv", q[row], S)
+            big = max(big, float((q[row].norm(dim=-1)[:, None] * S.norm(dim=1)).max()))
+            row += 1
+        out.append(S)
+    return o, out, big
+
+
+def first_states(x):
+    import torch
+    ids = [-1] * x["n"] if x["slot_in"] is None else x["slot_in"].tolist()
+    return [x["states"][i].clone() if 0 <= i < x["n_slots"] else torch.zeros_like(x["states"][0]) for i in ids]
+
+
+def check(L, form, x, **kw):
+    """Runs the call and compares all of its outputs, the rows and slots that it must leave alone among them."""
+    import torch
+    first, pool = first_states(x), x["states"].clone()
+    want, states, big = rule(x, first)
+    launch(L, form, x, **kw)
+    torch.cuda.synchronize()
+    total, longest = sum(x["lens"]), max(x["lens"] + [0])
+    factor = (x["dk"] + (16 if form == "step" else 24) * longest) * 2.0 ** -24
+    half = torch.finfo(x["o"].dtype).eps / 2
+    got = x["o"].double()
+    tiny = 2.0 ** -25 if x["kind"] == "fp16" else 0.0            # half a step of fp16's subnormal numbers
+    off = (got - want).abs() - half * want.abs()
+    assert float(off[:total].max()) <= factor * big + tiny if total else True
+    assert torch.equal(x["o"][total:], torch.full_like(x["o"][total:], 7.0))
+    written = {}
+    for n, s in enumerate([] if x["slot_out"] is None else x["slot_out"].tolist()):
+        if 0 <= s < x["n_slots"]:
+            written[s] = n
+    for s in range(x["n_slots"]):
+        if s not in written:
+            assert torch.equal(x["states"][s], pool[s])
+            continue
+        n = written[s]
+        if x["lens"][n] == 0:
+            assert torch.equal(x["states"][s], first[n])
+            continue
+        column = max(float(states[n].norm(dim=1).max()), float(first[n].double().norm(dim=1).max()))
+        assert float((x["states"][s].double() - states[n]).abs().max()) <= factor * column
+    return got, states
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("layout", LAYOUTS, ids=str)
+@pytest.mark.parametrize("lens", [[1], [1] * 7, [3, 0, 1, 8], [0], [33]], ids=str)
+def test_step(L, kind, layout, lens):
+    check(L, "step", make(kind, lens, *layout, seed=len(lens) + layout[2]))
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_step_on_slices_of_one_row_without_normalising(L, kind):
+    check(L, "step", make(kind, [2, 5, 1], 2, 4, 64, 128, seed=5, fused=True, unit=True))
+
+
+def slot_cases():
+    return {"none": (None, None), "in_place": ([2, 0, 4], [2, 0, 4]), "new": ([-1, -1, -1], [1, 5, 3]), "not_kept": ([3, 1, 1], [-1, -1, -1]),
+            "mixed": ([0, -1, 0], [1, 2, -1]), "outside": ([7, 1 << 30, -5], [3, 7, 1 << 30])}
+
+
+@gpu
+@pytest.mark.parametrize("form", ["step"])
+@pytest.mark.parametrize("name", list(slot_cases()))
+def test_slots(L, form, name):
+    """States read from and left in the slots that are named, by whom; a slot read by many; values that are no slot."""
+    import torch
+    s = tuple(None if v is None else torch.tensor(v, device="cuda", dtype=torch.int32) for v in slot_cases()[name])
+    for lens in ([1, 1, 1], [0, 3, 20]):
+        check(L, form, make("bf16", lens, 2, 4, 64, 128, seed=3, slots=s))
+    if name == "none":
+        x = make("bf16", [2, 3, 1], 2, 4, 64, 128, seed=3, slots=s)
+        x["states"], keep = None, x["states"]
+        a = binding.GdnSeqArgs.from_buffer_copy(args({**x, "states": keep}))
+        a.states, a.n_slots = None, 0
+        assert call(L, form, a, None if form == "step" else x.setdefault("ws", torch.empty(1 << 22, device="cuda", dtype=torch.uint8)).data_ptr(),
+                    torch.cuda.current_stream().cuda_stream) == 0
+        want = rule(x, [torch.zeros_like(keep[0])] * 3)
+        assert float((x["o"].double() - want[0]).abs().max()) < 0.02 * float(want[0][:6].abs().max())
+
+
+@gpu
+@pytest.mark.parametrize("form", ["step"])
+def test_bounds_of_sequences_that_are_no_bounds(L, form):
+    """Starts outside the rows are cut to them: nothing outside the caller's rows is touched, and the sequences that are well described
+    are right."""
+    import torch
+    x = make("bf16", [4, 3, 5], 2, 4, 64, 128, seed=9, tail=0)
+    x["seq_start"] = torch.tensor([0, 4, -9, 1 << 30], device="cuda", dtype=torch.int32)      # 4 rows; none; all 12
+    guard = x["states"][2 * x["n"]].clone()
+    launch(L, form, x)
+    torch.cuda.synchronize()
+    y = make("bf16", [4, 3, 5], 2, 4, 64, 128, seed=9, tail=0)
+    y["lens"], y["n"] = [4], 1
+    assert torch.equal(x["states"][2 * x["n"]], guard)
+    y["seq_start"] = x["seq_start"][:2].clone()
+    before = y["states"].clone()
+    launch(L, form, y)
+    torch.cuda.synchronize()
+    slot = int(x["slot_out"][0])
+    assert torch.equal(x["states"][slot], y["states"][slot]) and not torch.equal(y["states"][slot], before[slot])
+
+
+@gpu
+@pytest.mark.parametrize("form", ["step"])
+def test_a_decay_to_nothing_forgets_everything(L, form):
+    """g = -inf and g = the type's lowest value: what follows does not depend on the state before, not even where that is huge."""
+    import torch
+    lens = [40, 17]
+    for low in (-float("inf"), torch.finfo(torch.float32).min):
+        outs = []
+        for fill in (0.0, 1e30):
+            x = make("bf16", lens, 2, 4, 64, 128, seed=11)
+            x["g"][7] = low
+            x["g"][42] = low
+            x["states"][:2] = fill if fill else x["states"][:2]
+            launch(L, form, x)
+            torch.cuda.synchronize()
+            outs.append((x["o"][7:40].clone(), x["o"][42:57].clone(), x["states"][x["slot_out"].long()].clone()))
+        for a, b in zip(*outs):
+            assert torch.isfinite(a).all()
+            assert torch.allclose(a.float(), b.float(), rtol=0.05, atol=2e-2 * float(a.abs().max()))
+        x = make("bf16", lens, 2, 4, 64, 128, seed=11)
+        x["g"][7] = low
+        x["g"][42] = low
+        check(L, form, x)
+
+
+@gpu
+@pytest.mark.parametrize("form", ["step"])
+def test_not_a_number_stays_in_its_sequence_and_head(L, form):
+    import torch
+    x = make("bf16", [20, 19, 21], 2, 4, 64, 128, seed=13)
+    y = make("bf16", [20, 19, 21], 2, 4, 64, 128, seed=13)
+    x["v"][25, 128:256] = float("nan")                          # sequence 1, value head 1
+    x["k"][62] = x["q"][62] = x["v"][62] = float("nan")         # a row behind the last sequence
+    launch(L, form, x)
+    launch(L, form, y)
+    torch.cuda.synchronize()
+    bad = torch.zeros(x["rows"], 4, dtype=torch.bool, device="cuda")
+    bad[25:39, 1] = True
+    assert torch.isnan(x["o"][bad].float()).all()
+    assert torch.equal(x["o"][~bad], y["o"][~bad])
+    sx, sy = (z["states"][z["slot_out"].long()] for z in (x, y))
+    keep = torch.ones(3, 4, dtype=torch.bool, device="cuda")
+    keep[1, 1] = False
+    assert torch.equal(sx[keep], sy[keep])
+
+
+@gpu
+@pytest.mark.parametrize("form", ["step"])
+def test_a_sequence_gives_the_same_bits_alone_and_in_a_batch(L, form):
+    import torch
+    lens = [18, 1, 33, 0, 16, 47] * 9
+    x = make("bf16", lens, 2, 4, 128, 128, seed=21)
+    launch(L, form, x)
+    torch.cuda.synchronize()
+    starts = np.concatenate([[0], np.cumsum(lens)])
+    for n in (0, 2, 5, 53):
+        y = make("bf16", lens, 2, 4, 128, 128, seed=21)
+        y["n"], y["lens"] = 1, [lens[n]]
+        y["seq_start"] = y["seq_start"][n:n + 2].clone()
+        y["slot_in"], y["slot_out"] = y["slot_in"][n:n + 1].clone(), y["slot_out"][n:n + 1].clone()
+        launch(L, form, y)
+        torch.cuda.synchronize()
+        assert torch.equal(x["o"][starts[n]:starts[n + 1]], y["o"][starts[n]:starts[n + 1]])
+        s = int(y["slot_out"][0])
+        assert torch.equal(x["states"][s], y["states"][s])
+
+
+@gpu
+@pytest.mark.parametrize("form", ["step"])
+def test_captured_replayed_and_on_two_streams(L, form):
+    """A captured call replays on new contents of its buffers; two calls with their own buffers run side by side."""
+    import torch
+    x = make("bf16", [5, 0, 18], 2, 4, 64, 128, seed=31)
+    launch(L, form, x)                                          # sizes the workspace outside the capture
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        launch(L, form, x)
+    y = make("bf16", [5, 0, 18], 2, 4, 64, 128, seed=32)
+    for name in ("q", "k", "v", "g", "beta", "states", "slot_out"):
+        x[name].copy_(y[name])
+    graph.replay()
+    launch(L, form, y)
+    torch.cuda.synchronize()
+    assert torch.equal(x["o"], y["o"]) and torch.equal(x["states"], y["states"])
+    a, b = make("bf16", [64] * 8, 2, 4, 64, 128, seed=41), make("bf16", [64] * 8, 2, 4, 64, 128, seed=42)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        launch(L, form, a, stream=s1)
+        launch(L, form, b, stream=s2)
+    torch.cuda.synchronize()
+    for z, seed in ((a, 41), (b, 42)):
+        w = make("bf16", [64] * 8, 2, 4, 64, 128, seed=seed)
+        launch(L, form, w)
+        torch.cuda.synchronize()
+        assert torch.equal(z["o"], w["o"])
+
+
+@gpu
+def test_slots_past_two_gigabytes(L):
+    """A pool whose last slots lie beyond 2^31 values."""
+    import torch
+    hv, dk, dv = 16, 128, 256
+    slots = (1 << 31) // (hv * dk * dv) + 3
+    x = make("bf16", [1, 2], 2, hv, dk, dv, seed=51)
+    small = x["states"][:2].clone()
+    x["states"] = torch.empty(slots, hv, dk, dv, device="cuda")
+    x["n_slots"] = slots
+    x["states"][slots - 2:] = small
+    x["slot_in"] = torch.tensor([slots - 2, -1], device="cuda", dtype=torch.int32)
+    x["slot_out"] = torch.tensor([slots - 1, slots - 3], device="cuda", dtype=torch.int32)
+    want, states, _ = rule(x, [small[0], torch.zeros_like(small[0])])
+    launch(L, "step", x)
+    torch.cuda.synchronize()
+    for s, ref in ((slots - 1, states[0]), (slots - 3, states[1])):
+        assert float((x["states"][s].double() - ref).abs().max()) < 1e-5 * float(ref.abs().max())
+    assert torch.equal(x["states"][slots - 2], small[0])
+    del x
+    torch.cuda.empty_cache()
