@@ -6,7 +6,10 @@ arithmetic: a product with the state sums DK terms, whose partial sums are round
 to a state entry; errors carried by the state do not grow, because I - beta k k^T with |k| <= 1 and beta <= 1, and a decay below one,
 are contractions.  So an output is within (DK + 16 T) 2^-24 of the largest sum of magnitudes that enters one, |q| |S|, and a state
 within the same factor of the largest state column.  The prefill form's pieces are held in 22 bits, which adds two steps of 2^-22
-(8 x 2^-24) a chunk: its factor is (DK + 24 T) 2^-24.
+(8 x 2^-24) a chunk: its factor is (DK + 24 T) 2^-24.  Its bf16 outputs come from single fp16 pieces: S cut off to eleven bits (less
+than 2^-10 of each entry), and M and U rounded to them (2^-11 each), so that o = M U + Q S0 is off by less than 2^-10 of
+sum |M| |U| + |q| |S0| more; that sum, over the up to 16 tokens of a chunk, is taken over the last 16 here, and |q| |S0| over all of
+them.
 """
 import ctypes as C
 
@@ -51,6 +54,25 @@ BAD = [dict(n_seq=-1), dict(n_tokens=-1), dict(n_tokens=1 << 31), dict(dtype=3),
 @pytest.mark.parametrize("kw", BAD, ids=lambda d: "-".join(f"{k}={v}" for k, v in d.items()))
 def test_step_refuses(L, kw):
     assert call(L, "step", good(**kw)) == INVALID
+
+
+@pytest.mark.parametrize("kw", BAD + [dict(dtype=0, ldq=128)], ids=lambda d: "-".join(f"{k}={v}" for k, v in d.items()))
+def test_prefill_refuses(L, kw):
+    a = good(**kw)
+    assert L.shvk_gdn_prefill(C.byref(a), 0x200000, 1 << 40, None) == INVALID
+    if "dtype" not in kw:
+        assert L.shvk_gdn_prefill_workspace_bytes(C.byref(a)) == 0
+
+
+def test_prefill_refuses_its_workspace(L):
+    a = good()
+    need = L.shvk_gdn_prefill_workspace_bytes(C.byref(a))
+    assert need >= 4 * 3 * 2048                                 # 4 heads; 9 rows of two sequences take three chunks at most
+    for ws, size in ((None, need), (0x200008, need), (0x200000, need - 1), (0x200000, 0)):
+        assert L.shvk_gdn_prefill(C.byref(a), ws, size, None) == INVALID
+    assert L.shvk_gdn_prefill(C.byref(good(n_seq=0)), None, 0, None) == 0
+    assert L.shvk_gdn_prefill_workspace_bytes(C.byref(good(n_seq=0))) == 0
+    assert L.shvk_gdn_prefill_workspace_bytes(None) == 0 and L.shvk_gdn_prefill(None, 0x200000, need, None) == INVALID
 
 
 def test_step_of_nothing_launches_nothing(L):
@@ -120,7 +142,8 @@ def launch(L, form, x, stream=None):
 
 
 def rule(x, state0):
-    """o [rows, hv, dv] (7 where no sequence has a row), the state behind each sequence, |q| |S| at most, in float64."""
+    """o [rows, hv, dv] (7 where no sequence has a row), the state behind each sequence, |q| |S| at most, in float64; x["pieces"]: the most
+    that |M| |U| + |q| |S0| of a chunk can be."""
     import torch
     hk, hv, dk, dv, group = x["hk"], x["hv"], x["dk"], x["dv"], x["hv"] // x["hk"]
     q = x["q"].double().reshape(x["rows"], hk, dk)
@@ -131,16 +154,20 @@ def rule(x, state0):
     q = q * float(np.float32(x["scale"]))
     q, k = q.repeat_interleave(group, 1), k.repeat_interleave(group, 1)
     o = torch.full((x["rows"], hv, dv), 7.0, device="cuda", dtype=torch.float64)
-    out, big = [], 0.0
+    out, big, x["pieces"] = [], 0.0, 0.0
     row = 0
     for n, ln in enumerate(x["lens"]):
         S = state0[n].double().clone()
+        last, size = [], [S.norm(dim=1)]
         for _ in range(ln):
             S = S * torch.exp(x["g"][row].double())[:, None, None]
             u = x["beta"][row].double()[:, None] * (v[row] - torch.einsum("hk,hkv->hv", k[row], S))
             S = S + k[row][:, :, None] * u[:, None, :]
             o[row] = torch.einsum("hk,hkv->hv", q[row], S)
             big = max(big, float((q[row].norm(dim=-1)[:, None] * S.norm(dim=1)).max()))
+            last, size = last[-15:] + [(k[row], u.abs())], size[-16:] + [S.norm(dim=1)]
+            mixed = sum(torch.einsum("hk,hk->h", q[row], kj).abs()[:, None] * uj for kj, uj in last)
+            x["pieces"] = max(x["pieces"], float((mixed + q[row].norm(dim=-1)[:, None] * torch.stack(size).amax(0)).max()))
             row += 1
         out.append(S)
     return o, out, big
@@ -164,8 +191,12 @@ def check(L, form, x, **kw):
     half = torch.finfo(x["o"].dtype).eps / 2
     got = x["o"].double()
     tiny = 2.0 ** -25 if x["kind"] == "fp16" else 0.0            # half a step of fp16's subnormal numbers
-    off = (got - want).abs() - half * want.abs()
-    assert float(off[:total].max()) <= factor * big + tiny if total else True
+    most = torch.finfo(x["o"].dtype).max
+    over = want.abs() > 1.01 * most                              # what the type cannot hold is infinite in it
+    assert torch.equal(got[over], torch.inf * want[over].sign())
+    off = torch.where(want.abs() > 0.99 * most, 0, (got - want).abs() - half * want.abs())
+    single = 2.0 ** -10 * x["pieces"] if form == "prefill" and x["kind"] == "bf16" else 0.0
+    assert float(off[:total].max()) <= factor * big + single + tiny if total else True
     assert torch.equal(x["o"][total:], torch.full_like(x["o"][total:], 7.0))
     written = {}
     for n, s in enumerate([] if x["slot_out"] is None else x["slot_out"].tolist()):
@@ -198,13 +229,144 @@ def test_step_on_slices_of_one_row_without_normalising(L, kind):
     check(L, "step", make(kind, [2, 5, 1], 2, 4, 64, 128, seed=5, fused=True, unit=True))
 
 
+LENGTHS = [[1], [16], [17, 15], [0, 1, 33, 48], [0], [79], [130, 2, 64, 0, 0, 31]]
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("layout", LAYOUTS, ids=str)
+@pytest.mark.parametrize("lens", LENGTHS, ids=str)
+def test_prefill(L, kind, layout, lens):
+    check(L, "prefill", make(kind, lens, *layout, seed=len(lens) + layout[2]))
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+def test_prefill_on_slices_of_one_row_without_normalising(L, kind):
+    check(L, "prefill", make(kind, [70, 5, 1], 2, 4, 64, 128, seed=5, fused=True, unit=True))
+    check(L, "prefill", make(kind, [70, 5, 1], 2, 4, 128, 128, seed=6, fused=True))
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 30, 60, 200])
+def test_prefill_of_few_and_many_sequences(L, n):
+    """Every share of the value columns that a CTA may take: the same bits in all."""
+    import torch
+    x = make("bf16", [50] * n, 2, 4, 128, 128, seed=8)
+    for name in ("q", "k", "v", "g", "beta"):
+        x[name][:50 * n] = x[name][:50].repeat(n, 1)
+    x["states"][:n] = x["states"][0].clone()
+    y = make("bf16", [50], 2, 4, 128, 128, seed=8)
+    for name in ("q", "k", "v", "g", "beta"):
+        y[name][:50] = x[name][:50]
+    y["states"][0] = x["states"][0]
+    check(L, "prefill", y)
+    launch(L, "prefill", x)
+    torch.cuda.synchronize()
+    for i in range(n):
+        assert torch.equal(x["o"][50 * i:50 * i + 50], y["o"][:50])
+    assert torch.equal(x["states"][x["slot_out"].long()], y["states"][1:2].expand(n, -1, -1, -1))
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("what", ["tiny_values", "huge_values", "huge_state", "tiny_state", "rising", "falling", "large_keys", "small_keys", "no_decay"])
+def test_prefill_of_any_size_of_numbers(L, kind, what):
+    """The scales of the pieces follow the numbers: a state or values far from one, that grow or fade by many powers of two on the way,
+    keys and queries that are normalised from far away."""
+    import torch
+    x = make(kind, [300, 45], 2, 4, 64, 128, seed=17)
+    far = 1e-4 if kind == "fp16" else 1e-12
+    at = torch.arange(x["rows"], device="cuda", dtype=torch.float32)[:, None]
+    t = x["v"].dtype
+    if what == "tiny_values":
+        x["v"] = (x["v"].float() * far).to(t)
+        x["states"] *= far
+    elif what == "huge_values":
+        x["v"] = (x["v"].float() * (1e3 if kind == "fp16" else 1e12)).to(t)
+    elif what == "huge_state":
+        x["states"] *= 1e15
+    elif what == "tiny_state":
+        x["states"] *= 1e-15
+    elif what == "rising":
+        x["v"] = (x["v"].float() * torch.exp(-4 + at / 25)).to(t)
+    elif what == "falling":
+        x["v"] = (x["v"].float() * torch.exp(4 - at / 25)).to(t)
+        x["g"] -= 0.2
+    elif what == "large_keys":
+        x["k"], x["q"] = (x["k"].float() * 1000).to(t), (x["q"].float() * 300).to(t)
+    elif what == "small_keys":
+        x["k"], x["q"] = (x["k"].float() * 0.01).to(t), (x["q"].float() * 0.02).to(t)
+    else:
+        x["g"] *= 0
+    check(L, "prefill", x)
+
+
+@gpu
+def test_step_continues_what_prefill_left(L):
+    """A prompt by the chunked form, then token after token in place, against one walk over all of it; and the two forms agree."""
+    import torch
+    lens, new = [65, 1, 40], 5
+    whole = make("bf16", [n + new for n in lens], 2, 4, 128, 128, seed=23, tail=0)
+    want, states, big = rule(whole, first_states(whole))
+    starts = np.concatenate([[0], np.cumsum([n + new for n in lens])])
+    factor = (128 + 24 * 70) * 2.0 ** -24
+
+    def part(pick, n_rows):
+        x = dict(whole)
+        idx = torch.tensor(pick, device="cuda")
+        for name in ("q", "k", "v", "g", "beta"):
+            x[name] = whole[name][idx].contiguous()
+        x["rows"], x["lens"] = len(pick), n_rows
+        x["o"] = torch.full((len(pick), 4, 128), 7.0, device="cuda").to(whole["o"].dtype)
+        x["seq_start"] = torch.from_numpy(np.concatenate([[0], np.cumsum(n_rows)]).astype(np.int32)).cuda()
+        return x
+    pick = [starts[i] + j for i, n in enumerate(lens) for j in range(n)]
+    x = part(pick, lens)
+    x.pop("ws", None)
+    launch(L, "prefill", x)
+    half = 2.0 ** -8
+    ref = want[torch.tensor(pick, device="cuda")]
+    assert float(((x["o"].double() - ref).abs() - half * ref.abs()).max()) <= factor * big + 2.0 ** -10 * whole["pieces"]
+    for j in range(new):
+        pick = [starts[i] + n + j for i, n in enumerate(lens)]
+        y = part(pick, [1] * 3)
+        y["slot_in"] = whole["slot_out"]
+        launch(L, "step", y)
+        ref = want[torch.tensor(pick, device="cuda")]
+        assert float(((y["o"].double() - ref).abs() - half * ref.abs()).max()) <= factor * big
+    for i in range(3):
+        got = whole["states"][int(whole["slot_out"][i])].double()
+        assert float((got - states[i]).abs().max()) <= factor * float(states[i].norm(dim=1).max())
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_prefill_keeps_float32_over_a_long_sequence(L, kind, dk):
+    """4,099 tokens with next to no decay: 257 chunks' sums.  As norms, where roundings do not add up but their squares do, the state is
+    within 1e-6 of float64 and an output within 1.3 half steps' rms of its type (eps / 2 / sqrt 3 over a mantissa of 1.4 on average)."""
+    import torch
+    x = make(kind, [4099], 1, 1, dk, 128, seed=29)
+    x["g"] *= 0.01
+    want, states, _ = rule(x, first_states(x))
+    launch(L, "prefill", x)
+    torch.cuda.synchronize()
+    s = x["states"][int(x["slot_out"][0])].double()
+    rel_s = float((s - states[0]).norm() / states[0].norm())
+    rel_o = float((x["o"][:4099].double() - want[:4099]).norm() / want[:4099].norm())
+    rms = torch.finfo(x["o"].dtype).eps / 2 / 3 ** 0.5 / 1.4
+    print(f"state {rel_s:.2e}, outputs {rel_o:.2e} (rounding alone {rms:.2e})")
+    assert rel_s < 1e-6 and rel_o < 1.3 * rms
+
+
 def slot_cases():
     return {"none": (None, None), "in_place": ([2, 0, 4], [2, 0, 4]), "new": ([-1, -1, -1], [1, 5, 3]), "not_kept": ([3, 1, 1], [-1, -1, -1]),
             "mixed": ([0, -1, 0], [1, 2, -1]), "outside": ([7, 1 << 30, -5], [3, 7, 1 << 30])}
 
 
 @gpu
-@pytest.mark.parametrize("form", ["step"])
+@pytest.mark.parametrize("form", ["step", "prefill"])
 @pytest.mark.parametrize("name", list(slot_cases()))
 def test_slots(L, form, name):
     """States read from and left in the slots that are named, by whom; a slot read by many; values that are no slot."""
@@ -224,7 +386,7 @@ def test_slots(L, form, name):
 
 
 @gpu
-@pytest.mark.parametrize("form", ["step"])
+@pytest.mark.parametrize("form", ["step", "prefill"])
 def test_bounds_of_sequences_that_are_no_bounds(L, form):
     """Starts outside the rows are cut to them: nothing outside the caller's rows is touched, and the sequences that are well described
     are right."""
@@ -246,24 +408,30 @@ def test_bounds_of_sequences_that_are_no_bounds(L, form):
 
 
 @gpu
-@pytest.mark.parametrize("form", ["step"])
+@pytest.mark.parametrize("form", ["step", "prefill"])
 def test_a_decay_to_nothing_forgets_everything(L, form):
-    """g = -inf and g = the type's lowest value: what follows does not depend on the state before, not even where that is huge."""
+    """g = -inf and g = the type's lowest value: what follows does not depend on the state before, not even where that is huge.  The
+    prefill form holds a chunk's 16 values of W = V - e K S0 in a column to 2^-35 of the largest: with a state of `fill`, W before the
+    reset is at most 8 fill (|k|_1 <= sqrt 64), so U behind it is off by up to 16 x 8 x 2^-35 fill, and what 16 of those make of an
+    output or a state (each times at most 1) by 2^-24 fill."""
     import torch
     lens = [40, 17]
     for low in (-float("inf"), torch.finfo(torch.float32).min):
         outs = []
-        for fill in (0.0, 1e30):
+        for fill in (0.0, 1e3, 1e30):
             x = make("bf16", lens, 2, 4, 64, 128, seed=11)
             x["g"][7] = low
             x["g"][42] = low
             x["states"][:2] = fill if fill else x["states"][:2]
             launch(L, form, x)
             torch.cuda.synchronize()
-            outs.append((x["o"][7:40].clone(), x["o"][42:57].clone(), x["states"][x["slot_out"].long()].clone()))
-        for a, b in zip(*outs):
-            assert torch.isfinite(a).all()
-            assert torch.allclose(a.float(), b.float(), rtol=0.05, atol=2e-2 * float(a.abs().max()))
+            outs.append((fill, x["o"][7:40].clone(), x["o"][42:57].clone(), x["states"][x["slot_out"].long()].clone()))
+        for fill, *got in outs:
+            for a, b in zip(outs[0][1:], got):
+                assert torch.isfinite(b).all()
+                lost = 2.0 ** -24 * fill if form == "prefill" else 0.0
+                step = 0.0 if a.dtype == torch.float32 else 2.0 ** -7
+                assert float((a.double() - b.double()).abs().max()) <= lost + (step + 1e-5) * float(a.abs().max())
         x = make("bf16", lens, 2, 4, 64, 128, seed=11)
         x["g"][7] = low
         x["g"][42] = low
@@ -271,7 +439,7 @@ def test_a_decay_to_nothing_forgets_everything(L, form):
 
 
 @gpu
-@pytest.mark.parametrize("form", ["step"])
+@pytest.mark.parametrize("form", ["step", "prefill"])
 def test_not_a_number_stays_in_its_sequence_and_head(L, form):
     import torch
     x = make("bf16", [20, 19, 21], 2, 4, 64, 128, seed=13)
@@ -292,7 +460,36 @@ def test_not_a_number_stays_in_its_sequence_and_head(L, form):
 
 
 @gpu
-@pytest.mark.parametrize("form", ["step"])
+@pytest.mark.parametrize("form", ["step", "prefill"])
+@pytest.mark.parametrize("name", ["q", "k", "v", "g", "beta"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_bad_token_does_not_reach_the_tokens_before_it(L, form, name, bad):
+    """The same bits, but in the bad token's own chunk of the prefill form: the powers of two that scale its pieces follow the largest
+    numbers of the chunk, the bad token's among them; at either scale the pieces hold 22 bits or 2^-35 of the largest, so that an output
+    there may move by 2^-20 of what enters it and then round the other way (one step, 2^-7)."""
+    import torch
+    x, y = make("bf16", [20, 45, 21], 2, 4, 64, 128, seed=13), make("bf16", [20, 45, 21], 2, 4, 64, 128, seed=13)
+    x[name][20 + 23] = bad                                      # sequence 1, the middle of its second chunk, all heads
+    launch(L, form, x)
+    launch(L, form, y)
+    torch.cuda.synchronize()
+    keep = torch.ones(x["rows"], dtype=torch.bool, device="cuda")
+    keep[43:65] = False
+    if form == "prefill":
+        keep[36:43] = False
+        a, b = x["o"][36:43].double(), y["o"][36:43].double()
+        assert float(((a - b).abs() - 2.0 ** -7 * b.abs()).max()) <= 2.0 ** -20 * float(y["o"][20:65].double().abs().max())
+    assert torch.equal(x["o"][keep], y["o"][keep])
+    if name == "q":                                             # nothing but its own output
+        keep[44:65] = True
+        assert torch.equal(x["o"][keep], y["o"][keep])
+    assert not torch.isfinite(x["o"][43].float()).all()
+    sx, sy = (z["states"][z["slot_out"].long()] for z in (x, y))
+    assert torch.equal(sx[[0, 2]], sy[[0, 2]]) and (name == "q") == bool(torch.equal(sx[1], sy[1]))
+
+
+@gpu
+@pytest.mark.parametrize("form", ["step", "prefill"])
 def test_a_sequence_gives_the_same_bits_alone_and_in_a_batch(L, form):
     import torch
     lens = [18, 1, 33, 0, 16, 47] * 9
@@ -313,7 +510,7 @@ def test_a_sequence_gives_the_same_bits_alone_and_in_a_batch(L, form):
 
 
 @gpu
-@pytest.mark.parametrize("form", ["step"])
+@pytest.mark.parametrize("form", ["step", "prefill"])
 def test_captured_replayed_and_on_two_streams(L, form):
     """A captured call replays on new contents of its buffers; two calls with their own buffers run side by side."""
     import torch
