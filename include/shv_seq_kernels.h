@@ -195,13 +195,15 @@ typedef struct shvk_gdn_seq_args {
 } shvk_gdn_seq_args;
 /* Token by token in fp32, any storage type: new tokens of live sequences (one, or a few), and the exact tier's form of any length. */
 int shvk_gdn_step(const shvk_gdn_seq_args* a, void* stream);
-/* In chunks of 16 tokens on the tensor cores, dtype bf16 or fp16: prompts and histories.  Outputs and states are those of the rule to
- * float32's accuracy before o is rounded (in a value column, to 2^-34 of the chunk's largest |v - exp(.) S^T k|: what follows a decay
- * to nothing does not show it unless the state before it was 2^34 times larger).  Two launches; `workspace` (device, 16-byte aligned, at least as many bytes as
+/* In chunks of 64 (DV a multiple of 128) or 16 tokens on the tensor cores, dtype bf16 or fp16: prompts and histories.  Outputs and states are those of the rule to
+ * float32's accuracy before o is rounded (in a value column, to 2^-32 of the chunk's largest |v - exp(.) S^T k|: what follows a decay
+ * to nothing does not show it unless the state before it was some 2^20 times larger).  Two launches; `workspace` (device, 16-byte aligned, at least as many bytes as
  * shvk_gdn_prefill_workspace_bytes(a) says, contents irrelevant) holds what the first hands to the second: calls that may overlap need
  * their own.  The size follows from n_seq, n_tokens and HV alone; it is 0 for arguments that the call refuses. */
 size_t shvk_gdn_prefill_workspace_bytes(const shvk_gdn_seq_args* a);
 int shvk_gdn_prefill(const shvk_gdn_seq_args* a, void* workspace, size_t workspace_bytes, void* stream);
+/* Device status word of that call: nonzero after a bounded wait inside a kernel gave up (its outputs are unspecified then). */
+int shvk_gdn_prefill_status(int* status_out);
 
 /* What stands between two blocks, in one pass over rows of D values (1 .. 16384): the norm, gate and scale of a block's output, the
  * residual sum, the norm in front of the next block:

@@ -14,6 +14,7 @@
 // that the walk keeps or finds anew.  On the output's way, where the caller rounds to 16 bits, one piece is enough for bf16 (its step is
 // 2^-8, a piece's 2^-11); for fp16 outputs there are two here as well.  Sums over tokens that last, S = e S + P, are rounded float32 FMAs
 // and not tensor-core accumulations, whose truncation would lean one way for thousands of chunks.
+#include "gdn_pieces.cuh"
 #include "gdn_seq.cuh"
 
 #include <type_traits>
@@ -57,23 +58,6 @@ template <int ROWB> __device__ __forceinline__ uint32_t tile_off(int row, int pi
     constexpr int PER = ROWB / 16;                              // pieces of a row
     if constexpr (PER >= 8) return uint32_t(row * ROWB + ((piece ^ (row & 7)) << 4));
     else return uint32_t(row * ROWB + ((piece ^ ((row / (8 / PER)) & (PER - 1))) << 4));
-}
-
-// 2^n for a biased exponent n + 127 in [1, 254]
-__device__ __forceinline__ float pow2_biased(int b) { return __int_as_float(b << 23); }
-__device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) >> 23) & 255; }
-__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
-
-__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-// x = hi + lo: hi the upper eleven bits (an fp16 as it is), lo the rest rounded to fp16; |x| <= 2^15
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const float xh = __int_as_float(__float_as_int(x) & 0xffffe000), yh = __int_as_float(__float_as_int(y) & 0xffffe000);
-    const float2 r = add2(make_float2(x, y), make_float2(-xh, -yh));
-    hi = pack_half(xh, yh);
-    lo = pack_half(r.x, r.y);
 }
 
 // Chunks of sequence n stand at [start / 16 + n, .. + ceil(length / 16)) of the workspace: never over those of n + 1, for any lengths.
@@ -634,6 +618,7 @@ template <typename T, int DK> int launch_prefill(const shvk_gdn_seq_args& a, uin
 extern "C" size_t shvk_gdn_prefill_workspace_bytes(const shvk_gdn_seq_args* a) {
     using namespace sb;
     if (check_gdn_seq(a) || a->n_seq == 0) return 0;
+    if (a->DV % 128 == 0) return gdn_prefill_tc_workspace(*a);
     return size_t(prefill_chunks(*a)) * size_t(a->HV) * size_t(PW_BYTES);
 }
 
@@ -645,6 +630,7 @@ extern "C" int shvk_gdn_prefill(const shvk_gdn_seq_args* a, void* workspace, siz
     if (!workspace || !aligned16(workspace) || workspace_bytes < shvk_gdn_prefill_workspace_bytes(a)) return int(cudaErrorInvalidValue);
     cudaStream_t s = cudaStream_t(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (a->DV % 128 == 0) return gdn_prefill_tc(*a, ws, s);
     if (a->dtype == DT_BF16) return a->DK == 64 ? launch_prefill<__nv_bfloat16, 64>(*a, ws, s) : launch_prefill<__nv_bfloat16, 128>(*a, ws, s);
     return a->DK == 64 ? launch_prefill<__half, 64>(*a, ws, s) : launch_prefill<__half, 128>(*a, ws, s);
 }
