@@ -9,7 +9,8 @@
 // walk   a CTA per head and 128 value columns.  The values are the 128 lanes of tensor memory: S^T, W^T, U^T and D^T are operands that
 //        lie there as pieces, K, Q, T and M come from shared memory.  The state itself stays in registers: a value column's keys in two
 //        threads (eight warps), rounded by float32 FMAs; per chunk its pieces go to tensor memory and the product K^T D comes back.
-//        One warp issues the products; three bring K and Q (scaled and turned into fp16 on the way), V, T and M, a chunk or two ahead.
+//        Four more warps write the outputs, one issues the products, one brings V, T and M by bulk copies, two K and Q, scaled and turned
+//        into fp16 on the way, a chunk or two ahead.
 //
 // A chunk is a chain: pieces of S -> K S0 -> W -> T W -> D -> K^T D -> S.  Q S0 and M U run beside it, and the outputs of a chunk are
 // written while the next one's first product runs.
@@ -66,13 +67,49 @@ __device__ __forceinline__ int first_chunk(const SeqRows& r, int n) { return r.s
 template <int DK, bool FINE> struct PrepSmem {
     static constexpr int TILES = 2 * CT * DK * 2, IMAGES = Ws<FINE>::BYTES, LP = CT + 4;
     __align__(1024) uint8_t a[TILES > IMAGES ? TILES : IMAGES];  // K and Q as they are, then what leaves
-    __align__(16) float l[CT * LP];
+    __align__(16) float l[CT * LP], x[CT * LP];                  // L and (I + L)^-1
     double cum[CT], low[CT];                                     // cumulative decay, and its least value so far
-    float beta[CT], rk[CT], rq[CT], kk[CT], qq[CT], top[4];
+    float beta[CT], kk[CT], qq[CT], top[4];
+    float row[3][CT], col[CT];                                   // decay of a token since the end of block b; of a block's end since a token
+    float bk[CT], rk[CT], rq[CT];                                // beta / |k|, 1 / |k|, scale / |q| and M's row scale
 };
 
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d += A B of two 16 x 16 blocks (pitch P) in shared memory, to 22 bits: hi and lo are eleven bits each
+template <int P> __device__ __forceinline__ void block_product(float (&d)[2][4], const float* A, const float* B, int g, int t) {
+    auto split = [](float v, uint32_t& hi, uint32_t& lo) {
+        hi = __float_as_uint(v) & 0xffffe000u;
+        lo = __float_as_uint(v - __uint_as_float(hi)) & 0xffffe000u;
+    };
+#pragma unroll
+    for (int k = 0; k < 16; k += 8) {
+        uint32_t ah[4], al[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split(A[(g + 8 * (i & 1)) * P + k + t + 4 * (i >> 1)], ah[i], al[i]);
+#pragma unroll
+        for (int ni = 0; ni < 2; ++ni) {
+            uint32_t bh[2], bl[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) split(B[(k + t + 4 * i) * P + 8 * ni + g], bh[i], bl[i]);
+            mma_tf32(d[ni], al, bh[0], bh[1]);
+            mma_tf32(d[ni], ah, bl[0], bl[1]);
+            mma_tf32(d[ni], ah, bh[0], bh[1]);
+        }
+    }
+}
+template <int P> __device__ __forceinline__ void block_store(float* D, const float (&d)[2][4], float sign, int g, int t) {
+#pragma unroll
+    for (int ni = 0; ni < 2; ++ni)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<float2*>(D + (g + 8 * h) * P + 8 * ni + 2 * t) = make_float2(sign * d[ni][2 * h], sign * d[ni][2 * h + 1]);
+}
+
 template <typename T, int DK>
-__global__ void __launch_bounds__(128) gdn_prefill_tc_prep_kernel(const shvk_gdn_seq_args a, uint8_t* __restrict__ ws) {
+__global__ void __launch_bounds__(128, 3) gdn_prefill_tc_prep_kernel(const shvk_gdn_seq_args a, uint8_t* __restrict__ ws) {
     constexpr bool FINE = std::is_same<T, __half>::value;
     using W = Ws<FINE>;
     using Sm = PrepSmem<DK, FINE>;
@@ -92,20 +129,20 @@ __global__ void __launch_bounds__(128) gdn_prefill_tc_prep_kernel(const shvk_gdn
     const int t0 = rows.start + ahead * CT, left = rows.end - t0;
     uint8_t* kt = sm.a;
     uint8_t* qt = sm.a + CT * DK * 2;
+    const uint32_t k_s = smem_u32(kt), q_s = smem_u32(qt);
     {
         const T* Q = static_cast<const T*>(a.q) + t0 * a.ldq + khead * DK;
         const T* K = static_cast<const T*>(a.k) + t0 * a.ldk + khead * DK;
-        const uint4 z = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < CT * DK / 8 / 128; ++i) {
-            const int v = tid + 128 * i, row = v / (DK / 8), p = v % (DK / 8);
+            const int v = tid + 128 * i, row = v / (DK / 8), p = v % (DK / 8), has = row < left ? 16 : 0;
             const uint32_t off = (p >> 3) * (CT * 128) + sw128(row, p & 7);
-            *reinterpret_cast<uint4*>(kt + off) = row < left ? *reinterpret_cast<const uint4*>(K + row * a.ldk + p * 8) : z;
-            *reinterpret_cast<uint4*>(qt + off) = row < left ? *reinterpret_cast<const uint4*>(Q + row * a.ldq + p * 8) : z;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(k_s + off), "l"(has ? static_cast<const void*>(K + row * a.ldk + p * 8) : ws), "r"(has) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_s + off), "l"(has ? static_cast<const void*>(Q + row * a.ldq + p * 8) : ws), "r"(has) : "memory");
         }
     }
     if (warp == 0) {                                             // cumulative decays in double: their differences are exponents
-        double v[2], m[2];
+        double v[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int tok = 2 * lane + e;
@@ -121,9 +158,7 @@ __global__ void __launch_bounds__(128) gdn_prefill_tc_prep_kernel(const shvk_gdn
         const double until = __shfl_up_sync(0xffffffffu, s, 1);
         v[0] += lane ? until : 0.0;
         v[1] += v[0];
-        m[0] = v[0];
-        m[1] = fmin(v[0], v[1]);
-        double mm = m[1];
+        double mm = fmin(v[0], v[1]);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const double up = __shfl_up_sync(0xffffffffu, mm, o);
@@ -132,12 +167,13 @@ __global__ void __launch_bounds__(128) gdn_prefill_tc_prep_kernel(const shvk_gdn
         const double before = __shfl_up_sync(0xffffffffu, mm, 1);
         sm.cum[2 * lane] = v[0];
         sm.cum[2 * lane + 1] = v[1];
-        sm.low[2 * lane] = lane ? fmin(before, m[0]) : m[0];
-        sm.low[2 * lane + 1] = lane ? fmin(before, m[1]) : m[1];
+        sm.low[2 * lane] = lane ? fmin(before, v[0]) : v[0];
+        sm.low[2 * lane + 1] = lane ? fmin(before, fmin(v[0], v[1])) : fmin(v[0], v[1]);
     } else if (tid >= 64) {
         const int tok = tid - 64;
         sm.beta[tok] = tok < left ? a.beta[(t0 + tok) * a.ldgb + head] : 0.0f;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     // ---------------------------------------------------------------- Gram products of the blocks (bi, bj), bj <= bi; the first is (warp, warp)
     const int g = lane >> 2, t = lane & 3, lm = lane >> 3, lr = lane & 7;
@@ -145,7 +181,6 @@ __global__ void __launch_bounds__(128) gdn_prefill_tc_prep_kernel(const shvk_gdn
     auto bi_of = [&](int b) { return b == 0 ? warp : b == 1 ? (warp == 0 ? 3 : warp == 1 ? 1 : 2) : 3; };
     auto bj_of = [&](int b) { return b == 0 ? warp : b == 1 ? (warp == 3 ? 1 : 0) : warp == 0 ? 1 : 2; };     // w0 00 30 31, w1 11 10 32, w2 22 20, w3 33 21
     float kk[3][2][4] = {}, qk[3][2][4] = {};
-    const uint32_t k_s = smem_u32(kt), q_s = smem_u32(qt);
     {
         float qq[2][4] = {};
 #pragma unroll
@@ -158,11 +193,12 @@ __global__ void __launch_bounds__(128) gdn_prefill_tc_prep_kernel(const shvk_gdn
                 uint32_t ki[4], qi[4], kj[4];
                 ldsm4(q_s + half + sw128(ri, piece), qi);
                 ldsm4(k_s + half + sw128(ri, piece), ki);
-                ldsm4(k_s + half + sw128(rj, piece), kj);
+                if (b > 0) ldsm4(k_s + half + sw128(rj, piece), kj);
 #pragma unroll
                 for (int ni = 0; ni < 2; ++ni) {
-                    mma16<T>(kk[b][ni], ki, kj[ni], kj[ni + 2]);
-                    mma16<T>(qk[b][ni], qi, kj[ni], kj[ni + 2]);
+                    const uint32_t b0 = b > 0 ? kj[ni] : ki[ni], b1 = b > 0 ? kj[ni + 2] : ki[ni + 2];
+                    mma16<T>(kk[b][ni], ki, b0, b1);
+                    mma16<T>(qk[b][ni], qi, b0, b1);
                     if (b == 0) mma16<T>(qq[ni], qi, qi[ni], qi[ni + 2]);
                 }
             }
@@ -178,53 +214,73 @@ __global__ void __launch_bounds__(128) gdn_prefill_tc_prep_kernel(const shvk_gdn
     __syncthreads();                                             // norms are there; K and Q are read
     uint8_t* out = sm.a;
     auto outf = [&](int at) { return reinterpret_cast<float*>(out + at); };
+    const int tok = tid & 63;
+    const double cs = sm.cum[tok], last = sm.cum[CT - 1];
+    const float k2 = sm.kk[tok], rk = a.l2norm ? 1.0f / sqrtf(k2 + 1e-6f) : 1.0f;
+    {
+        const float most = warp_max(rk * sqrtf(k2));             // the longest key (of 32 tokens)
+        if (lane == 0 && warp < 2) sm.top[warp] = most;
+    }
+    // exp(c_i - c_j) of a block below the diagonal is exp(c_i - c_e) exp(c_e - c_j), e the last token of j's block
     if (tid < CT) {
-        const float k2 = sm.kk[tid], rk = a.l2norm ? 1.0f / sqrtf(k2 + 1e-6f) : 1.0f;
-        sm.rk[tid] = rk;
-        const float len = warp_max(rk * sqrtf(k2));
-        if (lane == 0) sm.top[warp] = len;
+        sm.col[tok] = expf(float(sm.cum[tok | 15] - cs));
+        sm.row[0][tok] = expf(float(cs - sm.cum[15]));
+    } else {
+        sm.row[1][tok] = expf(float(cs - sm.cum[31]));
+        sm.row[2][tok] = expf(float(cs - sm.cum[47]));
     }
     __syncthreads();
     if (tid < CT) {
-        const float k2 = sm.kk[tid], q2 = sm.qq[tid], rk = sm.rk[tid];
-        const float rq = a.scale * (a.l2norm ? 1.0f / sqrtf(q2 + 1e-6f) : 1.0f);
-        const double cs = sm.cum[tid], last = sm.cum[CT - 1];
-        const int ke = clampi(exponent_of(sqrtf(k2)), 27, 227), qe = clampi(exponent_of(sqrtf(q2)), 27, 227);
+        const int ke = clampi(exponent_of(sqrtf(k2)), 27, 227);
         const float e = expf(float(cs)), d = expf(float(last - cs)), kap = rk * pow2_biased(ke + 1);     // rk / ks
-        sm.rq[tid] = rq;
-        outf(W::KS)[tid] = pow2_biased(253 - ke);                // |ks k| < 1
-        outf(W::QS)[tid] = pow2_biased(253 - qe);
-        outf(W::ER)[tid] = e * kap;
-        outf(W::EQ)[tid] = e * (rq * pow2_biased(qe + 1));
-        outf(W::DK)[tid] = d * kap;
-        // a row of M is at most |q| |k| times its largest decay
-        const float most = fabsf(rq) * sqrtf(q2) * fmaxf(sm.top[0], sm.top[1]) * expf(float(cs - sm.low[tid]));
-        outf(W::OM)[tid] = pow2_biased(clampi(exponent_of(most), 27, 227) + 1);
+        sm.rk[tok] = rk;
+        sm.bk[tok] = sm.beta[tok] * rk;
+        outf(W::KS)[tok] = pow2_biased(253 - ke);                // |ks k| < 1
+        outf(W::ER)[tok] = e * kap;
+        outf(W::DK)[tok] = d * kap;
         if (tid == 0) *reinterpret_cast<float4*>(out + W::E64) = make_float4(expf(float(last)), 0.0f, 0.0f, 0.0f);
+    } else {
+        const float q2 = sm.qq[tok], rq = a.scale * (a.l2norm ? 1.0f / sqrtf(q2 + 1e-6f) : 1.0f);
+        const int qe = clampi(exponent_of(sqrtf(q2)), 27, 227);
+        outf(W::QS)[tok] = pow2_biased(253 - qe);
+        outf(W::EQ)[tok] = expf(float(cs)) * (rq * pow2_biased(qe + 1));
+        // a row of M is at most |q| |k| times its largest decay
+        const float most = fabsf(rq) * sqrtf(q2) * fmaxf(sm.top[0], sm.top[1]) * expf(float(cs - sm.low[tok]));
+        const int me = clampi(exponent_of(most), 27, 227);
+        outf(W::OM)[tok] = pow2_biased(me + 1);
+        sm.rq[tok] = rq * pow2_biased(253 - me);
     }
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < 3; ++b) {
         if (b >= blocks) break;
+        const int bi = bi_of(b), bj = bj_of(b);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int i = 16 * bi_of(b) + g + 8 * h;
-            const double ci = sm.cum[i];
-            const float bk = sm.beta[i] * sm.rk[i], rq = sm.rq[i] * pow2_biased(254 - exponent_of(outf(W::OM)[i]));
+            const int i = 16 * bi + g + 8 * h;
+            const float since = b > 0 ? sm.row[bj][i] : 1.0f, bk = sm.bk[i] * since, rq = sm.rq[i] * since;
 #pragma unroll
             for (int ni = 0; ni < 2; ++ni) {
-                float m[2];
+                const int j0 = 16 * bj + 8 * ni + 2 * t;
+                float l[2], m[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int j = 16 * bj_of(b) + 8 * ni + 2 * t + e;
-                    const float dcy = j <= i ? expf(float(ci - sm.cum[j])) * sm.rk[j] : 0.0f;
-                    sm.l[i * LP + j] = j < i ? bk * dcy * kk[b][ni][2 * h + e] : 0.0f;
+                    const int j = j0 + e;
+                    const float dcy = sm.rk[j] * (b > 0 ? sm.col[j] : j <= i ? expf(float(sm.cum[i] - sm.cum[j])) : 0.0f);
+                    l[e] = j < i ? bk * dcy * kk[b][ni][2 * h + e] : 0.0f;
                     m[e] = j <= i ? rq * dcy * qk[b][ni][2 * h + e] : 0.0f;
                 }
+                // A product with zeros would carry what is no number to rows in front of its own.  It leaves by the row's beta instead:
+                // T's column, and with it the walk's U, is none from the row itself on.
+                if (!(fabsf(l[0]) + fabsf(l[1]) <= 3.402823466e38f)) {
+                    l[0] = l[1] = 0.0f;
+                    sm.beta[i] = __int_as_float(0x7fffffff);
+                }
+                *reinterpret_cast<float2*>(sm.l + i * LP + j0) = make_float2(l[0], l[1]);
                 uint32_t mh, ml;
-                split_pair(m[0], m[1], mh, ml);
-                const int at = tri_at(i, 16 * bj_of(b) + 8 * ni + 2 * t);
+                const int at = tri_at(i, j0);
                 if (FINE) {
+                    split_pair(m[0], m[1], mh, ml);
                     *reinterpret_cast<uint32_t*>(out + W::M + at) = mh;
                     *reinterpret_cast<uint32_t*>(out + W::ML + at) = ml;
                 } else {
@@ -233,63 +289,66 @@ __global__ void __launch_bounds__(128) gdn_prefill_tc_prep_kernel(const shvk_gdn
             }
         }
     }
-    __syncthreads();
-    // ---------------------------------------------------------------- block column `warp` of (I + L)^-1: column 16 warp + c in lanes c, c + 16
-    {
-        const int c = lane & 15, half = lane >> 4;
-        float x[CT], top = 0.0f;
+    __syncwarp();
+    // ---------------------------------------------------------------- X = (I + L)^-1: the blocks on the diagonal by substitution, a column a lane
+    if (lane < 16) {
+        const float* lrow = sm.l + 16 * warp * (LP + 1);
+        float x[16];
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {                            // rows 16 (warp + d) ..
-            if (warp + d < 4) {
-                const float* lrow = sm.l + 16 * (warp + d) * LP + 16 * warp;
-                float rhs[16];
-                if (d == 0) {
+        for (int i = 0; i < 16; ++i) {
+            float s0 = i == lane ? 1.0f : 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) rhs[r] = r == c ? 1.0f : 0.0f;
-                } else {
-                    float acc[8];
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) {                // this half's eight rows of -sum L x
-                        float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-                        for (int m = 0; m < 16 * d; m += 4) {
-                            const float4 l = *reinterpret_cast<const float4*>(lrow + (8 * half + r) * LP + m);
-                            s0 = fmaf(-l.x, x[m], s0);
-                            s1 = fmaf(-l.y, x[m + 1], s1);
-                            s0 = fmaf(-l.z, x[m + 2], s0);
-                            s1 = fmaf(-l.w, x[m + 3], s1);
-                        }
-                        acc[r] = s0 + s1;
-                    }
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        const float other = __shfl_xor_sync(0xffffffffu, acc[r], 16);
-                        rhs[r] = half ? other : acc[r];
-                        rhs[8 + r] = half ? acc[r] : other;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float s0 = rhs[i], s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < i; j += 4) {
-                        const float4 l = *reinterpret_cast<const float4*>(lrow + i * LP + 16 * d + j);
-                        s0 = fmaf(-l.x, x[16 * d + j], s0);
-                        if (j + 1 < i) s1 = fmaf(-l.y, x[16 * d + j + 1], s1);
-                        if (j + 2 < i) s2 = fmaf(-l.z, x[16 * d + j + 2], s2);
-                        if (j + 3 < i) s3 = fmaf(-l.w, x[16 * d + j + 3], s3);
-                    }
-                    x[16 * d + i] = (s0 + s1) + (s2 + s3);
-                }
+            for (int j = 0; j < i; j += 4) {
+                const float4 l = *reinterpret_cast<const float4*>(lrow + i * LP + j);
+                s0 = fmaf(-l.x, x[j], s0);
+                if (j + 1 < i) s1 = fmaf(-l.y, x[j + 1], s1);
+                if (j + 2 < i) s2 = fmaf(-l.z, x[j + 2], s2);
+                if (j + 3 < i) s3 = fmaf(-l.w, x[j + 3], s3);
             }
+            x[i] = (s0 + s1) + (s2 + s3);
+            sm.x[(16 * warp + i) * LP + 16 * warp + lane] = x[i];
         }
-        const float bc = sm.beta[16 * warp + c];
+    }
+    __syncthreads();
+    // ... then pairs of blocks, X_10 = -X_11 L_10 X_00 and X_32 likewise, then the lower left quarter from the halves on its sides.  A
+    // product's result goes through shared memory: over the L that it used up.
+    auto L = [&](int i, int j) { return sm.l + 16 * (i * LP + j); };
+    auto X = [&](int i, int j) { return sm.x + 16 * (i * LP + j); };
+    if (warp < 2) {
+        const int i = 2 * warp + 1, j = 2 * warp;
+        float y[2][4] = {}, z[2][4] = {};
+        block_product<LP>(y, L(i, j), X(j, j), g, t);
+        __syncwarp();
+        block_store<LP>(L(i, j), y, 1.0f, g, t);
+        __syncwarp();
+        block_product<LP>(z, X(i, i), L(i, j), g, t);
+        block_store<LP>(X(i, j), z, -1.0f, g, t);
+    }
+    __syncthreads();
+    {
+        const int i = 2 + (warp >> 1), j = warp & 1;             // Y = L X of the quarter: Y_i0 = L_i0 X_00 + L_i1 X_10, Y_i1 = L_i1 X_11
+        float y[2][4] = {}, z[2][4] = {};
+        if (j == 0) block_product<LP>(y, L(i, 0), X(0, 0), g, t);
+        block_product<LP>(y, L(i, 1), X(1, j), g, t);
+        __syncthreads();                                         // the quarter of L is read
+        block_store<LP>(L(i, j), y, 1.0f, g, t);
+        __syncthreads();
+        if (i == 3) block_product<LP>(z, X(3, 2), L(2, j), g, t);      // X_ij = -(X_i2 Y_2j + X_i3 Y_3j)
+        block_product<LP>(z, X(i, i), L(i, j), g, t);
+        block_store<LP>(X(i, j), z, -1.0f, g, t);
+    }
+    __syncthreads();
+    {                                                            // T = X diag(beta) in pieces: pairs of columns of the ten blocks, ten a thread
+        float2 v[10];
+        float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < CT; ++i)
-            if (i < 16 * (4 - warp)) {
-                x[i] = i < c ? 0.0f : x[i] * bc;                 // (a beta that is no number stays behind its token)
-                top = fmaxf(top, fabsf(x[i]));
-            }
+        for (int b = 0; b < 10; ++b) {
+            const int bi = b == 0 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, bj = b - bi * (bi + 1) / 2;
+            const int i = 16 * bi + (tid >> 3), j = 16 * bj + 2 * (tid & 7);
+            const float2 x = *reinterpret_cast<const float2*>(sm.x + i * LP + j), bt = *reinterpret_cast<const float2*>(sm.beta + j);
+            v[b] = make_float2(j > i ? 0.0f : x.x * bt.x, j + 1 > i ? 0.0f : x.y * bt.y);
+            top = fmaxf(top, fmaxf(fabsf(v[b].x), fabsf(v[b].y)));
+        }
         top = warp_max(top);
         if (lane == 0) sm.top[warp] = top;
         __syncthreads();
@@ -297,14 +356,12 @@ __global__ void __launch_bounds__(128) gdn_prefill_tc_prep_kernel(const shvk_gdn
         const int te = clampi(exponent_of(top), 27, 227);
         const float sc = pow2_biased(253 - te);
         if (tid == 0) *outf(W::TAU) = pow2_biased(te + 1);
-        uint8_t* at = out + tri_step(warp) + (c >> 3) * 128 + (c & 7) * 2;
 #pragma unroll
-        for (int i = 0; i < CT; ++i)
-            if (i < 16 * (4 - warp) && (i & 1) == half) {
-                const float v = x[i] * sc, vh = __int_as_float(__float_as_int(v) & 0xffffe000);
-                *reinterpret_cast<__half*>(at + W::T + (i >> 3) * 256 + (i & 7) * 16) = __float2half_rn(vh);
-                *reinterpret_cast<__half*>(at + W::TL + (i >> 3) * 256 + (i & 7) * 16) = __float2half_rn(v - vh);
-            }
+        for (int b = 0; b < 10; ++b) {
+            const int bi = b == 0 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, bj = b - bi * (bi + 1) / 2;
+            const int at = tri_at(16 * bi + (tid >> 3), 16 * bj + 2 * (tid & 7));
+            split_pair(v[b].x * sc, v[b].y * sc, *reinterpret_cast<uint32_t*>(out + W::T + at), *reinterpret_cast<uint32_t*>(out + W::TL + at));
+        }
     }
     __syncthreads();
     uint4* dst = reinterpret_cast<uint4*>(ws + ((long long)chunk * a.HV + head) * W::BYTES);
@@ -313,17 +370,19 @@ __global__ void __launch_bounds__(128) gdn_prefill_tc_prep_kernel(const shvk_gdn
 }
 
 // ---------------------------------------------------------------------------------------------------- the walk
-constexpr int COMPUTE = 8, LOADERS = 3, TC_THREADS = 32 * (COMPUTE + 1 + LOADERS);
+// Warps 0-7 the value columns, 8-11 their outputs, 12 the products, 13 bulk copies, 14 and 15 K and Q.
+constexpr int COMPUTE = 8, OUTPUT = 4, CONVERT = 2, WARP_MMA = 12, WARP_COPY = 13, TC_THREADS = 512;
 constexpr uint32_t PREFILL_POLLS = 1u << 22;
 
 template <int DK, bool FINE, int STAGES> struct WalkSmem {
     struct Stage {
-        __align__(1024) uint8_t k[CT * DK * 2], q[CT * DK * 2];  // scaled fp16, halves of 64 keys, 128-byte rows, swizzled
+        __align__(1024) uint8_t kq[2 * CT * DK * 2];             // scaled fp16 by halves of 64 keys: 64 rows of K, 64 rows of Q, 128 bytes each, swizzled
         __align__(1024) uint8_t v[CT * TV * 2];                  // [token][value] as it is
         __align__(1024) uint8_t w[(Ws<FINE>::BYTES + 1023) / 1024 * 1024];
     } st[STAGES];
     __align__(16) float4 meet1[2][TV], meet2[2][TV];             // what the two threads of a value column tell each other
-    __align__(8) uint64_t bars[4 * STAGES + 8];
+    __align__(16) float4 scale[TV];                              // and the thread of its outputs: two factors, the first bad token
+    __align__(8) uint64_t bars[3 * STAGES + 8];
     uint32_t tmem;
     int abort;
 };
@@ -353,12 +412,19 @@ __device__ __forceinline__ void tc_st16(uint32_t t, const uint32_t* r) {
                  ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
                  "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
+__device__ __forceinline__ void tc_st8(uint32_t t, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void pair_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); }
+// registers of a warp group: 512 threads start with 128 each; 2 x 152 + 2 x 104 = 4 x 128
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <typename T, int DK, int STAGES>
 __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(const shvk_gdn_seq_args a, const uint8_t* __restrict__ ws, uint32_t polls) {
@@ -366,7 +432,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
     using W = Ws<FINE>;
     using Sm = WalkSmem<DK, FINE, STAGES>;
     using C = Cols<DK>;
-    constexpr int HALF = CT * 128;                               // bytes of 64 keys of a K or Q tile
+    constexpr int HALF = 2 * CT * 128;                           // bytes of 64 keys of K and Q
     extern __shared__ uint8_t walk_raw[];
     Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(walk_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -385,23 +451,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         return;
     }
     const uint32_t bars = smem_u32(sm.bars);
-    auto full = [&](int s) { return bars + 8u * s; };                                    // K, Q, V of a stage
-    auto wfull = [&](int s) { return bars + 8u * (STAGES + s); };                        // T, M and scalars
+    auto full = [&](int s) { return bars + 8u * s; };                                    // K and Q of a stage
+    auto wfull = [&](int s) { return bars + 8u * (STAGES + s); };                        // V, T, M and scalars
     auto empty = [&](int s) { return bars + 8u * (2 * STAGES + s); };
     const uint32_t b_s = bars + 8u * (3 * STAGES), b_r = b_s + 8, b_w = b_s + 16, b_u = b_s + 24, b_d = b_s + 32, b_p = b_s + 40, b_o = b_s + 48, b_q = b_s + 56;
     if (tid == 0) {
         sm.abort = 0;
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(full(s), 32 * LOADERS);
+            mbar_init(full(s), 32 * CONVERT);
             mbar_init(wfull(s), 1);
-            mbar_init(empty(s), COMPUTE + 1);
+            mbar_init(empty(s), COMPUTE + OUTPUT + 1);
         }
-        mbar_init(b_s, COMPUTE); mbar_init(b_w, COMPUTE); mbar_init(b_d, COMPUTE); mbar_init(b_q, COMPUTE);
+        mbar_init(b_s, COMPUTE); mbar_init(b_w, COMPUTE); mbar_init(b_d, COMPUTE); mbar_init(b_q, OUTPUT);
         mbar_init(b_r, 1); mbar_init(b_u, 1); mbar_init(b_p, 1); mbar_init(b_o, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_proxy_async();
     }
-    if (warp == COMPUTE) {
+    if (warp == WARP_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -418,12 +484,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         if (__any_sync(0xffffffffu, gave_up)) {
             dead = true;
             *abortp = 1;
-            atomicCAS(&g_prefill_status, 0, 1 + (warp < COMPUTE ? 0 : warp == COMPUTE ? 1 : 2));
+            atomicCAS(&g_prefill_status, 0, 1 + (warp < COMPUTE ? 0 : warp < WARP_MMA ? 1 : warp - 10));
         }
     };
+    constexpr float FINITE = 3.402823466e38f;
 
     if (warp < COMPUTE) {
         // ------------------------------------------------------------------------------------------- the value columns
+        regs_up<152>();
         constexpr int KH = DK / 2;                               // keys of a thread
         const int quad = warp & 3, half = warp >> 2, row = 32 * quad + lane;
         const uint32_t tl = tmem + (uint32_t(32 * quad) << 16);
@@ -461,22 +529,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             if (lane == 0) mbar_arrive(b_s);
         };
         give_state();
+        int s = 0;
+        uint32_t sph = 0;
         for (int c = 0; c < NB; ++c) {
-            const int s = c % STAGES;
             const typename Sm::Stage& st = sm.st[s];
-            const uint32_t ph = uint32_t(c) & 1u, sph = uint32_t(c / STAGES) & 1u;
+            const uint32_t ph = uint32_t(c) & 1u;
             const float* sc = reinterpret_cast<const float*>(st.w);
             auto four = [&](int at, int i) { return *reinterpret_cast<const float4*>(sc + at / 4 + 32 * half + i); };
             wait(wfull(s), sph);
-            wait(full(s), sph);
             wait(b_r, ph);
             tc_fence_after();
             // ------------------------------------------------------------------- W = V - e K S0 of this half's 32 tokens
             float x[32], most = 0.0f, sound = 0.0f;
             {
                 const T* v = reinterpret_cast<const T*>(st.v) + 32 * half * TV + row;
-                uint32_t r[32];
-                tc_ld32(tl + C::R + 32 * half, r);
+                tc_ld32(tl + C::R + 32 * half, reinterpret_cast<uint32_t*>(x));
                 tc_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
@@ -484,7 +551,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                     const float e[4] = {er.x, er.y, er.z, er.w};
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        x[i + u] = fmaf(-e[u], __uint_as_float(r[i + u]), to_float(v[(i + u) * TV]) * sig);
+                        x[i + u] = fmaf(-e[u], x[i + u], to_float(v[(i + u) * TV]) * sig);
                         most = fmaxf(most, fabsf(x[i + u]));
                         sound += x[i + u];
                     }
@@ -496,18 +563,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             auto find_bad = [&](const float (&y)[32]) {
 #pragma unroll
                 for (int i = 31; i >= 0; --i)
-                    if (!(fabsf(y[i]) <= 3.402823466e38f)) first = min(first, 32 * half + i);
+                    if (!(fabsf(y[i]) <= FINITE)) first = min(first, 32 * half + i);
             };
             auto cut = [&](float (&y)[32]) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
                     if (32 * half + i >= first) y[i] = 0.0f;
             };
-            if (!(fabsf(sound) <= 3.402823466e38f)) {
+            if (!(fabsf(sound) <= FINITE)) {
                 find_bad(x);
                 most = 0.0f;                                     // of the others: an infinity sets no scale
 #pragma unroll
-                for (int i = 0; i < 32; ++i) most = fmaxf(most, fabsf(x[i]) <= 3.402823466e38f ? fabsf(x[i]) : 0.0f);
+                for (int i = 0; i < 32; ++i) most = fmaxf(most, fabsf(x[i]) <= FINITE ? fabsf(x[i]) : 0.0f);
             }
             sm.meet1[half][row] = make_float4(most, mine, __int_as_float(first), 0.0f);
             pair_sync(quad);
@@ -517,12 +584,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             const float stop = fmaxf(mine, other.y);             // the column's largest |S|
             const int wb = clampi(exponent_of(fmaxf(most, other.x)), 27, 227);
             const float wsc = pow2_biased(261 - wb);             // W within 2^8, so that U, a sum of 64, is within 2^14
-            {
-                uint32_t hi[16], lo[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) split_pair(x[2 * i] * wsc, x[2 * i + 1] * wsc, hi[i], lo[i]);
-                tc_st16(tl + C::P + 16 * half, hi);
-                tc_st16(tl + C::P + 32 + 16 * half, lo);
+            for (int p = 0; p < 2; ++p) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) split_pair(x[16 * p + 2 * i] * wsc, x[16 * p + 2 * i + 1] * wsc, hi[i], lo[i]);
+                tc_st8(tl + C::P + 16 * half + 8 * p, hi);
+                tc_st8(tl + C::P + 32 + 16 * half + 8 * p, lo);
             }
             tc_wait_st();
             tc_fence_before();
@@ -534,19 +602,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             // ------------------------------------------------------------------- D = exp(c_64 - c_j) U, in the state's units
             float sum = 0.0f, f = 1.0f;
             const float e64 = *reinterpret_cast<const float*>(st.w + W::E64);
-            {
-                uint32_t r[32];
-                tc_ld32(tl + C::R + 32 * half, r);
-                tc_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
-            }
+            tc_ld32(tl + C::R + 32 * half, reinterpret_cast<uint32_t*>(x));
+            tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
                 const float4 dk = four(W::DK, i);
                 sum += (fabsf(x[i] * (uf * dk.x)) + fabsf(x[i + 1] * (uf * dk.y))) + (fabsf(x[i + 2] * (uf * dk.z)) + fabsf(x[i + 3] * (uf * dk.w)));
             }
-            if (!(sum <= 3.402823466e38f)) find_bad(x);
+            if (!(sum <= FINITE)) find_bad(x);
             sm.meet2[half][row] = make_float4(sum, __int_as_float(first), 0.0f, 0.0f);
             pair_sync(quad);
             {
@@ -559,34 +622,36 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                     f = pow2_biased(127 + clampi(nb - b, -120, 120));
                 }
             }
+            if (half == 0) sm.scale[row] = make_float4(inv, inv * uf, __int_as_float(first), 0.0f);
             if (first < CT) cut(x);
-            {
-                uint32_t hi[16], lo[16];
+            const float fu = first < CT ? __int_as_float(0x7fffffff) : f * uf;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if (FINE) split_pair(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
-                    else hi[i] = pack_half(x[2 * i], x[2 * i + 1]);
-                }
-                tc_st16(tl + C::R + 32 * half, hi);              // over the U that this warp has read
-                if (FINE) tc_st16(tl + C::R + 32 * half + 16, lo);
-                const float nan = __int_as_float(0x7fffffff), fu = first < CT ? nan : f * uf;
+            for (int p = 0; p < 2; ++p) {
+                uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    const float4 dk = four(W::DK, i);
-                    split_pair(x[i] * (fu * dk.x), x[i + 1] * (fu * dk.y), hi[i / 2], lo[i / 2]);
-                    split_pair(x[i + 2] * (fu * dk.z), x[i + 3] * (fu * dk.w), hi[i / 2 + 1], lo[i / 2 + 1]);
+                for (int i = 0; i < 8; ++i) {
+                    if (FINE) split_pair(x[16 * p + 2 * i], x[16 * p + 2 * i + 1], hi[i], lo[i]);
+                    else hi[i] = pack_half(x[16 * p + 2 * i], x[16 * p + 2 * i + 1]);
                 }
-                tc_st16(tl + C::S + 16 * half, hi);
-                tc_st16(tl + C::S + 32 + 16 * half, lo);
+                tc_st8(tl + C::R + 32 * half + 8 * p, hi);       // over the U that this warp has read
+                if (FINE) tc_st8(tl + C::R + 32 * half + 16 + 8 * p, lo);
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 dk = four(W::DK, 16 * p + i);
+                    split_pair(x[16 * p + i] * (fu * dk.x), x[16 * p + i + 1] * (fu * dk.y), hi[i / 2], lo[i / 2]);
+                    split_pair(x[16 * p + i + 2] * (fu * dk.z), x[16 * p + i + 3] * (fu * dk.w), hi[i / 2 + 1], lo[i / 2 + 1]);
+                }
+                tc_st8(tl + C::S + 16 * half + 8 * p, hi);
+                tc_st8(tl + C::S + 32 + 16 * half + 8 * p, lo);
             }
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(b_d);
+            if (lane == 0) { mbar_arrive(b_d); mbar_arrive(empty(s)); }
             wait(b_p, ph);
             tc_fence_after();
             // ------------------------------------------------------------------- S = e_64 S0 + K^T D
-            const float ef = e64 * f, was = inv;
+            const float ef = e64 * f;
             mine = 0.0f;
 #pragma unroll
             for (int p = 0; p < KH / 32; ++p) {
@@ -604,149 +669,189 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             sig *= f;
             inv = pow2_biased(254 - exponent_of(sig));
             if (c + 1 < NB) give_state();
-            // ------------------------------------------------------------------- O = M U + e Q S0
-            wait(b_o, ph);
-            tc_fence_after();
-            {
-                uint32_t q[32], m[32];
-                tc_ld32(tl + C::QS + 32 * half, q);
-                tc_ld32(tl + C::MU + 32 * half, m);
-                tc_wait_ld();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(b_q);
-                T* o = static_cast<T*>(a.o) + (rows.start + c * CT + 32 * half) * a.ldo + (long long)head * a.DV + split * TV + row;
-                const int left = dead ? 0 : len - c * CT - 32 * half;
-                const float fo = was * uf;
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    const float4 om = four(W::OM, i), eq = four(W::EQ, i);
-                    const float omv[4] = {om.x, om.y, om.z, om.w}, eqv[4] = {eq.x, eq.y, eq.z, eq.w};
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        float y = fmaf(__uint_as_float(m[i + u]) * fo, omv[u], was * (eqv[u] * __uint_as_float(q[i + u])));
-                        if (32 * half + i + u >= first) y = __int_as_float(0x7fffffff);
-                        if (i + u < left) o[(i + u) * a.ldo] = from_float<T>(y);
-                    }
-                }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty(s));
+            if (++s == STAGES) { s = 0; sph ^= 1u; }
         }
         if (out >= 0 && !dead) {
             float* dst = a.states + out * state_of + state_at + (long long)(half * KH) * a.DV + row;
 #pragma unroll
             for (int i = 0; i < KH; ++i) dst[i * (long long)a.DV] = S[i] * inv;
         }
-    } else if (warp == COMPUTE) {
-        // ------------------------------------------------------------------------------------------- the products
+    } else if (warp < COMPUTE + OUTPUT) {
+        // ------------------------------------------------------------------------------------------- O = M U + e Q S0
+        regs_down<104>();
+        const int quad = warp & 3, row = 32 * quad + lane;
+        const uint32_t tl = tmem + (uint32_t(32 * quad) << 16);
+        T* o = static_cast<T*>(a.o) + rows.start * a.ldo + (long long)head * a.DV + split * TV + row;
+        int s = 0;
+        uint32_t sph = 0;
         for (int c = 0; c < NB; ++c) {
-            const int s = c % STAGES;
-            const uint32_t ph = uint32_t(c) & 1u, sph = uint32_t(c / STAGES) & 1u;
-            const uint32_t kt = smem_u32(sm.st[s].k), qt = smem_u32(sm.st[s].q), wt = smem_u32(sm.st[s].w);
-            constexpr uint32_t id64 = idesc_f16(64, false);
-            wait(full(s), sph);
-            wait(b_s, ph);
-            if (c > 0) wait(b_o, ph ^ 1u);                       // M U has read the pieces of U that K S0 overwrites
-            tc_fence_after();
-            if (!dead && elect_one()) {
-#pragma unroll
-                for (int p = 0; p < DK / 16; ++p) {
-                    const uint64_t b = smem_desc_sw128(kt + (p >> 2) * HALF) + uint64_t(2 * (p & 3));
-                    mma_ts(tmem + C::R, tmem + C::S + 8 * p, b, id64, p > 0);
-                    mma_ts(tmem + C::R, tmem + C::S + DK / 2 + 8 * p, b, id64, true);
-                }
-                tc_commit(b_r);
-            }
-            __syncwarp();
-            if (c > 0) wait(b_q, ph ^ 1u);                       // the last chunk's outputs are read
-            tc_fence_after();
-            if (!dead && elect_one()) {
-#pragma unroll
-                for (int p = 0; p < DK / 16; ++p) {
-                    const uint64_t b = smem_desc_sw128(qt + (p >> 2) * HALF) + uint64_t(2 * (p & 3));
-                    mma_ts(tmem + C::QS, tmem + C::S + 8 * p, b, id64, p > 0);
-                    if (FINE) mma_ts(tmem + C::QS, tmem + C::S + DK / 2 + 8 * p, b, id64, true);
-                }
-            }
-            __syncwarp();
+            const typename Sm::Stage& st = sm.st[s];
+            const uint32_t ph = uint32_t(c) & 1u;
+            const float* sc = reinterpret_cast<const float*>(st.w);
             wait(wfull(s), sph);
-            wait(b_w, ph);
-            tc_fence_after();
-            if (!dead && elect_one()) {
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {                 // T is triangular: tokens 16 kk .. reach columns 16 kk .. 63
-                    const uint64_t th = desc_plain(wt + W::T + tri_step(kk), 128, 256), tlo = desc_plain(wt + W::TL + tri_step(kk), 128, 256);
-                    const uint32_t id = idesc_f16(64 - 16 * kk, false), d = tmem + C::R + 16 * kk;
-                    mma_ts(d, tmem + C::P + 8 * kk, th, id, kk > 0);
-                    mma_ts(d, tmem + C::P + 8 * kk, tlo, id, true);
-                    mma_ts(d, tmem + C::P + 32 + 8 * kk, th, id, true);
-                }
-                tc_commit(b_u);
-            }
-            __syncwarp();
             wait(b_d, ph);
+            wait(b_o, ph);
             tc_fence_after();
-            if (!dead && elect_one()) {
-                constexpr uint32_t idk = idesc_f16(DK, true);
+            const float4 mark = sm.scale[row];
+            const int first = __float_as_int(mark.z), left = dead ? 0 : len - c * CT;
+            uint32_t y[CT / 2];                                  // the column's outputs, two to a word
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    const uint64_t b = desc_mn(kt + 2048 * kk, HALF);
-                    mma_ts(tmem + C::P, tmem + C::S + 8 * kk, b, idk, kk > 0);
-                    mma_ts(tmem + C::P, tmem + C::S + 32 + 8 * kk, b, idk, true);
-                }
-                tc_commit(b_p);
+            for (int h = 0; h < 4; ++h) {
+                uint32_t q[16], m[16];
+                tc_ld16(tl + C::QS + 16 * h, q);
+                tc_ld16(tl + C::MU + 16 * h, m);
+                tc_wait_ld();
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    const uint64_t mh = desc_plain(wt + W::M + tri_step(kk), 128, 256);
-                    const uint32_t id = idesc_f16(64 - 16 * kk, false), d = tmem + C::MU + 16 * kk, u = tmem + C::R + 32 * (kk >> 1) + 8 * (kk & 1);
-                    mma_ts(d, u, mh, id, kk > 0);
-                    if (FINE) {
-                        mma_ts(d, u, desc_plain(wt + W::ML + tri_step(kk), 128, 256), id, true);
-                        mma_ts(d, u + 16, mh, id, true);
-                    }
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 om = *reinterpret_cast<const float4*>(sc + W::OM / 4 + 16 * h + i), eq = *reinterpret_cast<const float4*>(sc + W::EQ / 4 + 16 * h + i);
+                    const float omv[4] = {om.x, om.y, om.z, om.w}, eqv[4] = {eq.x, eq.y, eq.z, eq.w};
+                    float x[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        x[u] = fmaf(__uint_as_float(m[i + u]) * mark.y, omv[u], mark.x * (eqv[u] * __uint_as_float(q[i + u])));
+                    if (first < CT)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            if (16 * h + i + u >= first) x[u] = __int_as_float(0x7fffffff);
+                    y[8 * h + i / 2] = pack2<T>(x[0], x[1]);
+                    y[8 * h + i / 2 + 1] = pack2<T>(x[2], x[3]);
                 }
-                tc_commit(b_o);
-                tc_commit(empty(s));
             }
+            tc_fence_before();
             __syncwarp();
+            if (lane == 0) { mbar_arrive(b_q); mbar_arrive(empty(s)); }
+            if (left >= CT) {
+                T* at = o;
+#pragma unroll
+                for (int i = 0; i < CT; ++i) {
+                    *at = reinterpret_cast<const T*>(&y[i >> 1])[i & 1];
+                    at += a.ldo;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < CT; ++i)
+                    if (i < left) o[i * a.ldo] = reinterpret_cast<const T*>(&y[i >> 1])[i & 1];
+            }
+            o += CT * a.ldo;
+            if (++s == STAGES) { s = 0; sph ^= 1u; }
         }
     } else {
-        // ------------------------------------------------------------------------------------------- the operands
-        const int lt = tid - 32 * (COMPUTE + 1);
-        constexpr int NT = 32 * LOADERS, KALL = CT * DK / 8, KN = (KALL + NT - 1) / NT, VALL = CT * TV / 8;
-        const T* Q = static_cast<const T*>(a.q) + rows.start * a.ldq + khead * DK;
-        const T* K = static_cast<const T*>(a.k) + rows.start * a.ldk + khead * DK;
-        const T* V = static_cast<const T*>(a.v) + rows.start * a.ldv + (long long)head * a.DV + split * TV;
-        const uint8_t* src = ws + ((long long)first_chunk(rows, n) * a.HV + head) * W::BYTES;
-        const uint4 z = make_uint4(0, 0, 0, 0);
-        for (int c = 0; c < NB; ++c) {
-            const int s = c % STAGES;
-            typename Sm::Stage& st = sm.st[s];
-            const uint32_t sph = uint32_t(c / STAGES) & 1u;
-            const int left = len - c * CT;
-            uint4 k[KN], q[KN];
+        regs_down<104>();
+        if (warp == WARP_MMA) {
+            // --------------------------------------------------------------------------------------- the products
+            int s = 0;
+            uint32_t sph = 0;
+            for (int c = 0; c < NB; ++c) {
+                const uint32_t ph = uint32_t(c) & 1u;
+                const uint32_t kq = smem_u32(sm.st[s].kq), wt = smem_u32(sm.st[s].w);
+                constexpr uint32_t id64 = idesc_f16(64, false), id128 = idesc_f16(128, false);
+                wait(full(s), sph);
+                wait(b_s, ph);
+                if (c > 0) wait(b_q, ph ^ 1u);                   // the last chunk's outputs are read, M U has read the pieces of U
+                tc_fence_after();
+                if (!dead && elect_one()) {
 #pragma unroll
-            for (int i = 0; i < KN; ++i) {
-                const int x = lt + NT * i, row = x / (DK / 8), p = x % (DK / 8);
-                const bool has = x < KALL && row < left;
-                k[i] = has ? *reinterpret_cast<const uint4*>(K + (c * CT + row) * a.ldk + p * 8) : z;
-                q[i] = has ? *reinterpret_cast<const uint4*>(Q + (c * CT + row) * a.ldq + p * 8) : z;
+                    for (int p = 0; p < DK / 16; ++p) {          // (K S0)^T and (Q S0)^T beside it
+                        const uint64_t b = smem_desc_sw128(kq + (p >> 2) * HALF) + uint64_t(2 * (p & 3));
+                        mma_ts(tmem + C::R, tmem + C::S + 8 * p, b, id128, p > 0);
+                        mma_ts(tmem + C::R, tmem + C::S + DK / 2 + 8 * p, b, FINE ? id128 : id64, true);
+                    }
+                    tc_commit(b_r);
+                }
+                __syncwarp();
+                wait(wfull(s), sph);
+                wait(b_w, ph);
+                tc_fence_after();
+                if (!dead && elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {             // T is triangular: tokens 16 kk .. reach columns 16 kk .. 63
+                        const uint64_t th = desc_plain(wt + W::T + tri_step(kk), 128, 256), tlo = desc_plain(wt + W::TL + tri_step(kk), 128, 256);
+                        const uint32_t id = idesc_f16(64 - 16 * kk, false), d = tmem + C::R + 16 * kk;
+                        mma_ts(d, tmem + C::P + 8 * kk, th, id, kk > 0);
+                        mma_ts(d, tmem + C::P + 8 * kk, tlo, id, true);
+                        mma_ts(d, tmem + C::P + 32 + 8 * kk, th, id, true);
+                    }
+                    tc_commit(b_u);
+                }
+                __syncwarp();
+                wait(b_d, ph);
+                tc_fence_after();
+                if (!dead && elect_one()) {
+                    constexpr uint32_t idk = idesc_f16(DK, true);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint64_t b = desc_mn(kq + 2048 * kk, HALF);
+                        mma_ts(tmem + C::P, tmem + C::S + 8 * kk, b, idk, kk > 0);
+                        mma_ts(tmem + C::P, tmem + C::S + 32 + 8 * kk, b, idk, true);
+                    }
+                    tc_commit(b_p);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint64_t mh = desc_plain(wt + W::M + tri_step(kk), 128, 256);
+                        const uint32_t id = idesc_f16(64 - 16 * kk, false), d = tmem + C::MU + 16 * kk, u = tmem + C::R + 32 * (kk >> 1) + 8 * (kk & 1);
+                        mma_ts(d, u, mh, id, kk > 0);
+                        if (FINE) {
+                            mma_ts(d, u, desc_plain(wt + W::ML + tri_step(kk), 128, 256), id, true);
+                            mma_ts(d, u + 16, mh, id, true);
+                        }
+                    }
+                    tc_commit(b_o);
+                    tc_commit(empty(s));
+                }
+                __syncwarp();
+                if (++s == STAGES) { s = 0; sph ^= 1u; }
             }
-            wait(empty(s), sph ^ 1u);
-            if (lt == 0 && !dead) {
-                mbar_expect_tx(wfull(s), W::BYTES);
-                bulk_load(smem_u32(st.w), src + (long long)c * a.HV * W::BYTES, W::BYTES, wfull(s));
+        } else if (warp == WARP_COPY) {
+            // --------------------------------------------------------------------------------------- V, T, M and scalars
+            const T* V = static_cast<const T*>(a.v) + rows.start * a.ldv + (long long)head * a.DV + split * TV;
+            const uint8_t* src = ws + ((long long)first_chunk(rows, n) * a.HV + head) * W::BYTES;
+            int s = 0;
+            uint32_t sph = 0;
+            for (int c = 0; c < NB; ++c) {
+                typename Sm::Stage& st = sm.st[s];
+                const int left = len - c * CT;
+                wait(empty(s), sph ^ 1u);
+                if (left < CT) {                                 // rows past the sequence are zeros
+                    for (int i = lane; i < (CT - left) * (TV / 8); i += 32) reinterpret_cast<uint4*>(st.v)[left * (TV / 8) + i] = make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+                }
+                if (!dead) {
+                    if (lane == 0) {
+                        mbar_expect_tx(wfull(s), W::BYTES + uint32_t(min(left, CT)) * (TV * 2));
+                        bulk_load(smem_u32(st.w), src + (long long)c * a.HV * W::BYTES, W::BYTES, wfull(s));
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int r = lane + 32 * i;
+                        if (r < left) bulk_load(smem_u32(st.v) + r * (TV * 2), V + (long long)(c * CT + r) * a.ldv, TV * 2, wfull(s));
+                    }
+                }
+                if (++s == STAGES) { s = 0; sph ^= 1u; }
             }
-            for (int x = lt; x < VALL; x += NT) {
-                const int row = x / (TV / 8), p = x % (TV / 8), has = row < left ? 16 : 0;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(st.v) + row * (TV * 2) + p * 16),
-                             "l"(has ? static_cast<const void*>(V + (c * CT + row) * a.ldv + p * 8) : src), "r"(has) : "memory");
-            }
-            wait(wfull(s), sph);
-            const float* ks = reinterpret_cast<const float*>(st.w + W::KS);
-            const float* qs = reinterpret_cast<const float*>(st.w + W::QS);
-            auto turn = [&](uint4 x, float f) {
+        } else {
+            // --------------------------------------------------------------------------------------- K and Q
+            // copied as they are, a chunk ahead, then turned in place: a thread turns what it has copied itself
+            constexpr int NT = 32 * CONVERT, ROWP = DK / 8, STEP = NT / ROWP, PIECES = CT / STEP;
+            const int lt = tid - 32 * (WARP_COPY + 1), p = lt % ROWP, r0 = lt / ROWP;      // piece p of rows r0, r0 + STEP, ...
+            const T* Q = static_cast<const T*>(a.q) + (rows.start + r0) * a.ldq + khead * DK + p * 8;
+            const T* K = static_cast<const T*>(a.k) + (rows.start + r0) * a.ldk + khead * DK + p * 8;
+            auto copy = [&](int c, int s) {
+                const uint32_t base = smem_u32(sm.st[s].kq) + (p >> 3) * HALF;
+                const T* k = K + (long long)c * CT * a.ldk;
+                const T* q = Q + (long long)c * CT * a.ldq;
+#pragma unroll 4
+                for (int i = 0; i < PIECES; ++i) {
+                    const int r = r0 + i * STEP, has = c * CT + r < len ? 16 : 0;
+                    const uint32_t at = base + sw128(r, p & 7);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(has ? static_cast<const void*>(k) : ws), "r"(has) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + CT * 128), "l"(has ? static_cast<const void*>(q) : ws), "r"(has) : "memory");
+                    k += STEP * a.ldk;
+                    q += STEP * a.ldq;
+                }
+            };
+            auto turn = [&](uint4* at, float f) {
+                uint4 x = *at;
                 uint32_t* e = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
@@ -754,19 +859,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                     const float2 v = mul2(make_float2(to_float(two[0]), to_float(two[1])), make_float2(f, f));
                     e[u] = pack_half(v.x, v.y);
                 }
-                return x;
+                *at = x;
             };
-#pragma unroll
-            for (int i = 0; i < KN; ++i) {
-                const int x = lt + NT * i, row = x / (DK / 8), p = x % (DK / 8);
-                if (x >= KALL) break;
-                const uint32_t off = (p >> 3) * HALF + sw128(row, p & 7);
-                *reinterpret_cast<uint4*>(st.k + off) = turn(k[i], ks[row]);
-                *reinterpret_cast<uint4*>(st.q + off) = turn(q[i], qs[row]);
+            int s = 0, sn = 0;                                   // stages of the chunk to turn and of the one to copy
+            uint32_t sph = 0, snph = 0;
+            auto next_copy = [&](int c) {
+                if (c < NB) {
+                    wait(empty(sn), snph ^ 1u);
+                    if (!dead) copy(c, sn);
+                    if (++sn == STAGES) { sn = 0; snph ^= 1u; }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            next_copy(0);
+            for (int c = 0; c < NB; ++c) {
+                typename Sm::Stage& st = sm.st[s];
+                next_copy(c + 1);
+                wait(wfull(s), sph);                             // the scales
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                const float* ks = reinterpret_cast<const float*>(st.w + W::KS) + r0;
+                const float* qs = reinterpret_cast<const float*>(st.w + W::QS) + r0;
+                uint8_t* base = st.kq + (p >> 3) * HALF;
+#pragma unroll 4
+                for (int i = 0; i < PIECES; ++i) {
+                    uint8_t* at = base + sw128(r0 + i * STEP, p & 7);
+                    turn(reinterpret_cast<uint4*>(at), ks[i * STEP]);
+                    turn(reinterpret_cast<uint4*>(at + CT * 128), qs[i * STEP]);
+                }
+                fence_proxy_async();
+                mbar_arrive(full(s));
+                if (++s == STAGES) { s = 0; sph ^= 1u; }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_proxy_async();
-            mbar_arrive(full(s));
         }
     }
     tc_fence_before();
@@ -776,12 +900,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         __syncthreads();
     }
     tc_fence_after();
-    if (warp == COMPUTE) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (warp == WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s) {
     constexpr bool FINE = std::is_same<T, __half>::value;
-    constexpr int STAGES = 2;
+    constexpr int STAGES = 3;
     const long long items = (a.n_tokens / CT + a.n_seq + 1) * a.HV, ctas = (long long)a.n_seq * a.HV * (a.DV / TV);
     if (items > 0x7fffffff || ctas > 0x7fffffff) return int(cudaErrorInvalidValue);
     if (a.n_tokens > 0) {
