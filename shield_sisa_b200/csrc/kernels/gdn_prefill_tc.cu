@@ -35,10 +35,10 @@ __device__ __forceinline__ int tri_at(int i, int j) {
     const int kk = j >> 4, r = i - 16 * kk;
     return tri_step(kk) + (r >> 3) * 256 + ((j >> 3) & 1) * 128 + (r & 7) * 16 + (j & 7) * 2;
 }
-// workspace of a chunk and head: T hi | T lo | M hi | (M lo) | six arrays of 64 floats | e_64, T's scale, two zeros
+// workspace of a chunk and head: T hi | T lo | M hi | (M lo) | six arrays of 64 floats | e_64, T's scale, the largest ER, DK's scale
 template <bool FINE> struct Ws {
     static constexpr int T = 0, TL = TRI_BYTES, M = 2 * TRI_BYTES, ML = 3 * TRI_BYTES, SC = (FINE ? 4 : 3) * TRI_BYTES;
-    static constexpr int ER = SC, EQ = SC + 256, DK = SC + 512, OM = SC + 768, KS = SC + 1024, QS = SC + 1280, E64 = SC + 1536, TAU = SC + 1540;
+    static constexpr int ER = SC, EQ = SC + 256, DK = SC + 512, OM = SC + 768, KS = SC + 1024, QS = SC + 1280, E64 = SC + 1536;
     static constexpr int BYTES = SC + 1552;
 };
 
@@ -71,6 +71,7 @@ template <int DK, bool FINE> struct PrepSmem {
     double cum[CT], low[CT];                                     // cumulative decay, and its least value so far
     float beta[CT], kk[CT], qq[CT], top[4];
     float row[3][CT], col[CT];                                   // decay of a token since the end of block b; of a block's end since a token
+    float erm[2], dkm[2];                                        // the largest ER and DK of 32 tokens
     float bk[CT], rk[CT], rq[CT];                                // beta / |k|, 1 / |k|, scale / |q| and M's row scale
 };
 
@@ -237,8 +238,9 @@ __global__ void __launch_bounds__(128, 3) gdn_prefill_tc_prep_kernel(const shvk_
         sm.bk[tok] = sm.beta[tok] * rk;
         outf(W::KS)[tok] = pow2_biased(253 - ke);                // |ks k| < 1
         outf(W::ER)[tok] = e * kap;
-        outf(W::DK)[tok] = d * kap;
-        if (tid == 0) *reinterpret_cast<float4*>(out + W::E64) = make_float4(expf(float(last)), 0.0f, 0.0f, 0.0f);
+        outf(W::DK)[tok] = d * kap;                              // to be scaled to at most one
+        const float em = warp_max(e * kap <= 3.402823466e38f ? e * kap : 0.0f), dm = warp_max(d * kap);
+        if (lane == 0) { sm.erm[warp] = em; sm.dkm[warp] = dm; }
     } else {
         const float q2 = sm.qq[tok], rq = a.scale * (a.l2norm ? 1.0f / sqrtf(q2 + 1e-6f) : 1.0f);
         const int qe = clampi(exponent_of(sqrtf(q2)), 27, 227);
@@ -355,7 +357,10 @@ __global__ void __launch_bounds__(128, 3) gdn_prefill_tc_prep_kernel(const shvk_
         top = fmaxf(fmaxf(sm.top[0], sm.top[1]), fmaxf(sm.top[2], sm.top[3]));
         const int te = clampi(exponent_of(top), 27, 227);
         const float sc = pow2_biased(253 - te);
-        if (tid == 0) *outf(W::TAU) = pow2_biased(te + 1);
+        if (tid == 0)
+            *reinterpret_cast<float4*>(out + W::E64) = make_float4(expf(float(last)), pow2_biased(te + 1), fmaxf(sm.erm[0], sm.erm[1]),
+                                                                   pow2_biased(clampi(exponent_of(fmaxf(sm.dkm[0], sm.dkm[1])), 27, 227) + 1));
+        if (tid < CT) outf(W::DK)[tid] *= pow2_biased(253 - clampi(exponent_of(fmaxf(sm.dkm[0], sm.dkm[1])), 27, 227));
 #pragma unroll
         for (int b = 0; b < 10; ++b) {
             const int bi = b == 0 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, bj = b - bi * (bi + 1) / 2;
@@ -380,9 +385,9 @@ template <int DK, bool FINE, int STAGES> struct WalkSmem {
         __align__(1024) uint8_t v[CT * TV * 2];                  // [token][value] as it is
         __align__(1024) uint8_t w[(Ws<FINE>::BYTES + 1023) / 1024 * 1024];
     } st[STAGES];
-    __align__(16) float4 meet1[2][TV], meet2[2][TV];             // what the two threads of a value column tell each other
+    __align__(16) float2 meet1[2][TV], meet2[2][TV];             // what the two threads of a value column tell each other
     __align__(16) float4 scale[TV];                              // and the thread of its outputs: two factors, the first bad token
-    __align__(8) uint64_t bars[3 * STAGES + 8];
+    __align__(8) uint64_t bars[3 * STAGES + 9];
     uint32_t tmem;
     int abort;
 };
@@ -393,9 +398,19 @@ template <int DK> struct Cols {
 };
 
 // D[128 x N] (+)= A (tensor memory, fp16) x B (shared memory)
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
+// (issued by the lane that `lead` names, without a branch: the operands stay in uniform registers)
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 e, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t lead, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
+}
+// the largest magnitude of three; not a number if one is none
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 // float32 sums of fp16 products, 128 rows, n columns; the second operand's columns contiguous (`mn`) or its depth
 __host__ __device__ constexpr uint32_t idesc_f16(int n, bool mn) { return (1u << 4) | (mn ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (8u << 24); }
@@ -454,7 +469,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
     auto full = [&](int s) { return bars + 8u * s; };                                    // K and Q of a stage
     auto wfull = [&](int s) { return bars + 8u * (STAGES + s); };                        // V, T, M and scalars
     auto empty = [&](int s) { return bars + 8u * (2 * STAGES + s); };
-    const uint32_t b_s = bars + 8u * (3 * STAGES), b_r = b_s + 8, b_w = b_s + 16, b_u = b_s + 24, b_d = b_s + 32, b_p = b_s + 40, b_o = b_s + 48, b_q = b_s + 56;
+    const uint32_t b_s = bars + 8u * (3 * STAGES), b_r = b_s + 8, b_w = b_s + 16, b_u = b_s + 24, b_d = b_s + 32, b_p = b_s + 40, b_o = b_s + 48, b_q = b_s + 56,
+                   b_m = b_s + 64;
     if (tid == 0) {
         sm.abort = 0;
         for (int s = 0; s < STAGES; ++s) {
@@ -462,7 +478,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             mbar_init(wfull(s), 1);
             mbar_init(empty(s), COMPUTE + OUTPUT + 1);
         }
-        mbar_init(b_s, COMPUTE); mbar_init(b_w, COMPUTE); mbar_init(b_d, COMPUTE); mbar_init(b_q, OUTPUT);
+        mbar_init(b_s, COMPUTE); mbar_init(b_w, COMPUTE); mbar_init(b_d, COMPUTE); mbar_init(b_q, OUTPUT); mbar_init(b_m, COMPUTE / 2);
         mbar_init(b_r, 1); mbar_init(b_u, 1); mbar_init(b_p, 1); mbar_init(b_o, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_proxy_async();
@@ -474,11 +490,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sm.tmem;
+    const uint32_t tmem = sm.tmem;                               // 0: the columns are all there are
     volatile int* abortp = &sm.abort;
     // A role whose wait has given up goes on through its loop without waiting, issuing or writing, so that the barriers among warps are
     // met by all; the others' waits end with the flag.
-    bool dead = false;
+    bool dead = tmem != 0;
+    if (dead && tid == 0) atomicCAS(&g_prefill_status, 0, 8);
     auto wait = [&](uint32_t bar, uint32_t parity) {
         const bool gave_up = !dead && !mbar_wait(bar, parity & 1u, abortp, polls);
         if (__any_sync(0xffffffffu, gave_up)) {
@@ -494,7 +511,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         regs_up<152>();
         constexpr int KH = DK / 2;                               // keys of a thread
         const int quad = warp & 3, half = warp >> 2, row = 32 * quad + lane;
-        const uint32_t tl = tmem + (uint32_t(32 * quad) << 16);
+        const uint32_t tl = uint32_t(32 * quad) << 16;
         float S[KH], sig = 1.0f, inv = 1.0f, mine = 0.0f;       // S in units of inv; mine: the largest |S| here
         {
             const float* src = a.states + (in < 0 ? 0 : in) * state_of + state_at + (long long)(half * KH) * a.DV + row;
@@ -503,7 +520,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 S[i] = in < 0 ? 0.0f : src[i * (long long)a.DV];
                 mine = fmaxf(mine, fabsf(S[i]));
             }
-            sm.meet1[half][row] = make_float4(mine, 0.0f, 0.0f, 0.0f);
+            sm.meet1[half][row] = make_float2(mine, 0.0f);
             pair_sync(quad);
             const float m = fmaxf(mine, sm.meet1[half ^ 1][row].x);
             const int b = m > 0.0f ? clampi(265 - exponent_of(m), 27, 191) : 127;        // m sig in [2^11, 2^12)
@@ -536,59 +553,76 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             const uint32_t ph = uint32_t(c) & 1u;
             const float* sc = reinterpret_cast<const float*>(st.w);
             auto four = [&](int at, int i) { return *reinterpret_cast<const float4*>(sc + at / 4 + 32 * half + i); };
+            float x[32];
+            // What is no number, or none any more, belongs to its own token and those behind it.  It leaves the products, whose zeros would
+            // carry it to tokens in front of it; the column's outputs from there on, and its state, are marked instead.
+            int first = CT;
+            auto clean = [&]() {
+#pragma unroll
+                for (int i = 31; i >= 0; --i)
+                    if (!(fabsf(x[i]) <= FINITE)) {
+                        first = min(first, 32 * half + i);
+                        x[i] = 0.0f;
+                    }
+            };
+            auto largest = [&]() {
+                float m = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) m = max3_nan(m, x[i], x[i + 1]);
+                return m;
+            };
+            // ------------------------------------------------------------------- while K S0 runs: V of this half's 32 tokens, and a bound of W
             wait(wfull(s), sph);
-            wait(b_r, ph);
-            tc_fence_after();
-            // ------------------------------------------------------------------- W = V - e K S0 of this half's 32 tokens
-            float x[32], most = 0.0f, sound = 0.0f;
             {
                 const T* v = reinterpret_cast<const T*>(st.v) + 32 * half * TV + row;
-                tc_ld32(tl + C::R + 32 * half, reinterpret_cast<uint32_t*>(x));
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] = to_float(v[i * TV]);
+            }
+            float vtop = largest();
+            if (!(vtop <= FINITE)) {
+                vtop = 0.0f;                                     // of the others: an infinity sets no scale
+#pragma unroll
+                for (int i = 0; i < 32; ++i) vtop = fmaxf(vtop, fabsf(x[i]) <= FINITE ? fabsf(x[i]) : 0.0f);
+            }
+            sm.meet1[half][row] = make_float2(vtop, mine);
+            pair_sync(quad);
+            const float2 other = sm.meet1[half ^ 1][row];
+            const float4 tail = *reinterpret_cast<const float4*>(st.w + W::E64);     // e_64, T's scale, the largest ER, DK's scale
+            const float e64 = tail.x, stop = fmaxf(mine, other.y);                   // stop: the column's largest |S|
+            // |W| <= |V| + max ER |K'| |S|, |K'| < 1: at most 2^8 in its scale, so that U, a sum of 64, is within 2^14
+            const int wb = clampi(exponent_of(fmaf(fmaxf(vtop, other.x), sig, tail.z * stop * (DK == 64 ? 8.0f : 11.4f))), 27, 227);
+            const float wsc = pow2_biased(261 - wb), uf = pow2_biased(wb - 7) * tail.y;
+            {
+                const float2 vs = make_float2(sig * wsc, sig * wsc);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 v = mul2(make_float2(x[i], x[i + 1]), vs);
+                    x[i] = v.x;
+                    x[i + 1] = v.y;
+                }
+            }
+            wait(b_r, ph);
+            tc_fence_after();
+            // ------------------------------------------------------------------- W = V - e K S0
+            {
+                uint32_t r[32];
+                tc_ld32(tl + C::R + 32 * half, r);
                 tc_wait_ld();
+                const float2 ws2 = make_float2(-wsc, -wsc);
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
                     const float4 er = four(W::ER, i);
-                    const float e[4] = {er.x, er.y, er.z, er.w};
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        x[i + u] = fmaf(-e[u], x[i + u], to_float(v[(i + u) * TV]) * sig);
-                        most = fmaxf(most, fabsf(x[i + u]));
-                        sound += x[i + u];
-                    }
+                    const float2 lo = fma2(mul2(make_float2(er.x, er.y), ws2), make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), make_float2(x[i], x[i + 1]));
+                    const float2 hi = fma2(mul2(make_float2(er.z, er.w), ws2), make_float2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), make_float2(x[i + 2], x[i + 3]));
+                    x[i] = lo.x; x[i + 1] = lo.y; x[i + 2] = hi.x; x[i + 3] = hi.y;
                 }
             }
-            // What is no number, or none any more, belongs to its own token and those behind it, but a product's zeros in front of it
-            // spread it over the whole chunk: a column goes on with zeros from its first bad token on, and is marked from there on.
-            int first = CT;
-            auto find_bad = [&](const float (&y)[32]) {
-#pragma unroll
-                for (int i = 31; i >= 0; --i)
-                    if (!(fabsf(y[i]) <= FINITE)) first = min(first, 32 * half + i);
-            };
-            auto cut = [&](float (&y)[32]) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (32 * half + i >= first) y[i] = 0.0f;
-            };
-            if (!(fabsf(sound) <= FINITE)) {
-                find_bad(x);
-                most = 0.0f;                                     // of the others: an infinity sets no scale
-#pragma unroll
-                for (int i = 0; i < 32; ++i) most = fmaxf(most, fabsf(x[i]) <= FINITE ? fabsf(x[i]) : 0.0f);
-            }
-            sm.meet1[half][row] = make_float4(most, mine, __int_as_float(first), 0.0f);
-            pair_sync(quad);
-            const float4 other = sm.meet1[half ^ 1][row];
-            first = min(first, __float_as_int(other.z));
-            if (first < CT) cut(x);
-            const float stop = fmaxf(mine, other.y);             // the column's largest |S|
-            const int wb = clampi(exponent_of(fmaxf(most, other.x)), 27, 227);
-            const float wsc = pow2_biased(261 - wb);             // W within 2^8, so that U, a sum of 64, is within 2^14
+            if (!(largest() <= FINITE)) clean();
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) split_pair(x[16 * p + 2 * i] * wsc, x[16 * p + 2 * i + 1] * wsc, hi[i], lo[i]);
+                for (int i = 0; i < 8; ++i) split_pair(x[16 * p + 2 * i], x[16 * p + 2 * i + 1], hi[i], lo[i]);
                 tc_st8(tl + C::P + 16 * half + 8 * p, hi);
                 tc_st8(tl + C::P + 32 + 16 * half + 8 * p, lo);
             }
@@ -596,38 +630,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(b_w);
-            const float uf = pow2_biased(wb - 7) * *reinterpret_cast<const float*>(st.w + W::TAU);
             wait(b_u, ph);
             tc_fence_after();
-            // ------------------------------------------------------------------- D = exp(c_64 - c_j) U, in the state's units
-            float sum = 0.0f, f = 1.0f;
-            const float e64 = *reinterpret_cast<const float*>(st.w + W::E64);
+            // ------------------------------------------------------------------- pieces of U, and of D = exp(c_64 - c_j) U
             tc_ld32(tl + C::R + 32 * half, reinterpret_cast<uint32_t*>(x));
             tc_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                const float4 dk = four(W::DK, i);
-                sum += (fabsf(x[i] * (uf * dk.x)) + fabsf(x[i + 1] * (uf * dk.y))) + (fabsf(x[i + 2] * (uf * dk.z)) + fabsf(x[i + 3] * (uf * dk.w)));
-            }
-            if (!(sum <= FINITE)) find_bad(x);
-            sm.meet2[half][row] = make_float4(sum, __int_as_float(first), 0.0f, 0.0f);
-            pair_sync(quad);
-            {
-                const float4 o2 = sm.meet2[half ^ 1][row];
-                first = min(first, __float_as_int(o2.y));
-                const float top = fmaf(e64, stop, sum + o2.x);   // bounds the new |S|: |k| < 1 in its units
-                if (!(top <= 32768.0f && (top >= 512.0f || top == 0.0f))) {
-                    const int b = exponent_of(sig);
-                    const int nb = top > 0.0f ? clampi(b + clampi(138 - exponent_of(top), -100, 100), 27, 191) : b;     // top f in [2^11, 2^12)
-                    f = pow2_biased(127 + clampi(nb - b, -120, 120));
-                }
-            }
-            if (half == 0) sm.scale[row] = make_float4(inv, inv * uf, __int_as_float(first), 0.0f);
-            if (first < CT) cut(x);
-            const float fu = first < CT ? __int_as_float(0x7fffffff) : f * uf;
+            if (!(largest() <= FINITE)) clean();
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 dk = four(W::DK, 16 * p + i);
+                    const float2 d0 = mul2(make_float2(x[16 * p + i], x[16 * p + i + 1]), make_float2(dk.x, dk.y));
+                    const float2 d1 = mul2(make_float2(x[16 * p + i + 2], x[16 * p + i + 3]), make_float2(dk.z, dk.w));
+                    split_pair(d0.x, d0.y, hi[i / 2], lo[i / 2]);
+                    split_pair(d1.x, d1.y, hi[i / 2 + 1], lo[i / 2 + 1]);
+                }
+                tc_st8(tl + C::S + 16 * half + 8 * p, hi);
+                tc_st8(tl + C::S + 32 + 16 * half + 8 * p, lo);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     if (FINE) split_pair(x[16 * p + 2 * i], x[16 * p + 2 * i + 1], hi[i], lo[i]);
@@ -635,23 +656,41 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 }
                 tc_st8(tl + C::R + 32 * half + 8 * p, hi);       // over the U that this warp has read
                 if (FINE) tc_st8(tl + C::R + 32 * half + 16 + 8 * p, lo);
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const float4 dk = four(W::DK, 16 * p + i);
-                    split_pair(x[16 * p + i] * (fu * dk.x), x[16 * p + i + 1] * (fu * dk.y), hi[i / 2], lo[i / 2]);
-                    split_pair(x[16 * p + i + 2] * (fu * dk.z), x[16 * p + i + 3] * (fu * dk.w), hi[i / 2 + 1], lo[i / 2 + 1]);
-                }
-                tc_st8(tl + C::S + 16 * half + 8 * p, hi);
-                tc_st8(tl + C::S + 32 + 16 * half + 8 * p, lo);
             }
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(b_d); mbar_arrive(empty(s)); }
+            if (lane == 0) mbar_arrive(b_d);
+            // ------------------------------------------------------------------- while K^T D runs: a bound of the new state, its scale
+            float sum = 0.0f, f = 1.0f;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const float4 dk = four(W::DK, i);
+                sum = fmaf(fabsf(x[i]), dk.x, fmaf(fabsf(x[i + 1]), dk.y, fmaf(fabsf(x[i + 2]), dk.z, fmaf(fabsf(x[i + 3]), dk.w, sum))));
+            }
+            sm.meet2[half][row] = make_float2(sum, __int_as_float(first));
+            pair_sync(quad);
+            const float du = uf * tail.w;                        // of a unit of K^T D in the state's
+            {
+                const float2 o2 = sm.meet2[half ^ 1][row];
+                first = min(first, __float_as_int(o2.y));
+                const float top = fmaf(e64, stop, du * (sum + o2.x));      // |k| < 1 in its units
+                if (!(top <= 32768.0f && (top >= 512.0f || top == 0.0f))) {
+                    const int b = exponent_of(sig);
+                    const int nb = top > 0.0f ? clampi(b + clampi(138 - exponent_of(top), -100, 100), 27, 191) : b;     // top f in [2^11, 2^12)
+                    f = pow2_biased(127 + clampi(nb - b, -120, 120));
+                }
+            }
+            if (half == 0) sm.scale[row] = make_float4(inv, inv * uf, __int_as_float(first), 0.0f);
+            __syncwarp();
+            if (lane == 0) {
+                if (half == 0) mbar_arrive(b_m);
+                mbar_arrive(empty(s));
+            }
+            const float ef = e64 * f, df = first < CT ? __int_as_float(0x7fffffff) : du * f;
             wait(b_p, ph);
             tc_fence_after();
             // ------------------------------------------------------------------- S = e_64 S0 + K^T D
-            const float ef = e64 * f;
             mine = 0.0f;
 #pragma unroll
             for (int p = 0; p < KH / 32; ++p) {
@@ -660,10 +699,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 tc_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
-                    const float2 v = fma2(make_float2(ef, ef), make_float2(S[32 * p + i], S[32 * p + i + 1]), make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
+                    const float2 u = mul2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), make_float2(df, df));
+                    const float2 v = fma2(make_float2(ef, ef), make_float2(S[32 * p + i], S[32 * p + i + 1]), u);
                     S[32 * p + i] = v.x;
                     S[32 * p + i + 1] = v.y;
-                    mine = fmaxf(mine, fmaxf(fabsf(v.x), fabsf(v.y)));
+                    mine = max3_nan(mine, v.x, v.y);
                 }
             }
             sig *= f;
@@ -680,7 +720,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         // ------------------------------------------------------------------------------------------- O = M U + e Q S0
         regs_down<104>();
         const int quad = warp & 3, row = 32 * quad + lane;
-        const uint32_t tl = tmem + (uint32_t(32 * quad) << 16);
+        const uint32_t tl = uint32_t(32 * quad) << 16;
         T* o = static_cast<T*>(a.o) + rows.start * a.ldo + (long long)head * a.DV + split * TV + row;
         int s = 0;
         uint32_t sph = 0;
@@ -689,7 +729,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             const uint32_t ph = uint32_t(c) & 1u;
             const float* sc = reinterpret_cast<const float*>(st.w);
             wait(wfull(s), sph);
-            wait(b_d, ph);
+            wait(b_m, ph);
             wait(b_o, ph);
             tc_fence_after();
             const float4 mark = sm.scale[row];
@@ -739,6 +779,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         regs_down<104>();
         if (warp == WARP_MMA) {
             // --------------------------------------------------------------------------------------- the products
+            const uint32_t lead = elect_one();
             int s = 0;
             uint32_t sph = 0;
             for (int c = 0; c < NB; ++c) {
@@ -749,56 +790,55 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 wait(b_s, ph);
                 if (c > 0) wait(b_q, ph ^ 1u);                   // the last chunk's outputs are read, M U has read the pieces of U
                 tc_fence_after();
-                if (!dead && elect_one()) {
+                if (!dead) {
+                    const uint64_t b0 = smem_desc_sw128(kq);
 #pragma unroll
                     for (int p = 0; p < DK / 16; ++p) {          // (K S0)^T and (Q S0)^T beside it
-                        const uint64_t b = smem_desc_sw128(kq + (p >> 2) * HALF) + uint64_t(2 * (p & 3));
-                        mma_ts(tmem + C::R, tmem + C::S + 8 * p, b, id128, p > 0);
-                        mma_ts(tmem + C::R, tmem + C::S + DK / 2 + 8 * p, b, FINE ? id128 : id64, true);
+                        const uint64_t b = b0 + uint64_t((p >> 2) * (HALF / 16) + 2 * (p & 3));
+                        mma_ts(lead, C::R, C::S + 8 * p, b, id128, p > 0);
+                        mma_ts(lead, C::R, C::S + DK / 2 + 8 * p, b, FINE ? id128 : id64, true);
                     }
-                    tc_commit(b_r);
+                    commit_if(lead, b_r);
                 }
-                __syncwarp();
                 wait(wfull(s), sph);
                 wait(b_w, ph);
                 tc_fence_after();
-                if (!dead && elect_one()) {
+                if (!dead) {
+                    const uint64_t t0 = desc_plain(wt, 128, 256);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {             // T is triangular: tokens 16 kk .. reach columns 16 kk .. 63
-                        const uint64_t th = desc_plain(wt + W::T + tri_step(kk), 128, 256), tlo = desc_plain(wt + W::TL + tri_step(kk), 128, 256);
-                        const uint32_t id = idesc_f16(64 - 16 * kk, false), d = tmem + C::R + 16 * kk;
-                        mma_ts(d, tmem + C::P + 8 * kk, th, id, kk > 0);
-                        mma_ts(d, tmem + C::P + 8 * kk, tlo, id, true);
-                        mma_ts(d, tmem + C::P + 32 + 8 * kk, th, id, true);
+                        const uint64_t th = t0 + uint64_t((W::T + tri_step(kk)) / 16), tlo = t0 + uint64_t((W::TL + tri_step(kk)) / 16);
+                        const uint32_t id = idesc_f16(64 - 16 * kk, false), d = C::R + 16 * kk;
+                        mma_ts(lead, d, C::P + 8 * kk, th, id, kk > 0);
+                        mma_ts(lead, d, C::P + 8 * kk, tlo, id, true);
+                        mma_ts(lead, d, C::P + 32 + 8 * kk, th, id, true);
                     }
-                    tc_commit(b_u);
+                    commit_if(lead, b_u);
                 }
-                __syncwarp();
                 wait(b_d, ph);
                 tc_fence_after();
-                if (!dead && elect_one()) {
+                if (!dead) {
                     constexpr uint32_t idk = idesc_f16(DK, true);
+                    const uint64_t b0 = desc_mn(kq, HALF), m0 = desc_plain(wt, 128, 256);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
-                        const uint64_t b = desc_mn(kq + 2048 * kk, HALF);
-                        mma_ts(tmem + C::P, tmem + C::S + 8 * kk, b, idk, kk > 0);
-                        mma_ts(tmem + C::P, tmem + C::S + 32 + 8 * kk, b, idk, true);
+                        mma_ts(lead, C::P, C::S + 8 * kk, b0 + uint64_t(128 * kk), idk, kk > 0);
+                        mma_ts(lead, C::P, C::S + 32 + 8 * kk, b0 + uint64_t(128 * kk), idk, true);
                     }
-                    tc_commit(b_p);
+                    commit_if(lead, b_p);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
-                        const uint64_t mh = desc_plain(wt + W::M + tri_step(kk), 128, 256);
-                        const uint32_t id = idesc_f16(64 - 16 * kk, false), d = tmem + C::MU + 16 * kk, u = tmem + C::R + 32 * (kk >> 1) + 8 * (kk & 1);
-                        mma_ts(d, u, mh, id, kk > 0);
+                        const uint64_t mh = m0 + uint64_t((W::M + tri_step(kk)) / 16);
+                        const uint32_t id = idesc_f16(64 - 16 * kk, false), d = C::MU + 16 * kk, u = C::R + 32 * (kk >> 1) + 8 * (kk & 1);
+                        mma_ts(lead, d, u, mh, id, kk > 0);
                         if (FINE) {
-                            mma_ts(d, u, desc_plain(wt + W::ML + tri_step(kk), 128, 256), id, true);
-                            mma_ts(d, u + 16, mh, id, true);
+                            mma_ts(lead, d, u, m0 + uint64_t((W::ML + tri_step(kk)) / 16), id, true);
+                            mma_ts(lead, d, u + 16, mh, id, true);
                         }
                     }
-                    tc_commit(b_o);
-                    tc_commit(empty(s));
+                    commit_if(lead, b_o);
+                    commit_if(lead, empty(s));
                 }
-                __syncwarp();
                 if (++s == STAGES) { s = 0; sph ^= 1u; }
             }
         } else if (warp == WARP_COPY) {
