@@ -16,7 +16,7 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 // x = hi + lo: hi the upper eleven bits (an fp16 as it is), lo the rest rounded to fp16; |x| <= 2^15
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
     const float xh = __int_as_float(__float_as_int(x) & 0xffffe000), yh = __int_as_float(__float_as_int(y) & 0xffffe000);
-    const float2 r = add2(make_float2(x, y), make_float2(-xh, -yh));
+    const float2 r = fma2(make_float2(xh, yh), make_float2(-1.0f, -1.0f), make_float2(x, y));     // exact (packed sums take no sign)
     hi = pack_half(xh, yh);
     lo = pack_half(r.x, r.y);
 }

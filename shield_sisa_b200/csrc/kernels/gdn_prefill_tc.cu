@@ -734,44 +734,36 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             tc_fence_after();
             const float4 mark = sm.scale[row];
             const int first = __float_as_int(mark.z), left = dead ? 0 : len - c * CT;
-            uint32_t y[CT / 2];                                  // the column's outputs, two to a word
-#pragma unroll
+            // sixteen tokens at a time in a loop: the code of a chunk's roles has to fit the instruction cache
+#pragma unroll 1
             for (int h = 0; h < 4; ++h) {
                 uint32_t q[16], m[16];
                 tc_ld16(tl + C::QS + 16 * h, q);
                 tc_ld16(tl + C::MU + 16 * h, m);
                 tc_wait_ld();
+                if (h == 3) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(b_q);
+                }
+                T* at = o + 16 * h * a.ldo;
+                const float* om4 = sc + W::OM / 4 + 16 * h;
+                const float* eq4 = sc + W::EQ / 4 + 16 * h;
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
-                    const float4 om = *reinterpret_cast<const float4*>(sc + W::OM / 4 + 16 * h + i), eq = *reinterpret_cast<const float4*>(sc + W::EQ / 4 + 16 * h + i);
+                    const float4 om = *reinterpret_cast<const float4*>(om4 + i), eq = *reinterpret_cast<const float4*>(eq4 + i);
                     const float omv[4] = {om.x, om.y, om.z, om.w}, eqv[4] = {eq.x, eq.y, eq.z, eq.w};
-                    float x[4];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        x[u] = fmaf(__uint_as_float(m[i + u]) * mark.y, omv[u], mark.x * (eqv[u] * __uint_as_float(q[i + u])));
-                    if (first < CT)
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            if (16 * h + i + u >= first) x[u] = __int_as_float(0x7fffffff);
-                    y[8 * h + i / 2] = pack2<T>(x[0], x[1]);
-                    y[8 * h + i / 2 + 1] = pack2<T>(x[2], x[3]);
+                    for (int u = 0; u < 4; ++u) {
+                        float x = fmaf(__uint_as_float(m[i + u]) * mark.y, omv[u], mark.x * (eqv[u] * __uint_as_float(q[i + u])));
+                        if (16 * h + i + u >= first) x = __int_as_float(0x7fffffff);
+                        if (16 * h + i + u < left) *at = from_float<T>(x);
+                        at += a.ldo;
+                    }
                 }
             }
-            tc_fence_before();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(b_q); mbar_arrive(empty(s)); }
-            if (left >= CT) {
-                T* at = o;
-#pragma unroll
-                for (int i = 0; i < CT; ++i) {
-                    *at = reinterpret_cast<const T*>(&y[i >> 1])[i & 1];
-                    at += a.ldo;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < CT; ++i)
-                    if (i < left) o[i * a.ldo] = reinterpret_cast<const T*>(&y[i >> 1])[i & 1];
-            }
+            if (lane == 0) mbar_arrive(empty(s));
             o += CT * a.ldo;
             if (++s == STAGES) { s = 0; sph ^= 1u; }
         }
@@ -880,7 +872,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 const uint32_t base = smem_u32(sm.st[s].kq) + (p >> 3) * HALF;
                 const T* k = K + (long long)c * CT * a.ldk;
                 const T* q = Q + (long long)c * CT * a.ldq;
-#pragma unroll 4
+#pragma unroll 2
                 for (int i = 0; i < PIECES; ++i) {
                     const int r = r0 + i * STEP, has = c * CT + r < len ? 16 : 0;
                     const uint32_t at = base + sw128(r, p & 7);
@@ -920,7 +912,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 const float* ks = reinterpret_cast<const float*>(st.w + W::KS) + r0;
                 const float* qs = reinterpret_cast<const float*>(st.w + W::QS) + r0;
                 uint8_t* base = st.kq + (p >> 3) * HALF;
-#pragma unroll 4
+#pragma unroll 2
                 for (int i = 0; i < PIECES; ++i) {
                     uint8_t* at = base + sw128(r0 + i * STEP, p & 7);
                     turn(reinterpret_cast<uint4*>(at), ks[i * STEP]);
