@@ -9,14 +9,15 @@
 // walk   a CTA per head and 128 value columns.  The values are the 128 lanes of tensor memory: S^T, W^T, U^T and D^T are operands that
 //        lie there as pieces, K, Q, T and M come from shared memory.  The state itself stays in registers: a value column's keys in two
 //        threads (eight warps), rounded by float32 FMAs; per chunk its pieces go to tensor memory and the product K^T D comes back.
-//        Four more warps write the outputs, one issues the products, one brings V, T and M by bulk copies, two K and Q, scaled and turned
-//        into fp16 on the way, a chunk or two ahead.
+//        Four more warps write the outputs, one issues the products, one the copies (TMA, a chunk or two ahead), two turn K and Q into
+//        scaled fp16 in place.
 //
 // A chunk is a chain: pieces of S -> K S0 -> W -> T W -> D -> K^T D -> S.  Q S0 and M U run beside it, and the outputs of a chunk are
 // written while the next one's first product runs.
 #include "gdn_pieces.cuh"
 #include "gdn_seq.cuh"
 #include "tc_ptx.cuh"
+#include "tma_utils.cuh"
 
 #include <type_traits>
 
@@ -375,9 +376,11 @@ __global__ void __launch_bounds__(128, 3) gdn_prefill_tc_prep_kernel(const shvk_
 }
 
 // ---------------------------------------------------------------------------------------------------- the walk
-// Warps 0-7 the value columns, 8-11 their outputs, 12 the products, 13 bulk copies, 14 and 15 K and Q.
+// Warps 0-7 the value columns, 8-11 their outputs, 12 the products, 13 the copies, 14 and 15 K and Q to fp16.
 constexpr int COMPUTE = 8, OUTPUT = 4, CONVERT = 2, WARP_MMA = 12, WARP_COPY = 13, TC_THREADS = 512;
 constexpr uint32_t PREFILL_POLLS = 1u << 22;
+
+struct WalkMaps { CUtensorMap q, k, v; };                        // 64 rows x 64 columns swizzled, 64 x 128 columns of V as they are
 
 template <int DK, bool FINE, int STAGES> struct WalkSmem {
     struct Stage {
@@ -442,7 +445,7 @@ template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setma
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <typename T, int DK, int STAGES>
-__global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(const shvk_gdn_seq_args a, const uint8_t* __restrict__ ws, uint32_t polls) {
+__global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(const __grid_constant__ WalkMaps maps, const shvk_gdn_seq_args a, const uint8_t* __restrict__ ws, uint32_t polls) {
     constexpr bool FINE = std::is_same<T, __half>::value;
     using W = Ws<FINE>;
     using Sm = WalkSmem<DK, FINE, STAGES>;
@@ -466,8 +469,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         return;
     }
     const uint32_t bars = smem_u32(sm.bars);
-    auto full = [&](int s) { return bars + 8u * s; };                                    // K and Q of a stage
-    auto wfull = [&](int s) { return bars + 8u * (STAGES + s); };                        // V, T, M and scalars
+    auto full = [&](int s) { return bars + 8u * s; };                                    // K and Q of a stage, in fp16
+    auto wfull = [&](int s) { return bars + 8u * (STAGES + s); };                        // all of it, as it is
     auto empty = [&](int s) { return bars + 8u * (2 * STAGES + s); };
     const uint32_t b_s = bars + 8u * (3 * STAGES), b_r = b_s + 8, b_w = b_s + 16, b_u = b_s + 24, b_d = b_s + 32, b_p = b_s + 40, b_o = b_s + 48, b_q = b_s + 56,
                    b_m = b_s + 64;
@@ -578,6 +581,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
 #pragma unroll
                 for (int i = 0; i < 32; ++i) x[i] = to_float(v[i * TV]);
             }
+            if (len - c * CT < CT)                               // rows past the sequence
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (32 * half + i >= len - c * CT) x[i] = 0.0f;
             float vtop = largest();
             if (!(vtop <= FINITE)) {
                 vtop = 0.0f;                                     // of the others: an infinity sets no scale
@@ -834,56 +841,34 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 if (++s == STAGES) { s = 0; sph ^= 1u; }
             }
         } else if (warp == WARP_COPY) {
-            // --------------------------------------------------------------------------------------- V, T, M and scalars
-            const T* V = static_cast<const T*>(a.v) + rows.start * a.ldv + (long long)head * a.DV + split * TV;
+            // --------------------------------------------------------------------------------------- copies
             const uint8_t* src = ws + ((long long)first_chunk(rows, n) * a.HV + head) * W::BYTES;
+            const uint32_t lead = elect_one();
             int s = 0;
             uint32_t sph = 0;
             for (int c = 0; c < NB; ++c) {
-                typename Sm::Stage& st = sm.st[s];
-                const int left = len - c * CT;
+                const uint32_t kq = smem_u32(sm.st[s].kq), vt = smem_u32(sm.st[s].v), wt = smem_u32(sm.st[s].w);
+                const int y = rows.start + c * CT;
                 wait(empty(s), sph ^ 1u);
-                if (left < CT) {                                 // rows past the sequence are zeros
-                    for (int i = lane; i < (CT - left) * (TV / 8); i += 32) reinterpret_cast<uint4*>(st.v)[left * (TV / 8) + i] = make_uint4(0, 0, 0, 0);
-                    __syncwarp();
-                }
-                if (!dead) {
-                    if (lane == 0) {
-                        mbar_expect_tx(wfull(s), W::BYTES + uint32_t(min(left, CT)) * (TV * 2));
-                        bulk_load(smem_u32(st.w), src + (long long)c * a.HV * W::BYTES, W::BYTES, wfull(s));
-                    }
-                    __syncwarp();
+                if (!dead && lead) {                             // rows past the sequence are another's, past the last zeros: both unused
+                    mbar_expect_tx(wfull(s), W::BYTES + 2 * CT * DK * 2 + CT * TV * 2);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int r = lane + 32 * i;
-                        if (r < left) bulk_load(smem_u32(st.v) + r * (TV * 2), V + (long long)(c * CT + r) * a.ldv, TV * 2, wfull(s));
+                    for (int h = 0; h < DK / 64; ++h) {
+                        tma_load_2d(kq + h * HALF, &maps.k, khead * DK + 64 * h, y, wfull(s));
+                        tma_load_2d(kq + h * HALF + CT * 128, &maps.q, khead * DK + 64 * h, y, wfull(s));
                     }
+                    bulk_load(wt, src + (long long)c * a.HV * W::BYTES, W::BYTES, wfull(s));
+                    tma_load_2d(vt, &maps.v, head * a.DV + split * TV, y, wfull(s));
                 }
+                __syncwarp();
                 if (++s == STAGES) { s = 0; sph ^= 1u; }
             }
         } else {
-            // --------------------------------------------------------------------------------------- K and Q
-            // copied as they are, a chunk ahead, then turned in place: a thread turns what it has copied itself
+            // --------------------------------------------------------------------------------------- K and Q to fp16
+            // turned in place, eight pieces of 16 bytes at a time: a thread has the same piece of every STEP-th row
             constexpr int NT = 32 * CONVERT, ROWP = DK / 8, STEP = NT / ROWP, PIECES = CT / STEP;
-            const int lt = tid - 32 * (WARP_COPY + 1), p = lt % ROWP, r0 = lt / ROWP;      // piece p of rows r0, r0 + STEP, ...
-            const T* Q = static_cast<const T*>(a.q) + (rows.start + r0) * a.ldq + khead * DK + p * 8;
-            const T* K = static_cast<const T*>(a.k) + (rows.start + r0) * a.ldk + khead * DK + p * 8;
-            auto copy = [&](int c, int s) {
-                const uint32_t base = smem_u32(sm.st[s].kq) + (p >> 3) * HALF;
-                const T* k = K + (long long)c * CT * a.ldk;
-                const T* q = Q + (long long)c * CT * a.ldq;
-#pragma unroll 2
-                for (int i = 0; i < PIECES; ++i) {
-                    const int r = r0 + i * STEP, has = c * CT + r < len ? 16 : 0;
-                    const uint32_t at = base + sw128(r, p & 7);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(has ? static_cast<const void*>(k) : ws), "r"(has) : "memory");
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + CT * 128), "l"(has ? static_cast<const void*>(q) : ws), "r"(has) : "memory");
-                    k += STEP * a.ldk;
-                    q += STEP * a.ldq;
-                }
-            };
-            auto turn = [&](uint4* at, float f) {
-                uint4 x = *at;
+            const int lt = tid - 32 * (WARP_COPY + 1), p = lt % ROWP, r0 = lt / ROWP;
+            auto turn = [&](uint4 x, float f) {
                 uint32_t* e = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
@@ -891,38 +876,39 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                     const float2 v = mul2(make_float2(to_float(two[0]), to_float(two[1])), make_float2(f, f));
                     e[u] = pack_half(v.x, v.y);
                 }
-                *at = x;
+                return x;
             };
-            int s = 0, sn = 0;                                   // stages of the chunk to turn and of the one to copy
-            uint32_t sph = 0, snph = 0;
-            auto next_copy = [&](int c) {
-                if (c < NB) {
-                    wait(empty(sn), snph ^ 1u);
-                    if (!dead) copy(c, sn);
-                    if (++sn == STAGES) { sn = 0; snph ^= 1u; }
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-            next_copy(0);
+            int s = 0;
+            uint32_t sph = 0;
             for (int c = 0; c < NB; ++c) {
                 typename Sm::Stage& st = sm.st[s];
-                next_copy(c + 1);
-                wait(wfull(s), sph);                             // the scales
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                const int left = len - c * CT;
+                wait(wfull(s), sph);
                 const float* ks = reinterpret_cast<const float*>(st.w + W::KS) + r0;
                 const float* qs = reinterpret_cast<const float*>(st.w + W::QS) + r0;
                 uint8_t* base = st.kq + (p >> 3) * HALF;
-#pragma unroll 2
-                for (int i = 0; i < PIECES; ++i) {
-                    uint8_t* at = base + sw128(r0 + i * STEP, p & 7);
-                    turn(reinterpret_cast<uint4*>(at), ks[i * STEP]);
-                    turn(reinterpret_cast<uint4*>(at + CT * 128), qs[i * STEP]);
+#pragma unroll 1
+                for (int b = 0; b < PIECES; b += 4) {
+                    uint4 k[4], q[4];
+                    uint4* at[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        at[i] = reinterpret_cast<uint4*>(base + sw128(r0 + (b + i) * STEP, p & 7));
+                        k[i] = *at[i];
+                        q[i] = at[i][CT * 128 / 16];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool has = r0 + (b + i) * STEP < left;
+                        const uint4 z = make_uint4(0, 0, 0, 0);
+                        *at[i] = has ? turn(k[i], ks[(b + i) * STEP]) : z;
+                        at[i][CT * 128 / 16] = has ? turn(q[i], qs[(b + i) * STEP]) : z;
+                    }
                 }
                 fence_proxy_async();
                 mbar_arrive(full(s));
                 if (++s == STAGES) { s = 0; sph ^= 1u; }
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
         }
     }
     tc_fence_before();
@@ -951,7 +937,12 @@ template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t*
     static_assert(smem <= 227 * 1024, "the stages fit");
     const cudaError_t e = cudaFuncSetAttribute(gdn_prefill_tc_walk_kernel<T, DK, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return int(e);
-    gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(ctas), TC_THREADS, smem, s>>>(a, ws, PREFILL_POLLS);
+    WalkMaps maps;
+    if (a.n_tokens > 0 && (!tma::make_map_2d(&maps.q, a.q, 2, a.n_tokens, (long long)a.HK * DK, a.ldq, CT, 64, true) ||
+                           !tma::make_map_2d(&maps.k, a.k, 2, a.n_tokens, (long long)a.HK * DK, a.ldk, CT, 64, true) ||
+                           !tma::make_map_2d(&maps.v, a.v, 2, a.n_tokens, (long long)a.HV * a.DV, a.ldv, CT, TV, false)))
+        return int(cudaErrorInvalidValue);
+    gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(ctas), TC_THREADS, smem, s>>>(maps, a, ws, PREFILL_POLLS);
     return int(cudaGetLastError());
 }
 

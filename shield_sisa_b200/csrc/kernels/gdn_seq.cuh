@@ -36,7 +36,9 @@ inline int check_gdn_seq(const shvk_gdn_seq_args* a) {
         if (!a->q || !a->k || !a->v || !a->g || !a->beta || !a->o) return bad;
         if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o)) return bad;
         const long long vec = a->dtype == DT_F32 ? 4 : 8;
-        if (a->ldq < 0 || a->ldk < 0 || a->ldv < 0 || a->ldgb < 0 || a->ldo < (long long)a->HV * a->DV) return bad;
+        const long long kw = (long long)a->HK * a->DK, vw = (long long)a->HV * a->DV, most = 1ll << 32;
+        if (a->ldq < kw || a->ldk < kw || a->ldv < vw || a->ldgb < a->HV || a->ldo < vw) return bad;
+        if (a->ldq > most || a->ldk > most || a->ldv > most || a->ldo > most) return bad;
         if ((a->ldq | a->ldk | a->ldv | a->ldo) % vec) return bad;
     }
     if (a->n_slots < 0 || ((a->slot_in || a->slot_out) && (!a->states || !aligned16(a->states)))) return bad;
