@@ -147,7 +147,7 @@ def prepare(case, seed):
     s.workspace = None
     if case["op"] == "prefill":                                  # memory that a program keeps, one piece for all its layers
         chunks = s.tokens // 64 + n + 1
-        s.workspace = torch.empty(chunks * hv * 36864, dtype=torch.uint8, device="cuda")
+        s.workspace = torch.empty(chunks * hv * 40960, dtype=torch.uint8, device="cuda")
     return s
 
 
