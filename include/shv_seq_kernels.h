@@ -198,9 +198,10 @@ typedef struct shvk_gdn_seq_args {
 int shvk_gdn_step(const shvk_gdn_seq_args* a, void* stream);
 /* In chunks of 64 (DV a multiple of 128) or 16 tokens on the tensor cores, dtype bf16 or fp16: prompts and histories.  Outputs and states are those of the rule to
  * float32's accuracy before o is rounded (in a value column, to 2^-32 of the chunk's largest |v - exp(.) S^T k|: what follows a decay
- * to nothing does not show it unless the state before it was some 2^20 times larger).  Two launches; `workspace` (device, 16-byte aligned, at least as many bytes as
- * shvk_gdn_prefill_workspace_bytes(a) says, contents irrelevant) holds what the first hands to the second: calls that may overlap need
- * their own.  The size follows from n_seq, n_tokens and HV alone; it is 0 for arguments that the call refuses. */
+ * to nothing does not show it unless the state before it was some 2^20 times larger).  Two launches; four where long sequences are too few to fill the GPU and are
+ * walked in segments (by n_seq, n_tokens and the head sizes: a sequence's bits follow from those too).  `workspace` (device, 16-byte
+ * aligned, at least as many bytes as shvk_gdn_prefill_workspace_bytes(a) says, contents irrelevant) holds what they hand on: calls
+ * that may overlap need their own.  Its size follows from the counts, sizes and type; it is 0 for arguments that the call refuses. */
 size_t shvk_gdn_prefill_workspace_bytes(const shvk_gdn_seq_args* a);
 int shvk_gdn_prefill(const shvk_gdn_seq_args* a, void* workspace, size_t workspace_bytes, void* stream);
 /* Device status word of that call: nonzero after a bounded wait inside a kernel gave up (its outputs are unspecified then). */

@@ -13,11 +13,12 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-// x = hi + lo: hi the upper eleven bits (an fp16 as it is), lo the rest rounded to fp16; |x| <= 2^15
+// x = hi + lo, both fp16: 22 bits; |x| <= 2^15.  (hi by a conversion and back, not by a mask: a mask takes the pipe that the conversions
+// wait for.)
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const float xh = __int_as_float(__float_as_int(x) & 0xffffe000), yh = __int_as_float(__float_as_int(y) & 0xffffe000);
-    const float2 r = fma2(make_float2(xh, yh), make_float2(-1.0f, -1.0f), make_float2(x, y));     // exact (packed sums take no sign)
-    hi = pack_half(xh, yh);
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h), r = fma2(f, make_float2(-1.0f, -1.0f), make_float2(x, y));     // exact (packed sums take no sign)
+    hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = pack_half(r.x, r.y);
 }
 

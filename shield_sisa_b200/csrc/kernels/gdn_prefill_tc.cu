@@ -67,8 +67,9 @@ __device__ __forceinline__ int first_chunk(const SeqRows& r, int n) { return r.s
 // ---------------------------------------------------------------------------------------------------- what needs no state
 template <int DK, bool FINE> struct PrepSmem {
     static constexpr int TILES = 2 * CT * DK * 2, IMAGES = Ws<FINE>::BYTES, LP = CT + 4;
-    __align__(1024) uint8_t a[TILES > IMAGES ? TILES : IMAGES];  // K and Q as they are, then what leaves
-    __align__(16) float l[CT * LP], x[CT * LP];                  // L and (I + L)^-1
+    static constexpr int X_AT = (IMAGES + 15) / 16 * 16, BOTH = X_AT + CT * LP * 4;
+    __align__(1024) uint8_t a[TILES > BOTH ? TILES : BOTH];      // K and Q as they are, then what leaves and, behind it, X = (I + L)^-1
+    __align__(16) float l[CT * LP];
     double cum[CT], low[CT];                                     // cumulative decay, and its least value so far
     float beta[CT], kk[CT], qq[CT], top[4];
     float row[3][CT], col[CT];                                   // decay of a token since the end of block b; of a block's end since a token
@@ -110,8 +111,9 @@ template <int P> __device__ __forceinline__ void block_store(float* D, const flo
             *reinterpret_cast<float2*>(D + (g + 8 * h) * P + 8 * ni + 2 * t) = make_float2(sign * d[ni][2 * h], sign * d[ni][2 * h + 1]);
 }
 
+template <typename T> constexpr bool FINE_PREP = std::is_same<T, __half>::value;
 template <typename T, int DK>
-__global__ void __launch_bounds__(128, 3) gdn_prefill_tc_prep_kernel(const shvk_gdn_seq_args a, uint8_t* __restrict__ ws) {
+__global__ void __launch_bounds__(128, FINE_PREP<T> ? 3 : 4) gdn_prefill_tc_prep_kernel(const shvk_gdn_seq_args a, uint8_t* __restrict__ ws) {
     constexpr bool FINE = std::is_same<T, __half>::value;
     using W = Ws<FINE>;
     using Sm = PrepSmem<DK, FINE>;
@@ -131,6 +133,7 @@ __global__ void __launch_bounds__(128, 3) gdn_prefill_tc_prep_kernel(const shvk_
     const int t0 = rows.start + ahead * CT, left = rows.end - t0;
     uint8_t* kt = sm.a;
     uint8_t* qt = sm.a + CT * DK * 2;
+    float* xs = reinterpret_cast<float*>(sm.a + Sm::X_AT);
     const uint32_t k_s = smem_u32(kt), q_s = smem_u32(qt);
     {
         const T* Q = static_cast<const T*>(a.q) + t0 * a.ldq + khead * DK;
@@ -309,14 +312,14 @@ __global__ void __launch_bounds__(128, 3) gdn_prefill_tc_prep_kernel(const shvk_
                 if (j + 3 < i) s3 = fmaf(-l.w, x[j + 3], s3);
             }
             x[i] = (s0 + s1) + (s2 + s3);
-            sm.x[(16 * warp + i) * LP + 16 * warp + lane] = x[i];
+            xs[(16 * warp + i) * LP + 16 * warp + lane] = x[i];
         }
     }
     __syncthreads();
     // ... then pairs of blocks, X_10 = -X_11 L_10 X_00 and X_32 likewise, then the lower left quarter from the halves on its sides.  A
     // product's result goes through shared memory: over the L that it used up.
     auto L = [&](int i, int j) { return sm.l + 16 * (i * LP + j); };
-    auto X = [&](int i, int j) { return sm.x + 16 * (i * LP + j); };
+    auto X = [&](int i, int j) { return xs + 16 * (i * LP + j); };
     if (warp < 2) {
         const int i = 2 * warp + 1, j = 2 * warp;
         float y[2][4] = {}, z[2][4] = {};
@@ -348,7 +351,7 @@ __global__ void __launch_bounds__(128, 3) gdn_prefill_tc_prep_kernel(const shvk_
         for (int b = 0; b < 10; ++b) {
             const int bi = b == 0 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, bj = b - bi * (bi + 1) / 2;
             const int i = 16 * bi + (tid >> 3), j = 16 * bj + 2 * (tid & 7);
-            const float2 x = *reinterpret_cast<const float2*>(sm.x + i * LP + j), bt = *reinterpret_cast<const float2*>(sm.beta + j);
+            const float2 x = *reinterpret_cast<const float2*>(xs + i * LP + j), bt = *reinterpret_cast<const float2*>(sm.beta + j);
             v[b] = make_float2(j > i ? 0.0f : x.x * bt.x, j + 1 > i ? 0.0f : x.y * bt.y);
             top = fmaxf(top, fmaxf(fabsf(v[b].x), fabsf(v[b].y)));
         }
@@ -378,7 +381,18 @@ __global__ void __launch_bounds__(128, 3) gdn_prefill_tc_prep_kernel(const shvk_
 // ---------------------------------------------------------------------------------------------------- the walk
 // Warps 0-7 the value columns, 8-11 their outputs, 12 the products, 13 the copies, 14 and 15 K and Q to fp16.
 constexpr int COMPUTE = 8, OUTPUT = 4, CONVERT = 2, WARP_MMA = 12, WARP_COPY = 13, TC_THREADS = 512;
-constexpr uint32_t PREFILL_POLLS = 1u << 22;
+constexpr uint32_t PREFILL_POLLS = 1u << 17;            // about half a second (4 us a poll)
+
+// A long sequence of few heads is walked in segments of `chunks` chunks side by side.  The state behind a segment is Phi S + X, with S in
+// front of it: pass 1 walks every segment but the last from nothing (X), and from the identity without values (Phi); the first one from
+// its own state, outputs and all.  gdn_prefill_tc_join_kernel makes X of every segment the state behind it, pass 2 walks the others again
+// from there.  Sequence n's segments stand at first_chunk / chunks + n, as its chunks do.
+struct WalkSegments {
+    int chunks, pass;                                            // 0, 0: no segments
+    float* x;                                                    // [segment][head][DK][DV]
+    float* phi;                                                  // [segment][head][column][key]
+};
+__device__ __forceinline__ int first_segment(int first_chunk, int n, int chunks) { return first_chunk / chunks + n; }
 
 struct WalkMaps { CUtensorMap q, k, v; };                        // 64 rows x 64 columns swizzled, 64 x 128 columns of V as they are
 
@@ -388,16 +402,17 @@ template <int DK, bool FINE, int STAGES> struct WalkSmem {
         __align__(1024) uint8_t v[CT * TV * 2];                  // [token][value] as it is
         __align__(1024) uint8_t w[(Ws<FINE>::BYTES + 1023) / 1024 * 1024];
     } st[STAGES];
-    __align__(16) float2 meet1[2][TV], meet2[2][TV];             // what the two threads of a value column tell each other
+    float vtop[2][TV], meet1[2][TV];                             // the chunk's largest |V| of a column; what its two threads tell each other
+    __align__(16) float2 meet2[2][TV];
     __align__(16) float4 scale[TV];                              // and the thread of its outputs: two factors, the first bad token
-    __align__(8) uint64_t bars[3 * STAGES + 9];
+    __align__(8) uint64_t bars[3 * STAGES + 11];
     uint32_t tmem;
     int abort;
 };
 
 // columns of tensor memory
 template <int DK> struct Cols {
-    static constexpr int P = 0, S = DK, R = 2 * DK, QS = 2 * DK + 64, MU = 2 * DK + 128;     // W lies over P, D over S, U and its pieces over R
+    static constexpr int P = 0, S = DK, R = 2 * DK, MU = 2 * DK + 64, QS = 2 * DK + 128;     // W lies over P, D over S, U and its pieces over R; two of QS
 };
 
 // D[128 x N] (+)= A (tensor memory, fp16) x B (shared memory)
@@ -409,6 +424,19 @@ __device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, ui
 __device__ __forceinline__ void commit_if(uint32_t lead, uint32_t bar) {
     asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
 }
+// Waits for a phase of a barrier, at most `polls` times the hardware's own patience; a few instructions, for loops that must stay short.
+__device__ __forceinline__ bool mbar_wait_counted(uint32_t bar, uint32_t parity, uint32_t polls) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, %3;\n"
+        "WAIT_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE_%=;\n\tsub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra WAIT_%=;\n"
+        "DONE_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity), "r"(polls) : "memory");
+    return ok != 0;
+}
+// (A wait names a phase by its parity: no barrier may get two phases ahead of one that still waits.  Every barrier's next phase follows
+// from what its waiters do after the last one, but b_v's, of which there are two.)
+//
 // the largest magnitude of three; not a number if one is none
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float d;
@@ -445,7 +473,7 @@ template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setma
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <typename T, int DK, int STAGES>
-__global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(const __grid_constant__ WalkMaps maps, const shvk_gdn_seq_args a, const uint8_t* __restrict__ ws, uint32_t polls) {
+__global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(const __grid_constant__ WalkMaps maps, const shvk_gdn_seq_args a, const uint8_t* __restrict__ ws, const WalkSegments seg, uint32_t polls) {
     constexpr bool FINE = std::is_same<T, __half>::value;
     using W = Ws<FINE>;
     using Sm = WalkSmem<DK, FINE, STAGES>;
@@ -454,17 +482,40 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
     extern __shared__ uint8_t walk_raw[];
     Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(walk_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int splits = a.DV / TV, split = int(blockIdx.x % unsigned(splits));
-    const int nh = int(blockIdx.x / unsigned(splits)), n = nh / a.HV, head = nh % a.HV, khead = head / (a.HV / a.HK);
+    const int splits = a.DV / TV, kinds = splits + (seg.pass == 1), split = int(blockIdx.x % unsigned(kinds));
+    const int nh = int(blockIdx.x / unsigned(kinds)), head = nh % a.HV, khead = head / (a.HV / a.HK);
+    const bool phi = split == splits;                            // this CTA makes the segment's Phi
+    int n = nh / a.HV, at = 0, segment = 0;
+    if (seg.chunks) {                                            // the last sequence whose first segment is not behind this one
+        segment = n;
+        n = 0;
+        for (int lo = 0, hi = a.n_seq - 1; lo <= hi;) {
+            const int mid = (lo + hi) >> 1;
+            if (first_segment(first_chunk(SeqRows(a.seq_start, mid, int(a.n_tokens)), mid), mid, seg.chunks) <= segment) { n = mid; lo = mid + 1; } else hi = mid - 1;
+        }
+    }
     const SeqRows rows(a.seq_start, n, int(a.n_tokens));
-    const int len = rows.end - rows.start, NB = (len + CT - 1) / CT;
-    const long long in = slot_of(a.slot_in, n, a.n_slots), out = slot_of(a.slot_out, n, a.n_slots);
-    const long long state_at = (long long)head * DK * a.DV + split * TV, state_of = (long long)a.HV * DK * a.DV;
-    if (NB == 0) {                                               // nothing to walk: the state as it is
+    const int all = (rows.end - rows.start + CT - 1) / CT;       // chunks of the sequence; here: NB of them from chunk c0 on
+    if (seg.chunks) at = segment - first_segment(first_chunk(rows, n), n, seg.chunks);
+    const int c0 = at * seg.chunks, NB = seg.chunks ? min(all - c0, seg.chunks) : all;
+    const bool last = c0 + NB >= all;
+    if (at < 0 || (at > 0 && NB <= 0)) return;                   // no segment of any sequence stands here
+    if (seg.pass == 1 && ((at > 0 && last) || (at == 0 && phi))) return;
+    if (seg.pass == 2 && at == 0) return;
+    const int start = rows.start + c0 * CT, len = rows.end - start;
+    const bool writes = seg.pass != 1 || at == 0;                // outputs
+    const long long in = at == 0 ? slot_of(a.slot_in, n, a.n_slots) : -1, out = last ? slot_of(a.slot_out, n, a.n_slots) : -1;
+    const long long state_of = (long long)a.HV * DK * a.DV, state_at = (long long)head * DK * a.DV + split * TV;
+    // where the state comes from and goes to: columns to_c apart, keys to_k
+    const float* from = in >= 0 ? a.states + in * state_of + state_at : seg.pass == 2 ? seg.x + (segment - 1) * state_of + state_at : nullptr;
+    float* to = last ? (out >= 0 ? a.states + out * state_of + state_at : nullptr) : phi ? seg.phi + ((long long)segment * a.HV + head) * DK * DK
+                : seg.pass == 1 ? seg.x + segment * state_of + state_at : nullptr;
+    const long long to_k = phi ? 1 : a.DV, to_c = phi ? DK : 1;
+    if (NB <= 0) {                                               // nothing to walk: the state as it is
         if (out >= 0 && out != in)
             for (int i = tid; i < DK * TV; i += TC_THREADS) {
-                const long long at = state_at + (i / TV) * (long long)a.DV + i % TV;
-                a.states[out * state_of + at] = in < 0 ? 0.0f : a.states[in * state_of + at];
+                const long long e = (i / TV) * (long long)a.DV + i % TV;
+                to[e] = from ? from[e] : 0.0f;
             }
         return;
     }
@@ -473,7 +524,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
     auto wfull = [&](int s) { return bars + 8u * (STAGES + s); };                        // all of it, as it is
     auto empty = [&](int s) { return bars + 8u * (2 * STAGES + s); };
     const uint32_t b_s = bars + 8u * (3 * STAGES), b_r = b_s + 8, b_w = b_s + 16, b_u = b_s + 24, b_d = b_s + 32, b_p = b_s + 40, b_o = b_s + 48, b_q = b_s + 56,
-                   b_m = b_s + 64;
+                   b_m = b_s + 64, b_v = b_s + 72;
     if (tid == 0) {
         sm.abort = 0;
         for (int s = 0; s < STAGES; ++s) {
@@ -481,7 +532,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             mbar_init(wfull(s), 1);
             mbar_init(empty(s), COMPUTE + OUTPUT + 1);
         }
-        mbar_init(b_s, COMPUTE); mbar_init(b_w, COMPUTE); mbar_init(b_d, COMPUTE); mbar_init(b_q, OUTPUT); mbar_init(b_m, COMPUTE / 2);
+        mbar_init(b_s, COMPUTE); mbar_init(b_w, COMPUTE); mbar_init(b_d, COMPUTE); mbar_init(b_q, OUTPUT); mbar_init(b_v, OUTPUT); mbar_init(b_v + 8, OUTPUT); mbar_init(b_m, COMPUTE / 2);
         mbar_init(b_r, 1); mbar_init(b_u, 1); mbar_init(b_p, 1); mbar_init(b_o, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_proxy_async();
@@ -494,16 +545,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem;                               // 0: the columns are all there are
-    volatile int* abortp = &sm.abort;
     // A role whose wait has given up goes on through its loop without waiting, issuing or writing, so that the barriers among warps are
-    // met by all; the others' waits end with the flag.
+    // met by all; those that wait for it give up in turn.
     bool dead = tmem != 0;
     if (dead && tid == 0) atomicCAS(&g_prefill_status, 0, 8);
     auto wait = [&](uint32_t bar, uint32_t parity) {
-        const bool gave_up = !dead && !mbar_wait(bar, parity & 1u, abortp, polls);
-        if (__any_sync(0xffffffffu, gave_up)) {
+        if (__any_sync(0xffffffffu, !mbar_wait_counted(bar, parity & 1u, polls))) {
             dead = true;
-            *abortp = 1;
+            polls = 1;
+            sm.abort = 1;
             atomicCAS(&g_prefill_status, 0, 1 + (warp < COMPUTE ? 0 : warp < WARP_MMA ? 1 : warp - 10));
         }
     };
@@ -517,15 +567,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         const uint32_t tl = uint32_t(32 * quad) << 16;
         float S[KH], sig = 1.0f, inv = 1.0f, mine = 0.0f;       // S in units of inv; mine: the largest |S| here
         {
-            const float* src = a.states + (in < 0 ? 0 : in) * state_of + state_at + (long long)(half * KH) * a.DV + row;
+            const float* src = from + (long long)(half * KH) * a.DV + row;
 #pragma unroll
             for (int i = 0; i < KH; ++i) {
-                S[i] = in < 0 ? 0.0f : src[i * (long long)a.DV];
+                S[i] = from ? src[i * (long long)a.DV] : phi && row == half * KH + i ? 1.0f : 0.0f;
                 mine = fmaxf(mine, fabsf(S[i]));
             }
-            sm.meet1[half][row] = make_float2(mine, 0.0f);
+            sm.meet1[half][row] = mine;
             pair_sync(quad);
-            const float m = fmaxf(mine, sm.meet1[half ^ 1][row].x);
+            const float m = fmaxf(mine, sm.meet1[half ^ 1][row]);
             const int b = m > 0.0f ? clampi(265 - exponent_of(m), 27, 191) : 127;        // m sig in [2^11, 2^12)
             sig = pow2_biased(b);
             inv = pow2_biased(254 - b);
@@ -534,7 +584,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             mine *= sig;
             pair_sync(quad);                                     // meet1 is read
         }
-        auto give_state = [&]() {                                // pieces of S to tensor memory
+        int s = 0;
+        uint32_t sph = 0;
+#pragma unroll 1
+        for (int c = 0; c < NB; ++c) {
+            const typename Sm::Stage& st = sm.st[s];
+            const uint32_t ph = uint32_t(c) & 1u;
+            const float* sc = reinterpret_cast<const float*>(st.w);
+            // ------------------------------------------------------------------- pieces of S
 #pragma unroll
             for (int p = 0; p < KH / 32; ++p) {
                 uint32_t hi[16], lo[16];
@@ -547,89 +604,59 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(b_s);
-        };
-        give_state();
-        int s = 0;
-        uint32_t sph = 0;
-        for (int c = 0; c < NB; ++c) {
-            const typename Sm::Stage& st = sm.st[s];
-            const uint32_t ph = uint32_t(c) & 1u;
-            const float* sc = reinterpret_cast<const float*>(st.w);
-            auto four = [&](int at, int i) { return *reinterpret_cast<const float4*>(sc + at / 4 + 32 * half + i); };
-            float x[32];
             // What is no number, or none any more, belongs to its own token and those behind it.  It leaves the products, whose zeros would
             // carry it to tokens in front of it; the column's outputs from there on, and its state, are marked instead.
             int first = CT;
-            auto clean = [&]() {
-#pragma unroll
-                for (int i = 31; i >= 0; --i)
-                    if (!(fabsf(x[i]) <= FINITE)) {
-                        first = min(first, 32 * half + i);
-                        x[i] = 0.0f;
-                    }
-            };
-            auto largest = [&]() {
+            auto clean = [&](float (&x)[16], int p) {
                 float m = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) m = max3_nan(m, x[i], x[i + 1]);
-                return m;
+                for (int i = 0; i < 16; i += 2) m = max3_nan(m, x[i], x[i + 1]);
+                if (!(m <= FINITE))
+#pragma unroll
+                    for (int i = 15; i >= 0; --i)
+                        if (!(fabsf(x[i]) <= FINITE)) {
+                            first = min(first, 32 * half + 16 * p + i);
+                            x[i] = 0.0f;
+                        }
             };
-            // ------------------------------------------------------------------- while K S0 runs: V of this half's 32 tokens, and a bound of W
+            // ------------------------------------------------------------------- while K S0 runs: a bound of W
             wait(wfull(s), sph);
-            {
-                const T* v = reinterpret_cast<const T*>(st.v) + 32 * half * TV + row;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) x[i] = to_float(v[i * TV]);
-            }
-            if (len - c * CT < CT)                               // rows past the sequence
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (32 * half + i >= len - c * CT) x[i] = 0.0f;
-            float vtop = largest();
-            if (!(vtop <= FINITE)) {
-                vtop = 0.0f;                                     // of the others: an infinity sets no scale
-#pragma unroll
-                for (int i = 0; i < 32; ++i) vtop = fmaxf(vtop, fabsf(x[i]) <= FINITE ? fabsf(x[i]) : 0.0f);
-            }
-            sm.meet1[half][row] = make_float2(vtop, mine);
+            wait(full(s), sph);                                  // (V's rows past the sequence are cleared with K and Q)
+            wait(b_v + 8 * ph, uint32_t(c >> 1));
+            const T* v = reinterpret_cast<const T*>(st.v) + 32 * half * TV + row;
+            sm.meet1[half][row] = mine;
             pair_sync(quad);
-            const float2 other = sm.meet1[half ^ 1][row];
+            const float vtop = sm.vtop[ph][row], stop = fmaxf(mine, sm.meet1[half ^ 1][row]);      // stop: the column's largest |S|
             const float4 tail = *reinterpret_cast<const float4*>(st.w + W::E64);     // e_64, T's scale, the largest ER, DK's scale
-            const float e64 = tail.x, stop = fmaxf(mine, other.y);                   // stop: the column's largest |S|
+            const float e64 = tail.x;
             // |W| <= |V| + max ER |K'| |S|, |K'| < 1: at most 2^8 in its scale, so that U, a sum of 64, is within 2^14
-            const int wb = clampi(exponent_of(fmaf(fmaxf(vtop, other.x), sig, tail.z * stop * (DK == 64 ? 8.0f : 11.4f))), 27, 227);
+            // (not below 2^-55: the product of two scales, sig up to 2^64, has to stay finite)
+            const int wb = clampi(exponent_of(fmaf(vtop, sig, tail.z * stop * (DK == 64 ? 8.0f : 11.4f))), 72, 227);
             const float wsc = pow2_biased(261 - wb), uf = pow2_biased(wb - 7) * tail.y;
-            {
-                const float2 vs = make_float2(sig * wsc, sig * wsc);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 v = mul2(make_float2(x[i], x[i + 1]), vs);
-                    x[i] = v.x;
-                    x[i + 1] = v.y;
-                }
-            }
             wait(b_r, ph);
             tc_fence_after();
             // ------------------------------------------------------------------- W = V - e K S0
-            {
-                uint32_t r[32];
-                tc_ld32(tl + C::R + 32 * half, r);
-                tc_wait_ld();
-                const float2 ws2 = make_float2(-wsc, -wsc);
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    const float4 er = four(W::ER, i);
-                    const float2 lo = fma2(mul2(make_float2(er.x, er.y), ws2), make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), make_float2(x[i], x[i + 1]));
-                    const float2 hi = fma2(mul2(make_float2(er.z, er.w), ws2), make_float2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), make_float2(x[i + 2], x[i + 3]));
-                    x[i] = lo.x; x[i + 1] = lo.y; x[i + 2] = hi.x; x[i + 3] = hi.y;
-                }
-            }
-            if (!(largest() <= FINITE)) clean();
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-                uint32_t hi[8], lo[8];
+                uint32_t r[16], hi[8], lo[8];
+                tc_ld16(tl + C::R + 32 * half + 16 * p, r);
+                float x[16];
+                const float vs = sig * wsc;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) split_pair(x[16 * p + 2 * i], x[16 * p + 2 * i + 1], hi[i], lo[i]);
+                for (int i = 0; i < 16; ++i) x[i] = to_float(v[(16 * p + i) * TV]) * vs;
+                const float2 ws2 = make_float2(-wsc, -wsc);
+                const float4* er4 = reinterpret_cast<const float4*>(sc + W::ER / 4 + 32 * half + 16 * p);
+                tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 er = er4[i / 4];
+                    const float2 a0 = fma2(mul2(make_float2(er.x, er.y), ws2), make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), make_float2(x[i], x[i + 1]));
+                    const float2 a1 = fma2(mul2(make_float2(er.z, er.w), ws2), make_float2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), make_float2(x[i + 2], x[i + 3]));
+                    x[i] = a0.x; x[i + 1] = a0.y; x[i + 2] = a1.x; x[i + 3] = a1.y;
+                }
+                clean(x, p);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) split_pair(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
                 tc_st8(tl + C::P + 16 * half + 8 * p, hi);
                 tc_st8(tl + C::P + 32 + 16 * half + 8 * p, lo);
             }
@@ -640,41 +667,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             wait(b_u, ph);
             tc_fence_after();
             // ------------------------------------------------------------------- pieces of U, and of D = exp(c_64 - c_j) U
-            tc_ld32(tl + C::R + 32 * half, reinterpret_cast<uint32_t*>(x));
-            tc_wait_ld();
-            if (!(largest() <= FINITE)) clean();
+            float sum = 0.0f, f = 1.0f;
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
+                float x[16];
                 uint32_t hi[8], lo[8];
+                tc_ld16(tl + C::R + 32 * half + 16 * p, reinterpret_cast<uint32_t*>(x));
+                const float4* dk4 = reinterpret_cast<const float4*>(sc + W::DK / 4 + 32 * half + 16 * p);
+                tc_wait_ld();
+                clean(x, p);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (FINE) split_pair(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+                    else hi[i] = pack_half(x[2 * i], x[2 * i + 1]);
+                }
+                tc_st8(tl + C::R + 32 * half + 16 * p, hi);      // over the U that this round has read
+                if (FINE) tc_st8(tl + C::R + 32 * half + 16 * p + 8, lo);
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
-                    const float4 dk = four(W::DK, 16 * p + i);
-                    const float2 d0 = mul2(make_float2(x[16 * p + i], x[16 * p + i + 1]), make_float2(dk.x, dk.y));
-                    const float2 d1 = mul2(make_float2(x[16 * p + i + 2], x[16 * p + i + 3]), make_float2(dk.z, dk.w));
+                    const float4 dk = dk4[i / 4];
+                    const float2 d0 = mul2(make_float2(x[i], x[i + 1]), make_float2(dk.x, dk.y)), d1 = mul2(make_float2(x[i + 2], x[i + 3]), make_float2(dk.z, dk.w));
+                    sum += (fabsf(d0.x) + fabsf(d0.y)) + (fabsf(d1.x) + fabsf(d1.y));
                     split_pair(d0.x, d0.y, hi[i / 2], lo[i / 2]);
                     split_pair(d1.x, d1.y, hi[i / 2 + 1], lo[i / 2 + 1]);
                 }
                 tc_st8(tl + C::S + 16 * half + 8 * p, hi);
                 tc_st8(tl + C::S + 32 + 16 * half + 8 * p, lo);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (FINE) split_pair(x[16 * p + 2 * i], x[16 * p + 2 * i + 1], hi[i], lo[i]);
-                    else hi[i] = pack_half(x[16 * p + 2 * i], x[16 * p + 2 * i + 1]);
-                }
-                tc_st8(tl + C::R + 32 * half + 8 * p, hi);       // over the U that this warp has read
-                if (FINE) tc_st8(tl + C::R + 32 * half + 16 + 8 * p, lo);
             }
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(b_d);
             // ------------------------------------------------------------------- while K^T D runs: a bound of the new state, its scale
-            float sum = 0.0f, f = 1.0f;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                const float4 dk = four(W::DK, i);
-                sum = fmaf(fabsf(x[i]), dk.x, fmaf(fabsf(x[i + 1]), dk.y, fmaf(fabsf(x[i + 2]), dk.z, fmaf(fabsf(x[i + 3]), dk.w, sum))));
-            }
             sm.meet2[half][row] = make_float2(sum, __int_as_float(first));
             pair_sync(quad);
             const float du = uf * tail.w;                        // of a unit of K^T D in the state's
@@ -688,6 +712,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                     f = pow2_biased(127 + clampi(nb - b, -120, 120));
                 }
             }
+            wait(b_q, ph ^ 1u);                       // the last chunk's outputs have read theirs
             if (half == 0) sm.scale[row] = make_float4(inv, inv * uf, __int_as_float(first), 0.0f);
             __syncwarp();
             if (lane == 0) {
@@ -699,53 +724,73 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             tc_fence_after();
             // ------------------------------------------------------------------- S = e_64 S0 + K^T D
             mine = 0.0f;
+            {
+                uint32_t r[KH];
 #pragma unroll
-            for (int p = 0; p < KH / 32; ++p) {
-                uint32_t r[32];
-                tc_ld32(tl + C::P + half * KH + 32 * p, r);
+                for (int p = 0; p < KH / 32; ++p) tc_ld32(tl + C::P + half * KH + 32 * p, r + 32 * p);
                 tc_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
+                for (int i = 0; i < KH; i += 2) {
                     const float2 u = mul2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), make_float2(df, df));
-                    const float2 v = fma2(make_float2(ef, ef), make_float2(S[32 * p + i], S[32 * p + i + 1]), u);
-                    S[32 * p + i] = v.x;
-                    S[32 * p + i + 1] = v.y;
-                    mine = max3_nan(mine, v.x, v.y);
+                    const float2 w = fma2(make_float2(ef, ef), make_float2(S[i], S[i + 1]), u);
+                    S[i] = w.x;
+                    S[i + 1] = w.y;
+                    mine = max3_nan(mine, w.x, w.y);
                 }
             }
             sig *= f;
             inv = pow2_biased(254 - exponent_of(sig));
-            if (c + 1 < NB) give_state();
             if (++s == STAGES) { s = 0; sph ^= 1u; }
         }
-        if (out >= 0 && !dead) {
-            float* dst = a.states + out * state_of + state_at + (long long)(half * KH) * a.DV + row;
+        if (to && !dead && (!phi || row < DK)) {
+            float* dst = to + (half * KH) * to_k + row * to_c;
 #pragma unroll
-            for (int i = 0; i < KH; ++i) dst[i * (long long)a.DV] = S[i] * inv;
+            for (int i = 0; i < KH; ++i) dst[i * to_k] = S[i] * inv;
         }
     } else if (warp < COMPUTE + OUTPUT) {
         // ------------------------------------------------------------------------------------------- O = M U + e Q S0
         regs_down<104>();
         const int quad = warp & 3, row = 32 * quad + lane;
         const uint32_t tl = uint32_t(32 * quad) << 16;
-        T* o = static_cast<T*>(a.o) + rows.start * a.ldo + (long long)head * a.DV + split * TV + row;
-        int s = 0;
-        uint32_t sph = 0;
+        T* o = static_cast<T*>(a.o) + start * a.ldo + (long long)head * a.DV + split * TV + row;
+        int s = 0, sn = 0;                                       // stages of the chunk to write and of the next one
+        uint32_t sph = 0, snph = 0;
+        auto next_top = [&](int c) {                             // the largest |V| of chunk c: what W will be scaled by (an infinity sets no scale)
+            if (c >= NB) return;
+            wait(wfull(sn), snph);
+            wait(full(sn), snph);
+            const T* v = reinterpret_cast<const T*>(sm.st[sn].v) + row;
+            float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll 1
+            for (int p = 0; p < CT; p += 16)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float y0 = fabsf(to_float(v[(p + i) * TV])), y1 = fabsf(to_float(v[(p + i + 1) * TV]));
+                    m0 = fmaxf(m0, y0 <= FINITE ? y0 : 0.0f);
+                    m1 = fmaxf(m1, y1 <= FINITE ? y1 : 0.0f);
+                }
+            sm.vtop[c & 1][row] = fmaxf(m0, m1);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_v + 8 * (c & 1));     // (two barriers: this may be a chunk ahead of those that wait)
+            if (++sn == STAGES) { sn = 0; snph ^= 1u; }
+        };
+        next_top(0);
+#pragma unroll 1
         for (int c = 0; c < NB; ++c) {
             const typename Sm::Stage& st = sm.st[s];
             const uint32_t ph = uint32_t(c) & 1u;
             const float* sc = reinterpret_cast<const float*>(st.w);
-            wait(wfull(s), sph);
+            next_top(c + 1);
             wait(b_m, ph);
             wait(b_o, ph);
             tc_fence_after();
             const float4 mark = sm.scale[row];
-            const int first = __float_as_int(mark.z), left = dead ? 0 : len - c * CT;
+            const int first = __float_as_int(mark.z), left = dead || !writes ? 0 : len - c * CT;
             // sixteen tokens at a time in a loop: the code of a chunk's roles has to fit the instruction cache
 #pragma unroll 1
             for (int h = 0; h < 4; ++h) {
                 uint32_t q[16], m[16];
-                tc_ld16(tl + C::QS + 16 * h, q);
+                tc_ld16(tl + C::QS + 64 * ph + 16 * h, q);
                 tc_ld16(tl + C::MU + 16 * h, m);
                 tc_wait_ld();
                 if (h == 3) {
@@ -779,25 +824,30 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         if (warp == WARP_MMA) {
             // --------------------------------------------------------------------------------------- the products
             const uint32_t lead = elect_one();
-            int s = 0;
-            uint32_t sph = 0;
-            for (int c = 0; c < NB; ++c) {
+            auto products = [&](int c, int s, uint32_t sph) {
                 const uint32_t ph = uint32_t(c) & 1u;
                 const uint32_t kq = smem_u32(sm.st[s].kq), wt = smem_u32(sm.st[s].w);
-                constexpr uint32_t id64 = idesc_f16(64, false), id128 = idesc_f16(128, false);
+                constexpr uint32_t id64 = idesc_f16(64, false);
                 wait(full(s), sph);
+                wait(b_o, ph ^ 1u);                              // M U has read the pieces of U, which K S0 overwrites
                 wait(b_s, ph);
-                if (c > 0) wait(b_q, ph ^ 1u);                   // the last chunk's outputs are read, M U has read the pieces of U
                 tc_fence_after();
+                const uint32_t qs = C::QS + 64 * ph;             // (read by the outputs of chunk c - 2 before M U of chunk c - 1 was let in)
                 if (!dead) {
                     const uint64_t b0 = smem_desc_sw128(kq);
 #pragma unroll
-                    for (int p = 0; p < DK / 16; ++p) {          // (K S0)^T and (Q S0)^T beside it
+                    for (int p = 0; p < DK / 16; ++p) {          // (K S0)^T, for which the chain waits
                         const uint64_t b = b0 + uint64_t((p >> 2) * (HALF / 16) + 2 * (p & 3));
-                        mma_ts(lead, C::R, C::S + 8 * p, b, id128, p > 0);
-                        mma_ts(lead, C::R, C::S + DK / 2 + 8 * p, b, FINE ? id128 : id64, true);
+                        mma_ts(lead, C::R, C::S + 8 * p, b, id64, p > 0);
+                        mma_ts(lead, C::R, C::S + DK / 2 + 8 * p, b, id64, true);
                     }
                     commit_if(lead, b_r);
+#pragma unroll
+                    for (int p = 0; p < DK / 16; ++p) {          // (Q S0)^T
+                        const uint64_t b = b0 + uint64_t((p >> 2) * (HALF / 16) + 2 * (p & 3) + CT * 128 / 16);
+                        mma_ts(lead, qs, C::S + 8 * p, b, id64, p > 0);
+                        if (FINE) mma_ts(lead, qs, C::S + DK / 2 + 8 * p, b, id64, true);
+                    }
                 }
                 wait(wfull(s), sph);
                 wait(b_w, ph);
@@ -818,37 +868,49 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 tc_fence_after();
                 if (!dead) {
                     constexpr uint32_t idk = idesc_f16(DK, true);
-                    const uint64_t b0 = desc_mn(kq, HALF), m0 = desc_plain(wt, 128, 256);
+                    const uint64_t b0 = desc_mn(kq, HALF);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
                         mma_ts(lead, C::P, C::S + 8 * kk, b0 + uint64_t(128 * kk), idk, kk > 0);
                         mma_ts(lead, C::P, C::S + 32 + 8 * kk, b0 + uint64_t(128 * kk), idk, true);
                     }
                     commit_if(lead, b_p);
+                }
+                wait(b_q, ph ^ 1u);                   // the last chunk's outputs are read
+                tc_fence_after();
+                if (!dead) {
+                    const uint64_t m0 = desc_plain(wt, 128, 256);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
                         const uint64_t mh = m0 + uint64_t((W::M + tri_step(kk)) / 16);
-                        const uint32_t id = idesc_f16(64 - 16 * kk, false), d = C::MU + 16 * kk, u = C::R + 32 * (kk >> 1) + 8 * (kk & 1);
+                        const uint32_t id = idesc_f16(64 - 16 * kk, false), d = C::MU + 16 * kk, u = C::R + 16 * kk;
                         mma_ts(lead, d, u, mh, id, kk > 0);
                         if (FINE) {
                             mma_ts(lead, d, u, m0 + uint64_t((W::ML + tri_step(kk)) / 16), id, true);
-                            mma_ts(lead, d, u + 16, mh, id, true);
+                            mma_ts(lead, d, u + 8, mh, id, true);
                         }
                     }
                     commit_if(lead, b_o);
                     commit_if(lead, empty(s));
                 }
-                if (++s == STAGES) { s = 0; sph ^= 1u; }
-            }
+            };
+            // (a stage's addresses have to be constants: computed, they cost every product a move to a uniform register, 30 of 65 cycles)
+            uint32_t sph = 0;
+#pragma unroll 1
+            for (int c0 = 0; c0 < NB; c0 += STAGES, sph ^= 1u)
+#pragma unroll
+                for (int s = 0; s < STAGES; ++s)
+                    if (c0 + s < NB) products(c0 + s, s, sph);
         } else if (warp == WARP_COPY) {
             // --------------------------------------------------------------------------------------- copies
-            const uint8_t* src = ws + ((long long)first_chunk(rows, n) * a.HV + head) * W::BYTES;
+            const uint8_t* src = ws + ((long long)(first_chunk(rows, n) + c0) * a.HV + head) * W::BYTES;
             const uint32_t lead = elect_one();
             int s = 0;
             uint32_t sph = 0;
-            for (int c = 0; c < NB; ++c) {
+    #pragma unroll 1
+        for (int c = 0; c < NB; ++c) {
                 const uint32_t kq = smem_u32(sm.st[s].kq), vt = smem_u32(sm.st[s].v), wt = smem_u32(sm.st[s].w);
-                const int y = rows.start + c * CT;
+                const int y = start + c * CT;
                 wait(empty(s), sph ^ 1u);
                 if (!dead && lead) {                             // rows past the sequence are another's, past the last zeros: both unused
                     mbar_expect_tx(wfull(s), W::BYTES + 2 * CT * DK * 2 + CT * TV * 2);
@@ -858,7 +920,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                         tma_load_2d(kq + h * HALF + CT * 128, &maps.q, khead * DK + 64 * h, y, wfull(s));
                     }
                     bulk_load(wt, src + (long long)c * a.HV * W::BYTES, W::BYTES, wfull(s));
-                    tma_load_2d(vt, &maps.v, head * a.DV + split * TV, y, wfull(s));
+                    tma_load_2d(vt, &maps.v, head * a.DV + (phi ? 0 : split * TV), y, wfull(s));
                 }
                 __syncwarp();
                 if (++s == STAGES) { s = 0; sph ^= 1u; }
@@ -880,7 +942,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             };
             int s = 0;
             uint32_t sph = 0;
-            for (int c = 0; c < NB; ++c) {
+    #pragma unroll 1
+        for (int c = 0; c < NB; ++c) {
                 typename Sm::Stage& st = sm.st[s];
                 const int left = len - c * CT;
                 wait(wfull(s), sph);
@@ -905,6 +968,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                         at[i][CT * 128 / 16] = has ? turn(q[i], qs[(b + i) * STEP]) : z;
                     }
                 }
+                if (left < CT || phi)                            // (Phi has no values)
+                    for (int i = (phi ? 0 : left * (TV / 8)) + lt; i < CT * (TV / 8); i += NT) reinterpret_cast<uint4*>(st.v)[i] = make_uint4(0, 0, 0, 0);
                 fence_proxy_async();
                 mbar_arrive(full(s));
                 if (++s == STAGES) { s = 0; sph ^= 1u; }
@@ -913,7 +978,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
     }
     tc_fence_before();
     __syncthreads();
-    if (*abortp) {                                               // products may still be on their way: a millisecond is a thousand times theirs
+    if (sm.abort) {                                               // products may still be on their way: a millisecond is a thousand times theirs
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
         __syncthreads();
     }
@@ -921,35 +986,112 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
     if (warp == WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
+// X of segment g becomes Phi_g X_(g-1) + X_g, g = 1 .. the last but one, in float32: a CTA takes JC columns of a head through all segments
+// of a sequence, the state so far in shared memory.
+constexpr int JC = 8, JOIN_THREADS = 256;
+template <int DK> __global__ void __launch_bounds__(JOIN_THREADS) gdn_prefill_tc_join_kernel(const shvk_gdn_seq_args a, const WalkSegments seg) {
+    constexpr int GROUPS = JOIN_THREADS / DK, CPT = JC / GROUPS;      // a thread: one key, CPT columns
+    __shared__ __align__(16) float s[2][DK][JC];
+    const int parts = a.DV / JC, part = int(blockIdx.x % unsigned(parts)), nh = int(blockIdx.x / unsigned(parts)), n = nh / a.HV, head = nh % a.HV;
+    const SeqRows rows(a.seq_start, n, int(a.n_tokens));
+    const int segments = ((rows.end - rows.start + CT - 1) / CT + seg.chunks - 1) / seg.chunks;
+    if (segments < 3) return;
+    const int key = threadIdx.x % DK, c = threadIdx.x / DK * CPT;
+    const long long first = first_segment(first_chunk(rows, n), n, seg.chunks), state_of = (long long)a.HV * DK * a.DV;
+    float* x = seg.x + first * state_of + ((long long)head * DK + key) * a.DV + part * JC + c;
+    const float* phi = seg.phi + (first * a.HV + head) * DK * DK + key;
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) s[0][key][c + u] = x[u];
+    for (int g = 1; g < segments - 1; ++g) {
+        x += state_of;
+        phi += (long long)a.HV * DK * DK;
+        float acc[CPT];
+#pragma unroll
+        for (int u = 0; u < CPT; ++u) acc[u] = x[u];
+        __syncthreads();
+        const float (*now)[JC] = s[(g - 1) & 1];
+#pragma unroll 16
+        for (int k = 0; k < DK; ++k) {
+            const float p = phi[k * DK];
+#pragma unroll
+            for (int u = 0; u < CPT; ++u) acc[u] = fmaf(p, now[k][c + u], acc[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < CPT; ++u) {
+            x[u] = acc[u];
+            s[g & 1][key][c + u] = acc[u];
+        }
+    }
+}
+
+// Chunks of a segment, 0 where sequences are walked whole.  Counted in chunks' times of one wave of CTAs (a walk's chunk takes 7,200 cycles,
+// a join's segment about 2,000, the two launches more about as much as two chunks) for sequences of the average length; segments are not
+// shorter than 13 chunks, so that their states take less room than their chunks' T and M.
+inline int segment_chunks(const shvk_gdn_seq_args& a) {
+    const long long sms = device_sms(), splits = a.DV / TV, heads = (long long)a.n_seq * a.HV, chunks = a.n_tokens / CT / a.n_seq;
+    auto waves = [&](long long ctas) { return (ctas + sms - 1) / sms; };
+    double best = 0.9 * double(chunks * waves(heads * splits));
+    int found = 0;
+    for (long long g = 2; g <= 64 && (chunks + g - 1) / g >= 13; ++g) {
+        const long long len = (chunks + g - 1) / g;
+        const double t = double(len * (waves(heads * (splits + (g - 2) * (splits + 1))) + waves(heads * splits * (g - 1)))) + 0.3 * double(g - 2) + 2.0;
+        if (t < best) { best = t; found = int(len); }
+    }
+    return found;
+}
+inline long long segment_count(const shvk_gdn_seq_args& a, int chunks) { return (a.n_tokens / CT + a.n_seq + 1) / chunks + a.n_seq + 1; }
+inline size_t chunk_bytes(const shvk_gdn_seq_args& a) {
+    const size_t each = a.dtype == DT_F16 ? Ws<true>::BYTES : Ws<false>::BYTES;
+    return (size_t(a.n_tokens / CT + a.n_seq + 1) * size_t(a.HV) * each + 15) / 16 * 16;
+}
+
 template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s) {
     constexpr bool FINE = std::is_same<T, __half>::value;
     constexpr int STAGES = 3;
-    const long long items = (a.n_tokens / CT + a.n_seq + 1) * a.HV, ctas = (long long)a.n_seq * a.HV * (a.DV / TV);
+    const int chunks = segment_chunks(a);
+    const long long segments = chunks ? segment_count(a, chunks) : 0, splits = a.DV / TV;
+    const long long items = (a.n_tokens / CT + a.n_seq + 1) * a.HV, ctas = (chunks ? segments : a.n_seq) * a.HV * (splits + (chunks ? 1 : 0));
     if (items > 0x7fffffff || ctas > 0x7fffffff) return int(cudaErrorInvalidValue);
+    cudaError_t e;
     if (a.n_tokens > 0) {
         constexpr int smem = int(sizeof(PrepSmem<DK, FINE>)) + 1024;
-        const cudaError_t e = cudaFuncSetAttribute(gdn_prefill_tc_prep_kernel<T, DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        e = cudaFuncSetAttribute(gdn_prefill_tc_prep_kernel<T, DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return int(e);
         gdn_prefill_tc_prep_kernel<T, DK><<<unsigned(items), 128, smem, s>>>(a, ws);
-        if (const cudaError_t le = cudaGetLastError(); le != cudaSuccess) return int(le);
+        if ((e = cudaGetLastError()) != cudaSuccess) return int(e);
     }
     constexpr int smem = int(sizeof(WalkSmem<DK, FINE, STAGES>)) + 1024;
     static_assert(smem <= 227 * 1024, "the stages fit");
-    const cudaError_t e = cudaFuncSetAttribute(gdn_prefill_tc_walk_kernel<T, DK, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(gdn_prefill_tc_walk_kernel<T, DK, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return int(e);
     WalkMaps maps;
     if (a.n_tokens > 0 && (!tma::make_map_2d(&maps.q, a.q, 2, a.n_tokens, (long long)a.HK * DK, a.ldq, CT, 64, true) ||
                            !tma::make_map_2d(&maps.k, a.k, 2, a.n_tokens, (long long)a.HK * DK, a.ldk, CT, 64, true) ||
                            !tma::make_map_2d(&maps.v, a.v, 2, a.n_tokens, (long long)a.HV * a.DV, a.ldv, CT, TV, false)))
         return int(cudaErrorInvalidValue);
-    gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(ctas), TC_THREADS, smem, s>>>(maps, a, ws, PREFILL_POLLS);
+    WalkSegments seg{};
+    if (!chunks) {
+        gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(ctas), TC_THREADS, smem, s>>>(maps, a, ws, seg, PREFILL_POLLS);
+        return int(cudaGetLastError());
+    }
+    seg.chunks = chunks;
+    seg.x = reinterpret_cast<float*>(ws + chunk_bytes(a));
+    seg.phi = seg.x + segments * a.HV * DK * a.DV;
+    seg.pass = 1;
+    gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(ctas), TC_THREADS, smem, s>>>(maps, a, ws, seg, PREFILL_POLLS);
+    if ((e = cudaGetLastError()) != cudaSuccess) return int(e);
+    gdn_prefill_tc_join_kernel<DK><<<unsigned((long long)a.n_seq * a.HV * (a.DV / JC)), JOIN_THREADS, 0, s>>>(a, seg);
+    if ((e = cudaGetLastError()) != cudaSuccess) return int(e);
+    seg.pass = 2;
+    gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(segments * a.HV * splits), TC_THREADS, smem, s>>>(maps, a, ws, seg, PREFILL_POLLS);
     return int(cudaGetLastError());
 }
 
 }  // namespace
 
 size_t gdn_prefill_tc_workspace(const shvk_gdn_seq_args& a) {
-    return size_t(a.n_tokens / CT + a.n_seq + 1) * size_t(a.HV) * size_t(a.dtype == DT_F16 ? Ws<true>::BYTES : Ws<false>::BYTES);
+    const int chunks = segment_chunks(a);
+    return chunk_bytes(a) + (chunks ? size_t(segment_count(a, chunks)) * size_t(a.HV) * size_t(a.DK) * size_t(a.DK + a.DV) * sizeof(float) : 0);
 }
 int gdn_prefill_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s) {
     if (a.dtype == DT_BF16) return a.DK == 64 ? launch_tc<__nv_bfloat16, 64>(a, ws, s) : launch_tc<__nv_bfloat16, 128>(a, ws, s);

@@ -272,7 +272,7 @@ def test_prefill_of_few_and_many_sequences(L, n):
 
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "fp16"])
-@pytest.mark.parametrize("what", ["tiny_values", "huge_values", "huge_state", "tiny_state", "rising", "falling", "large_keys", "small_keys", "no_decay"])
+@pytest.mark.parametrize("what", ["tiny_values", "huge_values", "huge_state", "tiny_state", "rising", "falling", "vanishing", "large_keys", "small_keys", "no_decay"])
 def test_prefill_of_any_size_of_numbers(L, kind, what):
     """The scales of the pieces follow the numbers: a state or values far from one, that grow or fade by many powers of two on the way,
     keys and queries that are normalised from far away."""
@@ -295,6 +295,9 @@ def test_prefill_of_any_size_of_numbers(L, kind, what):
     elif what == "falling":
         x["v"] = (x["v"].float() * torch.exp(4 - at / 25)).to(t)
         x["g"] -= 0.2
+    elif what == "vanishing":                                   # no values any more, and a state that fades to nothing
+        x["v"][100:] = 0
+        x["g"] -= 0.8
     elif what == "large_keys":
         x["k"], x["q"] = (x["k"].float() * 1000).to(t), (x["q"].float() * 300).to(t)
     elif what == "small_keys":
@@ -302,6 +305,58 @@ def test_prefill_of_any_size_of_numbers(L, kind, what):
     else:
         x["g"] *= 0
     check(L, "prefill", x)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("layout,lens", [((1, 1, 128, 128), [4099]), ((1, 2, 64, 128), [3000, 64 * 13 * 3]), ((1, 1, 128, 256), [2496]),
+                                         ((1, 1, 64, 128), [0, 5000, 1, 900]), ((1, 1, 64, 128), [0, 9000, 1, 2000])], ids=str)
+def test_few_long_sequences_are_walked_in_segments(L, kind, layout, lens):
+    """Segments of at least 13 chunks: whole ones, a last one of a few tokens, sequences of one segment and of none among them; states
+    left where they were read from."""
+    import torch
+    x = make(kind, lens, *layout, seed=61)
+    x["g"] *= 0.1
+    x["slot_out"] = x["slot_in"].clone()
+    chunks = (16912 if kind == "bf16" else 22032) * (x["rows"] // 64 + x["n"] + 1) * layout[1]
+    segments = L.shvk_gdn_prefill_workspace_bytes(C.byref(args(x))) - chunks > 4 * layout[2] * layout[3]      # room for their states
+    assert segments == (sum(lens) / len(lens) >= 39 * 64)         # by the average: three of 13 chunks at least (two are walked one after the other)
+    check(L, "prefill", x)
+
+
+@gpu
+def test_segments_of_a_sequence_that_begins_behind_the_first_row(L):
+    import torch
+    x = make("bf16", [200, 3300], 1, 1, 128, 128, seed=63)
+    y = make("bf16", [200, 3300], 1, 1, 128, 128, seed=63)
+    y["n"], y["lens"] = 1, [3300]
+    for name in ("seq_start", "slot_in", "slot_out"):
+        y[name] = y[name][1:].clone()
+    first = x["states"][1:2].clone()
+    z = {**x, "q": x["q"][200:], "k": x["k"][200:], "v": x["v"][200:], "g": x["g"][200:], "beta": x["beta"][200:], "lens": [3300], "rows": 3303}
+    want, states, big = rule(z, first)
+    launch(L, "prefill", y)
+    torch.cuda.synchronize()
+    factor = (128 + 24 * 3300) * 2.0 ** -24
+    got = y["o"][200:].double()
+    assert float(((got - want).abs() - 2.0 ** -8 * want.abs())[:3300].max()) <= factor * big + 2.0 ** -10 * z["pieces"]
+    assert torch.equal(y["o"][:200], torch.full_like(y["o"][:200], 7.0))
+    s = y["states"][int(y["slot_out"][0])].double()
+    assert float((s - states[0]).abs().max()) <= factor * float(states[0].norm(dim=1).max())
+
+
+@gpu
+def test_not_a_number_in_a_segment_stays_in_its_column_and_behind(L):
+    import torch
+    x, y = (make("bf16", [3900], 1, 1, 128, 128, seed=65) for _ in range(2))
+    x["v"][2000, 5] = float("nan")
+    launch(L, "prefill", x)
+    launch(L, "prefill", y)
+    torch.cuda.synchronize()
+    assert torch.isnan(x["o"][2000:3900, 0, 5].float()).all() and torch.isfinite(x["o"][:2000].float()).all()
+    keep = torch.arange(128, device="cuda") != 5
+    assert torch.equal(x["o"][:, 0, keep], y["o"][:, 0, keep])
+    assert torch.equal(x["states"][1][0][:, keep], y["states"][1][0][:, keep]) and torch.isnan(x["states"][1][0][:, 5]).all()
 
 
 @gpu
