@@ -987,45 +987,60 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
 }
 
 // X of segment g becomes Phi_g X_(g-1) + X_g, g = 1 .. the last but one, in float32: a CTA takes JC columns of a head through all segments
-// of a sequence, the state so far in shared memory.
-constexpr int JC = 8, JOIN_THREADS = 256;
+// of a sequence, the state so far in shared memory.  A thread has one key of the result and a share of the sum's keys; its part of the
+// next Phi does not depend on the state and is on its way while this one is used.
+constexpr int JC = 8, JOIN_THREADS = 512;
 template <int DK> __global__ void __launch_bounds__(JOIN_THREADS) gdn_prefill_tc_join_kernel(const shvk_gdn_seq_args a, const WalkSegments seg) {
-    constexpr int GROUPS = JOIN_THREADS / DK, CPT = JC / GROUPS;      // a thread: one key, CPT columns
-    __shared__ __align__(16) float s[2][DK][JC];
-    const int parts = a.DV / JC, part = int(blockIdx.x % unsigned(parts)), nh = int(blockIdx.x / unsigned(parts)), n = nh / a.HV, head = nh % a.HV;
+    constexpr int SHARES = JOIN_THREADS / DK, KPT = DK / SHARES, EPT = DK * JC / JOIN_THREADS;      // EPT: values of the result a thread adds up
+    static_assert(JC % EPT == 0, "a thread's values lie side by side");
+    __shared__ __align__(16) float s[DK][JC], part[SHARES][DK][JC + 1];
+    const int parts = a.DV / JC, block = int(blockIdx.x % unsigned(parts)), nh = int(blockIdx.x / unsigned(parts)), n = nh / a.HV, head = nh % a.HV;
     const SeqRows rows(a.seq_start, n, int(a.n_tokens));
     const int segments = ((rows.end - rows.start + CT - 1) / CT + seg.chunks - 1) / seg.chunks;
     if (segments < 3) return;
-    const int key = threadIdx.x % DK, c = threadIdx.x / DK * CPT;
-    const long long first = first_segment(first_chunk(rows, n), n, seg.chunks), state_of = (long long)a.HV * DK * a.DV;
-    float* x = seg.x + first * state_of + ((long long)head * DK + key) * a.DV + part * JC + c;
-    const float* phi = seg.phi + (first * a.HV + head) * DK * DK + key;
+    const int key = threadIdx.x % DK, share = threadIdx.x / DK;
+    const int k1 = threadIdx.x * EPT / JC, c1 = threadIdx.x * EPT % JC;
+    const long long first = first_segment(first_chunk(rows, n), n, seg.chunks), state_of = (long long)a.HV * DK * a.DV, phi_of = (long long)a.HV * DK * DK;
+    float* x = seg.x + first * state_of + ((long long)head * DK + k1) * a.DV + block * JC + c1;
+    const float* phi = seg.phi + (first * a.HV + head) * DK * DK + (long long)(share * KPT) * DK + key;
+    float p[KPT], y[EPT];
+    auto fetch = [&](int g) {
 #pragma unroll
-    for (int u = 0; u < CPT; ++u) s[0][key][c + u] = x[u];
+        for (int k = 0; k < KPT; ++k) p[k] = phi[g * phi_of + k * DK];
+#pragma unroll
+        for (int u = 0; u < EPT; ++u) y[u] = x[g * state_of + u];
+    };
+#pragma unroll
+    for (int u = 0; u < EPT; ++u) s[k1][c1 + u] = x[u];
+    fetch(1);
     for (int g = 1; g < segments - 1; ++g) {
-        x += state_of;
-        phi += (long long)a.HV * DK * DK;
-        float acc[CPT];
-#pragma unroll
-        for (int u = 0; u < CPT; ++u) acc[u] = x[u];
+        float acc[JC] = {};
         __syncthreads();
-        const float (*now)[JC] = s[(g - 1) & 1];
-#pragma unroll 16
-        for (int k = 0; k < DK; ++k) {
-            const float p = phi[k * DK];
 #pragma unroll
-            for (int u = 0; u < CPT; ++u) acc[u] = fmaf(p, now[k][c + u], acc[u]);
+        for (int k = 0; k < KPT; ++k) {
+            const float4 lo = *reinterpret_cast<const float4*>(&s[share * KPT + k][0]), hi = *reinterpret_cast<const float4*>(&s[share * KPT + k][4]);
+            acc[0] = fmaf(p[k], lo.x, acc[0]); acc[1] = fmaf(p[k], lo.y, acc[1]); acc[2] = fmaf(p[k], lo.z, acc[2]); acc[3] = fmaf(p[k], lo.w, acc[3]);
+            acc[4] = fmaf(p[k], hi.x, acc[4]); acc[5] = fmaf(p[k], hi.y, acc[5]); acc[6] = fmaf(p[k], hi.z, acc[6]); acc[7] = fmaf(p[k], hi.w, acc[7]);
         }
+        float sum[EPT];
 #pragma unroll
-        for (int u = 0; u < CPT; ++u) {
-            x[u] = acc[u];
-            s[g & 1][key][c + u] = acc[u];
+        for (int u = 0; u < EPT; ++u) sum[u] = y[u];
+        if (g + 1 < segments - 1) fetch(g + 1);
+#pragma unroll
+        for (int c = 0; c < JC; ++c) part[share][key][c] = acc[c];
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < EPT; ++u) {
+#pragma unroll
+            for (int h = 0; h < SHARES; ++h) sum[u] += part[h][k1][c1 + u];
+            s[k1][c1 + u] = sum[u];
+            x[g * state_of + u] = sum[u];
         }
     }
 }
 
 // Chunks of a segment, 0 where sequences are walked whole.  Counted in chunks' times of one wave of CTAs (a walk's chunk takes 7,200 cycles,
-// a join's segment about 2,000, the two launches more about as much as two chunks) for sequences of the average length; segments are not
+// a join's segment about 1,000, the two launches more about as much as two chunks) for sequences of the average length; segments are not
 // shorter than 13 chunks, so that their states take less room than their chunks' T and M.
 inline int segment_chunks(const shvk_gdn_seq_args& a) {
     const long long sms = device_sms(), splits = a.DV / TV, heads = (long long)a.n_seq * a.HV, chunks = a.n_tokens / CT / a.n_seq;
@@ -1034,7 +1049,7 @@ inline int segment_chunks(const shvk_gdn_seq_args& a) {
     int found = 0;
     for (long long g = 2; g <= 64 && (chunks + g - 1) / g >= 13; ++g) {
         const long long len = (chunks + g - 1) / g;
-        const double t = double(len * (waves(heads * (splits + (g - 2) * (splits + 1))) + waves(heads * splits * (g - 1)))) + 0.3 * double(g - 2) + 2.0;
+        const double t = double(len * (waves(heads * (splits + (g - 2) * (splits + 1))) + waves(heads * splits * (g - 1)))) + 0.15 * double(g - 2) + 2.0;
         if (t < best) { best = t; found = int(len); }
     }
     return found;
