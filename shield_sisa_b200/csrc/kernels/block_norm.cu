@@ -4,7 +4,7 @@
 // with rstd(z) = 1 / sqrt(mean(z^2) + eps), every step in float32 and each output rounded once.  HBM binds: a row's arrays are read
 // once into registers, its two sums of squares are reductions over the threads that hold the row.
 //
-// A thread has NV groups of eight consecutive values (16-byte accesses): 16 threads, a warp or a whole CTA to a row, by its length.
+// A thread has NV groups of eight consecutive values (16-byte accesses): 8 or 16 threads, a warp or a whole CTA to a row, by its length.
 // Rows whose pitch is no multiple of eight start anywhere in such a group.  All arrays of a call then start at the same place of it (or
 // the call goes to block_norm_any_kernel), and the place repeats every eight rows at most: a CTA walks rows of one class, which are
 // cut at the same places, so that its copy of the weights in shared memory, shifted as its rows are, serves them all with 16-byte
@@ -43,43 +43,110 @@ template <typename T> __device__ __forceinline__ void put8(T* p, const float (&v
     }
 }
 
-// act(g): SiLU and sigmoid from one exponential
-template <typename T> __device__ __forceinline__ float gate_of(float g, int act) {
-    if (act == 0) return g;
-    const float s = sizeof(T) == 4 ? 1.0f / (1.0f + expf(-g)) : __fdividef(1.0f, 1.0f + __expf(-g));
-    return act == 1 ? g * s : s;
+// A group of eight values as it lies in memory: 16 or 32 bytes.
+template <typename T> struct Raw { uint4 w[sizeof(T) == 4 ? 2 : 1]; };
+// The values [lo, hi) of a group, the others as it may be: the whole group in one or two accesses where all of it lies in the array
+// (`whole`: everywhere but at an array's end), else value by value.  (Value by value at every row's edges, loads waited for one another:
+// 189 us instead of 58 for 16,384 rows of 2,047.)
+template <typename T> __device__ __forceinline__ Raw<T> get_raw(const T* p, int lo, int hi, bool whole) {
+    Raw<T> r;
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < int(sizeof(r.w) / 16); ++i) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+        T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = p[min(max(i, lo), hi - 1)];
+    }
+    return r;
+}
+template <typename T> __device__ __forceinline__ void values_of(const Raw<T>& r, int lo, int hi, float (&v)[8]) {
+    const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
+    if (hi - lo != 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < lo || i >= hi) v[i] = 0.0f;
 }
 
-// ROWT: threads of a row: 16, 32, or 0 = the whole CTA.  P: classes of rows (1 where every row starts on a group).
-template <typename T, typename TH, int NV, int ROWT>
-__global__ void __launch_bounds__(ROWT ? 128 : 512)
+// sigmoid(g); for 16-bit types with the hardware's exponential and reciprocal (some 2^-21 off, far below half a step of the type)
+template <typename T> __device__ __forceinline__ float sigmoid_of(float g) {
+    if constexpr (sizeof(T) == 4) {
+        return 1.0f / (1.0f + expf(-g));
+    } else {
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-g)));
+        return r;
+    }
+}
+template <typename T> __device__ __forceinline__ float gate_of(float g, int act) {
+    return act == 0 ? g : act == 1 ? g * sigmoid_of<T>(g) : sigmoid_of<T>(g);
+}
+// x *= act(g)
+template <typename T> __device__ __forceinline__ void gate8(float (&x)[8], const float (&g)[8], int act) {
+    if (act == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= g[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= (act == 1 ? g[e] : 1.0f) * sigmoid_of<T>(g[e]);
+    }
+}
+
+// ROWT: threads of a row: 8, 16, 32, or 0 = the whole CTA.  EDGE: a group may reach over a row's ends.  P: classes of rows (1 where every row starts on a group).  The next row's values
+// are asked for before this one's are used (not with four groups a thread: no registers).
+template <typename T, typename TH, int NV, int ROWT, bool EDGE>
+__global__ void __launch_bounds__(ROWT ? 128 : 512, ROWT == 0 ? 1 : NV == 1 ? 6 : 4)
 block_norm_kernel(const shvk_block_norm_args a, int P) {
     extern __shared__ __align__(16) float bn_w[];                // post_w | pre_w | gate row, each `span` floats
     __shared__ float red[2][2][32];                              // [row parity][which sum][warp]
     const int tid = threadIdx.x, rt = ROWT ? ROWT : blockDim.x, span = rt * NV * 8;
     const int groups = ROWT ? blockDim.x / ROWT : 1, grp = ROWT ? tid / ROWT : 0, j = ROWT ? tid % ROWT : tid;
-    const int cls = blockIdx.x % P;
-    const long long cta = blockIdx.x / P, ctas = gridDim.x / P, total = a.rows * a.heads;
+    const int cls = blockIdx.x % P, cta = blockIdx.x / P, total = int(a.rows * a.heads);
     const int off = int(cls * (a.ldx & 7) & 7);                  // where the class's rows start in a group (0 where P is 1)
-    const bool post = a.post_w, pre = a.pre_w, one_gate = a.gate && a.ldgate == 0 && a.heads == 1;
+    // this group's rows are R, R + step, ...; as (row, head) they move by (step_row, step_head)
+    const int step = int(gridDim.x / P) * groups * P, step_row = step / a.heads, step_head = step % a.heads;
+    int R = (cta * groups + grp) * P + cls, row = R / a.heads, head = R % a.heads;
+    const bool post = a.post_w, pre = a.pre_w, one_gate = a.gate && a.ldgate == 0 && a.heads == 1, row_gate = a.gate && !one_gate;
     const float inv_d = 1.0f / float(a.D);
+    const int width = a.heads * a.D;                             // of a row
     int lo[NV], hi[NV];                                          // the values of each group that belong to the row: [lo, hi)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (j + i * rt) * 8 - off;                    // column of the group's first value
-        lo[i] = c < 0 ? min(-c, 8) : 0;
-        hi[i] = max(min(a.D - c, 8), 0);
+        lo[i] = EDGE && c < 0 ? min(-c, 8) : 0;
+        hi[i] = EDGE ? max(min(a.D - c, 8), 0) : c < a.D ? 8 : 0;
     }
-    auto load = [&](const auto* p, int i, float (&v)[8]) {            // p: the group's first value
-        if (hi[i] - lo[i] == 8) {
-            get8(p, v);
-        } else {
+    auto full = [&](int i) { return !EDGE || hi[i] - lo[i] == 8; };
+    struct Row {
+        Raw<T> x[NV], g[NV];
+        Raw<TH> h[NV];
+    };
+    // the values of (row, head); where there are none (no such row, no such group) zeros
+    auto fetch = [&](bool on, int row, int head, Row& r) {
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        const int base = head * a.D - off + j * 8;
+        const T* px = static_cast<const T*>(a.x) + row * a.ldx + base;
+        const T* pg = static_cast<const T*>(a.gate) + row * a.ldgate + base;
+        const TH* ph = static_cast<const TH*>(a.h_in) + row * a.ldh_in + base;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = e >= lo[i] && e < hi[i] ? to_float(p[e]) : 0.0f;
+        for (int i = 0; i < NV; ++i) {
+            r.x[i].w[0] = r.g[i].w[0] = z;
+            r.h[i].w[0] = z;
+            if constexpr (sizeof(T) == 4) r.x[i].w[1] = r.g[i].w[1] = z;
+            if constexpr (sizeof(TH) == 4) r.h[i].w[1] = z;
+            if (on && hi[i] > lo[i]) {
+                const int c = i * rt * 8;
+                const bool fits = !EDGE || base + c + 8 <= width, before = row + 1 < a.rows;
+                r.x[i] = get_raw(px + c, lo[i], hi[i], fits || (before && a.ldx >= width));
+                if (a.h_in) r.h[i] = get_raw(ph + c, lo[i], hi[i], fits || (before && a.ldh_in >= width));
+                if (row_gate) r.g[i] = get_raw(pg + c, lo[i], hi[i], fits || (before && a.ldgate >= width));
+            }
         }
     };
     auto store = [&](auto* p, int i, const float (&v)[8]) {
-        if (hi[i] - lo[i] == 8) {
+        if (full(i)) {
             put8(p, v);
         } else {
 #pragma unroll
@@ -87,51 +154,47 @@ block_norm_kernel(const shvk_block_norm_args a, int P) {
                 if (e >= lo[i] && e < hi[i]) p[e] = from_float<std::remove_pointer_t<decltype(p)>>(v[e]);
         }
     };
-    bool staged = false;
+    constexpr bool AHEAD = NV < 4;
+    Row now;
+    fetch(R < total, row, head, now);
+    for (int e = tid; e < span; e += blockDim.x) {               // the weights, behind the first row's loads
+        const int c = e - off;
+        const bool in = c >= 0 && c < a.D;
+        if (post) bn_w[e] = in ? a.post_w[c] : 0.0f;
+        if (pre) bn_w[span + e] = in ? a.pre_w[c] : 0.0f;
+        if (one_gate) bn_w[2 * span + e] = in ? gate_of<T>(to_float(static_cast<const T*>(a.gate)[c]), a.gate_act) : 0.0f;
+    }
+    __syncthreads();
     int par = 0;
     // whole CTAs walk the rows in step: a group without a row of its own goes along without touching memory
-    for (long long at = cta * groups; P * at + cls < total; at += ctas * groups, par ^= 1) {
-        const long long R = P * (at + grp) + cls;
+    for (int first = cta * groups * P + cls; first < total; first += step, par ^= 1) {
         const bool on = R < total;
-        const long long row = on ? (a.heads == 1 ? R : R / a.heads) : 0;
-        const long long base = (on ? R - row * a.heads : 0) * a.D - off + j * 8;
+        const int this_row = row, this_base = head * a.D - off + j * 8;
+        R += step;
+        row += step_row;
+        head += step_head;
+        if (head >= a.heads) {
+            head -= a.heads;
+            ++row;
+        }
+        Row next;
+        if (AHEAD) fetch(R < total, row, head, next);
         float x[NV][8], h[NV][8], ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const long long c = base + i * rt * 8;
-            const bool any = on && hi[i] > lo[i];
+            float gt[8];
+            values_of(now.x[i], EDGE ? lo[i] : 0, EDGE ? hi[i] : 8, x[i]);
+            values_of(now.h[i], EDGE ? lo[i] : 0, EDGE ? hi[i] : 8, h[i]);
+            if (row_gate) values_of(now.g[i], EDGE ? lo[i] : 0, EDGE ? hi[i] : 8, gt);
+            if (post)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = h[i][e] = 0.0f;
-            float gt[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
-            if (any) {
-                load(static_cast<const T*>(a.x) + row * a.ldx + c, i, x[i]);
-                if (a.h_in) load(static_cast<const TH*>(a.h_in) + row * a.ldh_in + c, i, h[i]);
-                if (a.gate && !one_gate) {
-                    load(static_cast<const T*>(a.gate) + row * a.ldgate + c, i, gt);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) gt[e] = gate_of<T>(gt[e], a.gate_act);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {                        // the row's rstd is one factor of all its values: the gate may go first
-                ss = fmaf(x[i][e], x[i][e], ss);
-                x[i][e] *= gt[e];
-            }
-        }
-        if (!staged) {                                           // behind the first row's loads
-            for (int e = tid; e < span; e += blockDim.x) {
-                const int c = e - off;
-                const bool in = c >= 0 && c < a.D;
-                if (post) bn_w[e] = in ? a.post_w[c] : 0.0f;
-                if (pre) bn_w[span + e] = in ? a.pre_w[c] : 0.0f;
-                if (one_gate) bn_w[2 * span + e] = in ? gate_of<T>(to_float(static_cast<const T*>(a.gate)[c]), a.gate_act) : 0.0f;
-            }
-            __syncthreads();
-            staged = true;
+                for (int e = 0; e < 8; ++e) ss = fmaf(x[i][e], x[i][e], ss);
+            if (row_gate)                                        // the row's rstd is one factor of all its values: the gate may go first
+                gate8<T>(x[i], gt, a.gate_act);
         }
         auto row_sum = [&](float v, int which) {
 #pragma unroll
-            for (int o = ROWT == 16 ? 8 : 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            for (int o = ROWT ? ROWT / 2 : 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
             if constexpr (ROWT == 0) {
                 if ((tid & 31) == 0) red[par][which][tid >> 5] = v;
                 __syncthreads();
@@ -143,7 +206,7 @@ block_norm_kernel(const shvk_block_norm_args a, int P) {
             return v;
         };
         if (post) {
-            const float r = 1.0f / sqrtf(row_sum(ss, 0) * inv_d + a.eps);
+            const float r = rsqrtf(row_sum(ss, 0) * inv_d + a.eps);      // (two steps of 2^-23 off at most)
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 float w[8];
@@ -162,23 +225,25 @@ block_norm_kernel(const shvk_block_norm_args a, int P) {
                 for (int e = 0; e < 8; ++e) x[i][e] *= w[e];
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[i][e] = a.h_in ? fmaf(x[i][e], a.scale, h[i][e]) : x[i][e] * a.scale;
-            const bool any = on && hi[i] > lo[i];
-            if (any && a.h_out) store(static_cast<TH*>(a.h_out) + row * a.ldh_out + base + i * rt * 8, i, h[i]);
+            for (int e = 0; e < 8; ++e) h[i][e] = fmaf(x[i][e], a.scale, h[i][e]);       // (h is zero where there is no residual)
+            if (pre)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+                for (int e = 0; e < 8; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+            if (on && hi[i] > lo[i] && a.h_out) store(static_cast<TH*>(a.h_out) + this_row * a.ldh_out + this_base + i * rt * 8, i, h[i]);
         }
         if (pre) {
-            const float r = 1.0f / sqrtf(row_sum(ss, 1) * inv_d + a.eps);
+            const float r = rsqrtf(row_sum(ss, 1) * inv_d + a.eps);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 float w[8];
                 get8<float>(bn_w + span + (j + i * rt) * 8, w);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[e] = h[i][e] * r * w[e];
-                if (on && hi[i] > lo[i]) store(static_cast<T*>(a.xn) + row * a.ldxn + base + i * rt * 8, i, w);
+                if (on && hi[i] > lo[i]) store(static_cast<T*>(a.xn) + this_row * a.ldxn + this_base + i * rt * 8, i, w);
             }
         }
+        if (AHEAD) now = next;
+        else fetch(R < total, row, head, now);
     }
 }
 
@@ -225,19 +290,27 @@ __global__ void __launch_bounds__(256) block_norm_any_kernel(const shvk_block_no
     }
 }
 
-template <typename T, typename TH, int NV, int ROWT>
+template <typename T, typename TH, int NV, int ROWT, bool EDGE>
 int launch_rows(const shvk_block_norm_args& a, int P, int threads, cudaStream_t s) {
     const int groups = ROWT ? threads / ROWT : 1, span = (ROWT ? ROWT : threads) * NV * 8;
     const int smem = 3 * span * int(sizeof(float));
     static_assert(3 * 4 * 512 * 8 * sizeof(float) <= 200 * 1024, "the longest row's weights fit");
-    const cudaError_t e = cudaFuncSetAttribute(block_norm_kernel<T, TH, NV, ROWT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(block_norm_kernel<T, TH, NV, ROWT, EDGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return int(e);
     const long long need = ((a.rows * a.heads + P - 1) / P + groups - 1) / groups * P;     // CTAs of one pass over the rows
-    const int resident = 1024 / threads;
+    const int resident = ROWT ? (NV == 1 ? 6 : 4) : threads > 256 ? 1 : 512 / threads;      // CTAs of an SM, by registers
     const long long most = (long long)device_sms() * resident / P * P;
     const long long ctas = need < most ? need : (most > 0 ? most : P);
-    block_norm_kernel<T, TH, NV, ROWT><<<unsigned(ctas), threads, smem, s>>>(a, P);
+    block_norm_kernel<T, TH, NV, ROWT, EDGE><<<unsigned(ctas), threads, smem, s>>>(a, P);
     return int(cudaGetLastError());
+}
+
+template <typename T, typename TH, bool EDGE> int launch_vec(const shvk_block_norm_args& a, int P, int nvec, cudaStream_t s) {
+    if (nvec <= 16) return launch_rows<T, TH, 2, 8, EDGE>(a, P, 128, s);
+    if (nvec <= 32) return launch_rows<T, TH, 2, 16, EDGE>(a, P, 128, s);
+    if (nvec <= 64) return launch_rows<T, TH, 2, 32, EDGE>(a, P, 128, s);
+    if (nvec <= 1024) return launch_rows<T, TH, 2, 0, EDGE>(a, P, ((nvec + 1) / 2 + 31) / 32 * 32, s);
+    return launch_rows<T, TH, 4, 0, EDGE>(a, P, ((nvec + 3) / 4 + 31) / 32 * 32, s);
 }
 
 inline bool on_group(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -251,18 +324,13 @@ template <typename T, typename TH> int launch_block_norm(const shvk_block_norm_a
                      (!gate_rows || (a.ldgate & 7) == ld) && (a.heads == 1 || (ld == 0 && a.D % 8 == 0));
     const int P = a.rows == 1 ? 1 : ld == 0 ? 1 : ld % 2 ? 8 : ld % 4 ? 4 : 2, nvec = (a.D + (P > 1 ? 7 : 0) + 7) / 8;
     if (!vec || nvec > 2048) {
-        if (a.rows * a.heads > 0x7fffffff) return int(cudaErrorInvalidValue);
         const int smem = a.D * int(sizeof(float));
         const cudaError_t e = cudaFuncSetAttribute(block_norm_any_kernel<T, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return int(e);
         block_norm_any_kernel<T, TH><<<unsigned(a.rows * a.heads), 256, smem, s>>>(a);
         return int(cudaGetLastError());
     }
-    if (nvec <= 16) return launch_rows<T, TH, 1, 16>(a, P, 128, s);
-    if (nvec <= 32) return launch_rows<T, TH, 1, 32>(a, P, 128, s);
-    if (nvec <= 64) return launch_rows<T, TH, 2, 32>(a, P, 128, s);
-    if (nvec <= 1024) return launch_rows<T, TH, 2, 0>(a, P, ((nvec + 1) / 2 + 31) / 32 * 32, s);
-    return launch_rows<T, TH, 4, 0>(a, P, ((nvec + 3) / 4 + 31) / 32 * 32, s);
+    return P == 1 && a.D % 8 == 0 ? launch_vec<T, TH, false>(a, P, nvec, s) : launch_vec<T, TH, true>(a, P, nvec, s);
 }
 
 inline bool on_type(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == DT_F32 ? 3 : 1)) == 0; }
@@ -281,6 +349,7 @@ extern "C" int shvk_block_norm(const shvk_block_norm_args* a, void* stream) {
     if (!!a->pre_w != !!a->xn || (!a->h_out && !a->xn)) return bad;
     if (a->rows == 0) return 0;
     if (!a->x) return bad;
+    if (a->rows > 0x3fffffff / a->heads) return bad;
     const long long width = (long long)a->heads * a->D;
     if (a->ldx < 0 || (a->h_in && a->ldh_in < 0) || (a->gate && a->ldgate < 0)) return bad;
     if (a->rows > 1 && ((a->h_out && a->ldh_out < width) || (a->xn && a->ldxn < width))) return bad;
@@ -288,6 +357,14 @@ extern "C" int shvk_block_norm(const shvk_block_norm_args* a, void* stream) {
         !on_type(a->post_w, DT_F32) || !on_type(a->pre_w, DT_F32))
         return bad;
     cudaStream_t s = cudaStream_t(stream);
+    shvk_block_norm_args dense = *a;                             // heads that follow one another without a gap are rows
+    auto packed = [&](const void* p, long long ld) { return !p || ld == width; };
+    if (a->heads > 1 && packed(a->x, a->ldx) && packed(a->gate, a->ldgate) && packed(a->h_in, a->ldh_in) && packed(a->h_out, a->ldh_out) && packed(a->xn, a->ldxn)) {
+        dense.rows *= a->heads;
+        dense.heads = 1;
+        dense.ldx = dense.ldgate = dense.ldh_in = dense.ldh_out = dense.ldxn = a->D;
+        a = &dense;
+    }
     if (t == DT_F32) return launch_block_norm<float, float>(*a, s);
     if (t == DT_BF16) return a->h_dtype == DT_F32 ? launch_block_norm<__nv_bfloat16, float>(*a, s) : launch_block_norm<__nv_bfloat16, __nv_bfloat16>(*a, s);
     return a->h_dtype == DT_F32 ? launch_block_norm<__half, float>(*a, s) : launch_block_norm<__half, __half>(*a, s);

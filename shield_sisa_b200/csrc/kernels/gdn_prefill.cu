@@ -594,6 +594,11 @@ template <typename T, int DK, int NW, int NSLOT, int MINCTA> int launch_scan(con
     return int(cudaGetLastError());
 }
 
+// Whether the chunks of 64 tokens take a call: heads of whole 128 values, sequences that on average fill a chunk (with the narrower keys:
+// two).  us, 64 / 16: DK 128, 128 sequences of 6 heads, 48 tokens 109 / 89, 64 111 / 111, 128 154 / 169; 37 of 500 138 / 185; 512 of 32
+// 352 / 247, of 64 362 / 369, of 321 1,098 / 1,324.  DK 64: 128 of 64 84 / 68, of 128 117 / 113; 37 of 500 107 / 122; 1 of 1,000 64 / 91.
+inline bool takes_tc(const shvk_gdn_seq_args& a) { return a.DV % 128 == 0 && a.n_tokens >= (long long)a.n_seq * (a.DK == 64 ? 128 : 64); }
+
 inline long long prefill_chunks(const shvk_gdn_seq_args& a) { return a.n_tokens / PB + a.n_seq + 1; }
 
 template <typename T, int DK> int launch_prefill(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s) {
@@ -618,7 +623,7 @@ template <typename T, int DK> int launch_prefill(const shvk_gdn_seq_args& a, uin
 extern "C" size_t shvk_gdn_prefill_workspace_bytes(const shvk_gdn_seq_args* a) {
     using namespace sb;
     if (check_gdn_seq(a) || a->n_seq == 0) return 0;
-    if (a->DV % 128 == 0) return gdn_prefill_tc_workspace(*a);
+    if (takes_tc(*a)) return gdn_prefill_tc_workspace(*a);
     return size_t(prefill_chunks(*a)) * size_t(a->HV) * size_t(PW_BYTES);
 }
 
@@ -630,7 +635,7 @@ extern "C" int shvk_gdn_prefill(const shvk_gdn_seq_args* a, void* workspace, siz
     if (!workspace || !aligned16(workspace) || workspace_bytes < shvk_gdn_prefill_workspace_bytes(a)) return int(cudaErrorInvalidValue);
     cudaStream_t s = cudaStream_t(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    if (a->DV % 128 == 0) return gdn_prefill_tc(*a, ws, s);
+    if (takes_tc(*a)) return gdn_prefill_tc(*a, ws, s);
     if (a->dtype == DT_BF16) return a->DK == 64 ? launch_prefill<__nv_bfloat16, 64>(*a, ws, s) : launch_prefill<__nv_bfloat16, 128>(*a, ws, s);
     return a->DK == 64 ? launch_prefill<__half, 64>(*a, ws, s) : launch_prefill<__half, 128>(*a, ws, s);
 }

@@ -32,7 +32,7 @@ def good(**kw):
     return binding.BlockNormArgs(**a)
 
 
-BAD = [dict(rows=-1), dict(heads=0), dict(heads=5000), dict(D=0), dict(D=16385), dict(x=None), dict(x_dtype=3), dict(x_dtype=-1),
+BAD = [dict(rows=-1), dict(rows=1 << 30), dict(rows=1 << 28, heads=6, ldx=4096, ldh_in=4096, ldh_out=4096, ldxn=4096, ldgate=4096), dict(heads=0), dict(heads=5000), dict(D=0), dict(D=16385), dict(x=None), dict(x_dtype=3), dict(x_dtype=-1),
        dict(h_dtype=2), dict(h_dtype=3), dict(gate_dtype=0), dict(gate_dtype=2), dict(xn_dtype=0), dict(gate_act=3), dict(gate_act=-1),
        dict(pre_w=None), dict(xn=None), dict(pre_w=None, xn=None, h_out=None), dict(ldx=-1), dict(ldh_in=-8), dict(ldgate=-1),
        dict(ldh_out=383), dict(ldxn=376), dict(heads=2), dict(x=0x100001), dict(h_in=0x100002), dict(post_w=0x100002)]
