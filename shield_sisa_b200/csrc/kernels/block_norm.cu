@@ -97,10 +97,10 @@ template <typename T> __device__ __forceinline__ void gate8(float (&x)[8], const
 // ROWT: threads of a row: 8, 16, 32, or 0 = the whole CTA.  EDGE: a group may reach over a row's ends.  P: classes of rows (1 where every row starts on a group).  The next row's values
 // are asked for before this one's are used (not with four groups a thread: no registers).
 template <typename T, typename TH, int NV, int ROWT, bool EDGE>
-__global__ void __launch_bounds__(ROWT ? 128 : 512, ROWT == 0 ? 1 : NV == 1 ? 6 : 4)
+__global__ void __launch_bounds__(ROWT ? 128 : 512, ROWT ? 4 : NV == 1 ? 2 : 1)
 block_norm_kernel(const shvk_block_norm_args a, int P) {
     extern __shared__ __align__(16) float bn_w[];                // post_w | pre_w | gate row, each `span` floats
-    __shared__ float red[2][2][32];                              // [row parity][which sum][warp]
+    __shared__ __align__(16) float red[2][2][16];                            // [row parity][which sum][warp]
     const int tid = threadIdx.x, rt = ROWT ? ROWT : blockDim.x, span = rt * NV * 8;
     const int groups = ROWT ? blockDim.x / ROWT : 1, grp = ROWT ? tid / ROWT : 0, j = ROWT ? tid % ROWT : tid;
     const int cls = blockIdx.x % P, cta = blockIdx.x / P, total = int(a.rows * a.heads);
@@ -157,6 +157,7 @@ block_norm_kernel(const shvk_block_norm_args a, int P) {
     constexpr bool AHEAD = NV < 4;
     Row now;
     fetch(R < total, row, head, now);
+    if (ROWT == 0 && tid < 64) (&red[0][0][0])[tid] = 0.0f;
     for (int e = tid; e < span; e += blockDim.x) {               // the weights, behind the first row's loads
         const int c = e - off;
         const bool in = c >= 0 && c < a.D;
@@ -198,10 +199,13 @@ block_norm_kernel(const shvk_block_norm_args a, int P) {
             if constexpr (ROWT == 0) {
                 if ((tid & 31) == 0) red[par][which][tid >> 5] = v;
                 __syncthreads();
-                const int nw = blockDim.x >> 5;
-                v = (tid & 31) < nw ? red[par][which][tid & 31] : 0.0f;
+                v = 0.0f;
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                for (int w = 0; w < 16; w += 4)                  // (no more than sixteen warps, the sums of those that are not there zero)
+                    if (w * 32 < blockDim.x) {
+                        const float4 q = *reinterpret_cast<const float4*>(&red[par][which][w]);
+                        v += (q.x + q.y) + (q.z + q.w);
+                    }
             }
             return v;
         };
@@ -298,7 +302,7 @@ int launch_rows(const shvk_block_norm_args& a, int P, int threads, cudaStream_t 
     const cudaError_t e = cudaFuncSetAttribute(block_norm_kernel<T, TH, NV, ROWT, EDGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return int(e);
     const long long need = ((a.rows * a.heads + P - 1) / P + groups - 1) / groups * P;     // CTAs of one pass over the rows
-    const int resident = ROWT ? (NV == 1 ? 6 : 4) : threads > 256 ? 1 : 512 / threads;      // CTAs of an SM, by registers
+    const int resident = ROWT ? 4 : NV == 1 ? 1024 / threads : threads > 256 ? 1 : 512 / threads;      // CTAs of an SM, by registers
     const long long most = (long long)device_sms() * resident / P * P;
     const long long ctas = need < most ? need : (most > 0 ? most : P);
     block_norm_kernel<T, TH, NV, ROWT, EDGE><<<unsigned(ctas), threads, smem, s>>>(a, P);
@@ -309,6 +313,8 @@ template <typename T, typename TH, bool EDGE> int launch_vec(const shvk_block_no
     if (nvec <= 16) return launch_rows<T, TH, 2, 8, EDGE>(a, P, 128, s);
     if (nvec <= 32) return launch_rows<T, TH, 2, 16, EDGE>(a, P, 128, s);
     if (nvec <= 64) return launch_rows<T, TH, 2, 32, EDGE>(a, P, 128, s);
+    // one group a thread while a CTA may hold the row so (16,384 rows of 2,048: 65 us, two groups 71; of 2,047, with edges: 100 and 94)
+    if (!EDGE && nvec <= 512) return launch_rows<T, TH, 1, 0, false>(a, P, (nvec + 31) / 32 * 32, s);
     if (nvec <= 1024) return launch_rows<T, TH, 2, 0, EDGE>(a, P, ((nvec + 1) / 2 + 31) / 32 * 32, s);
     return launch_rows<T, TH, 4, 0, EDGE>(a, P, ((nvec + 3) / 4 + 31) / 32 * 32, s);
 }

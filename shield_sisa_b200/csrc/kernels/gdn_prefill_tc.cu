@@ -29,13 +29,10 @@ using namespace tc;
 constexpr int CT = 64;                                           // tokens of a chunk
 constexpr int TV = 128;                                          // value columns of a CTA
 // A triangular 64 x 64 fp16 matrix [i][j], j in steps of 16: step kk holds rows 16 kk .. 63, 32 bytes each, in core matrices of 8 rows x 16
-// bytes (rows 16 bytes apart, the two of a step's 16 columns 128 apart, the next 8 rows 256 apart).
+// bytes (rows 16 bytes apart, the two of a step's 16 columns 128 apart, the next 8 rows 256 apart): (i, j) at
+// tri_at(i, j) = tri_step(j / 16) + (r / 8) 256 + (j / 8 % 2) 128 + (r % 8) 16 + (j % 8) 2, r = i - 16 (j / 16).
 constexpr int TRI_BYTES = 5120;
 __host__ __device__ constexpr int tri_step(int kk) { return 32 * (64 * kk - 8 * kk * (kk - 1)); }
-__device__ __forceinline__ int tri_at(int i, int j) {
-    const int kk = j >> 4, r = i - 16 * kk;
-    return tri_step(kk) + (r >> 3) * 256 + ((j >> 3) & 1) * 128 + (r & 7) * 16 + (j & 7) * 2;
-}
 // workspace of a chunk and head: T hi | T lo | M hi | (M lo) | six arrays of 64 floats | e_64, T's scale, the largest ER, DK's scale
 template <bool FINE> struct Ws {
     static constexpr int T = 0, TL = TRI_BYTES, M = 2 * TRI_BYTES, ML = 3 * TRI_BYTES, SC = (FINE ? 4 : 3) * TRI_BYTES;
@@ -284,7 +281,7 @@ __global__ void __launch_bounds__(128, FINE_PREP<T> ? 3 : 4) gdn_prefill_tc_prep
                 }
                 *reinterpret_cast<float2*>(sm.l + i * LP + j0) = make_float2(l[0], l[1]);
                 uint32_t mh, ml;
-                const int at = tri_at(i, j0);
+                const int at = tri_step(bj) + (2 * (bi - bj) + h) * 256 + ni * 128 + g * 16 + 4 * t;      // tri_at(i, j0)
                 if (FINE) {
                     split_pair(m[0], m[1], mh, ml);
                     *reinterpret_cast<uint32_t*>(out + W::M + at) = mh;
@@ -364,11 +361,12 @@ __global__ void __launch_bounds__(128, FINE_PREP<T> ? 3 : 4) gdn_prefill_tc_prep
         if (tid == 0)
             *reinterpret_cast<float4*>(out + W::E64) = make_float4(expf(float(last)), pow2_biased(te + 1), fmaxf(sm.erm[0], sm.erm[1]),
                                                                    pow2_biased(clampi(exponent_of(fmaxf(sm.dkm[0], sm.dkm[1])), 27, 227) + 1));
+        const int in_block = (tid >> 6) * 256 + ((tid >> 2) & 1) * 128 + ((tid >> 3) & 7) * 16 + (tid & 3) * 4;
         if (tid < CT) outf(W::DK)[tid] *= pow2_biased(253 - clampi(exponent_of(fmaxf(sm.dkm[0], sm.dkm[1])), 27, 227));
 #pragma unroll
         for (int b = 0; b < 10; ++b) {
             const int bi = b == 0 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, bj = b - bi * (bi + 1) / 2;
-            const int at = tri_at(16 * bi + (tid >> 3), 16 * bj + 2 * (tid & 7));
+            const int at = tri_step(bj) + (bi - bj) * 512 + in_block;      // tri_at(16 bi + tid / 8, 16 bj + 2 (tid % 8))
             split_pair(v[b].x * sc, v[b].y * sc, *reinterpret_cast<uint32_t*>(out + W::T + at), *reinterpret_cast<uint32_t*>(out + W::TL + at));
         }
     }
@@ -633,6 +631,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             // (not below 2^-55: the product of two scales, sig up to 2^64, has to stay finite)
             const int wb = clampi(exponent_of(fmaf(vtop, sig, tail.z * stop * (DK == 64 ? 8.0f : 11.4f))), 72, 227);
             const float wsc = pow2_biased(261 - wb), uf = pow2_biased(wb - 7) * tail.y;
+            float scaled[32];                                    // V in W's scale
+#pragma unroll
+            for (int i = 0; i < 32; ++i) scaled[i] = to_float(v[i * TV]) * (sig * wsc);
             wait(b_r, ph);
             tc_fence_after();
             // ------------------------------------------------------------------- W = V - e K S0
@@ -640,10 +641,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             for (int p = 0; p < 2; ++p) {
                 uint32_t r[16], hi[8], lo[8];
                 tc_ld16(tl + C::R + 32 * half + 16 * p, r);
-                float x[16];
-                const float vs = sig * wsc;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = to_float(v[(16 * p + i) * TV]) * vs;
+                float (&x)[16] = *reinterpret_cast<float (*)[16]>(scaled + 16 * p);
                 const float2 ws2 = make_float2(-wsc, -wsc);
                 const float4* er4 = reinterpret_cast<const float4*>(sc + W::ER / 4 + 32 * half + 16 * p);
                 tc_wait_ld();

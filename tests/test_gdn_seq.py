@@ -252,13 +252,13 @@ def test_prefill_on_slices_of_one_row_without_normalising(L, kind):
 @gpu
 @pytest.mark.parametrize("n", [1, 30, 60, 200])
 def test_prefill_of_few_and_many_sequences(L, n):
-    """Every share of the value columns that a CTA may take: the same bits in all."""
+    """Short sequences: every share of the value columns that a CTA of the 16-token form may take: the same bits in all."""
     import torch
-    x = make("bf16", [50] * n, 2, 4, 128, 128, seed=8)
+    x = make("bf16", [50] * n, 2, 4, 128, 128, seed=8, tail=0)
     for name in ("q", "k", "v", "g", "beta"):
         x[name][:50 * n] = x[name][:50].repeat(n, 1)
     x["states"][:n] = x["states"][0].clone()
-    y = make("bf16", [50], 2, 4, 128, 128, seed=8)
+    y = make("bf16", [50], 2, 4, 128, 128, seed=8, tail=0)
     for name in ("q", "k", "v", "g", "beta"):
         y[name][:50] = x[name][:50]
     y["states"][0] = x["states"][0]
@@ -547,23 +547,25 @@ def test_a_bad_token_does_not_reach_the_tokens_before_it(L, form, name, bad):
 
 @gpu
 @pytest.mark.parametrize("form", ["step", "prefill"])
-def test_a_sequence_gives_the_same_bits_alone_and_in_a_batch(L, form):
+def test_a_sequence_gives_the_same_bits_whatever_is_beside_it(L, form):
+    """Next to others, and where all others of the call are empty (the prefill form takes its chunks and segments by the call's counts, so
+    those stay)."""
     import torch
-    lens = [18, 1, 33, 0, 16, 47] * 9
-    x = make("bf16", lens, 2, 4, 128, 128, seed=21)
-    launch(L, form, x)
-    torch.cuda.synchronize()
-    starts = np.concatenate([[0], np.cumsum(lens)])
-    for n in (0, 2, 5, 53):
-        y = make("bf16", lens, 2, 4, 128, 128, seed=21)
-        y["n"], y["lens"] = 1, [lens[n]]
-        y["seq_start"] = y["seq_start"][n:n + 2].clone()
-        y["slot_in"], y["slot_out"] = y["slot_in"][n:n + 1].clone(), y["slot_out"][n:n + 1].clone()
-        launch(L, form, y)
+    for lens in ([18, 1, 33, 0, 16, 47] * 9, [200, 64, 333, 0, 100, 129] * 9):
+        x = make("bf16", lens, 2, 4, 128, 128, seed=21)
+        launch(L, form, x)
         torch.cuda.synchronize()
-        assert torch.equal(x["o"][starts[n]:starts[n + 1]], y["o"][starts[n]:starts[n + 1]])
-        s = int(y["slot_out"][0])
-        assert torch.equal(x["states"][s], y["states"][s])
+        starts = np.concatenate([[0], np.cumsum(lens)])
+        for n in (0, 2, 5, 53):
+            y = make("bf16", lens, 2, 4, 128, 128, seed=21)
+            alone = np.full(len(lens) + 1, starts[n + 1], np.int32)
+            alone[:n + 1] = starts[n]
+            y["seq_start"] = torch.from_numpy(alone).cuda()
+            launch(L, form, y)
+            torch.cuda.synchronize()
+            assert torch.equal(x["o"][starts[n]:starts[n + 1]], y["o"][starts[n]:starts[n + 1]])
+            s = int(y["slot_out"][n])
+            assert torch.equal(x["states"][s], y["states"][s])
 
 
 @gpu
