@@ -758,16 +758,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             wait(wfull(sn), snph);
             wait(full(sn), snph);
             const T* v = reinterpret_cast<const T*>(sm.st[sn].v) + row;
-            float m0 = 0.0f, m1 = 0.0f;
+            float m = 0.0f;
 #pragma unroll 1
             for (int p = 0; p < CT; p += 16)
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float y0 = fabsf(to_float(v[(p + i) * TV])), y1 = fabsf(to_float(v[(p + i + 1) * TV]));
-                    m0 = fmaxf(m0, y0 <= FINITE ? y0 : 0.0f);
-                    m1 = fmaxf(m1, y1 <= FINITE ? y1 : 0.0f);
+                for (int i = 0; i < 16; i += 2) m = max3_nan(m, to_float(v[(p + i) * TV]), to_float(v[(p + i + 1) * TV]));
+            if (!(m <= FINITE)) {
+                m = 0.0f;
+#pragma unroll 1
+                for (int p = 0; p < CT; ++p) {
+                    const float y = fabsf(to_float(v[p * TV]));
+                    m = y <= FINITE ? fmaxf(m, y) : m;
                 }
-            sm.vtop[c & 1][row] = fmaxf(m0, m1);
+            }
+            sm.vtop[c & 1][row] = m;
             __syncwarp();
             if (lane == 0) mbar_arrive(b_v + 8 * (c & 1));     // (two barriers: this may be a chunk ahead of those that wait)
             if (++sn == STAGES) { sn = 0; snph ^= 1u; }
@@ -784,9 +788,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             tc_fence_after();
             const float4 mark = sm.scale[row];
             const int first = __float_as_int(mark.z), left = dead || !writes ? 0 : len - c * CT;
+            const bool plain = __all_sync(0xffffffffu, left >= CT && first >= CT);
             // sixteen tokens at a time in a loop: the code of a chunk's roles has to fit the instruction cache
 #pragma unroll 1
-            for (int h = 0; h < 4; ++h) {
+            for (int h = left > 0 ? 0 : 3; h < 4; ++h) {         // (without outputs: the last round, for its barrier)
                 uint32_t q[16], m[16];
                 tc_ld16(tl + C::QS + 64 * ph + 16 * h, q);
                 tc_ld16(tl + C::MU + 16 * h, m);
@@ -796,18 +801,33 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                     __syncwarp();
                     if (lane == 0) mbar_arrive(b_q);
                 }
+                if (left <= 0) break;
                 T* at = o + 16 * h * a.ldo;
-                const float* om4 = sc + W::OM / 4 + 16 * h;
-                const float* eq4 = sc + W::EQ / 4 + 16 * h;
+                const float4* om4 = reinterpret_cast<const float4*>(sc + W::OM / 4 + 16 * h);
+                const float4* eq4 = reinterpret_cast<const float4*>(sc + W::EQ / 4 + 16 * h);
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
-                    const float4 om = *reinterpret_cast<const float4*>(om4 + i), eq = *reinterpret_cast<const float4*>(eq4 + i);
-                    const float omv[4] = {om.x, om.y, om.z, om.w}, eqv[4] = {eq.x, eq.y, eq.z, eq.w};
+                    const float4 om = om4[i / 4], eq = eq4[i / 4];
+                    const float2 a0 = mul2(mul2(make_float2(om.x, om.y), make_float2(mark.y, mark.y)), make_float2(__uint_as_float(m[i]), __uint_as_float(m[i + 1])));
+                    const float2 a1 = mul2(mul2(make_float2(om.z, om.w), make_float2(mark.y, mark.y)), make_float2(__uint_as_float(m[i + 2]), __uint_as_float(m[i + 3])));
+                    const float2 x0 = fma2(mul2(make_float2(eq.x, eq.y), make_float2(mark.x, mark.x)), make_float2(__uint_as_float(q[i]), __uint_as_float(q[i + 1])), a0);
+                    const float2 x1 = fma2(mul2(make_float2(eq.z, eq.w), make_float2(mark.x, mark.x)), make_float2(__uint_as_float(q[i + 2]), __uint_as_float(q[i + 3])), a1);
+                    m[i / 2] = pack2<T>(x0.x, x0.y);
+                    m[i / 2 + 1] = pack2<T>(x1.x, x1.y);
+                }
+                const T* two = reinterpret_cast<const T*>(m);
+                if (plain) {
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        float x = fmaf(__uint_as_float(m[i + u]) * mark.y, omv[u], mark.x * (eqv[u] * __uint_as_float(q[i + u])));
-                        if (16 * h + i + u >= first) x = __int_as_float(0x7fffffff);
-                        if (16 * h + i + u < left) *at = from_float<T>(x);
+                    for (int i = 0; i < 16; ++i) {
+                        *at = two[i];
+                        at += a.ldo;
+                    }
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < 16; ++i) {               // (few chunks: the last of a sequence, or one with a bad token)
+                        const uint32_t word = i < 8 ? (i < 4 ? (i < 2 ? m[0] : m[1]) : (i < 6 ? m[2] : m[3])) : (i < 12 ? (i < 10 ? m[4] : m[5]) : (i < 14 ? m[6] : m[7]));
+                        const T x = reinterpret_cast<const T*>(&word)[i & 1];
+                        if (16 * h + i < left) *at = 16 * h + i < first ? x : from_float<T>(__int_as_float(0x7fffffff));
                         at += a.ldo;
                     }
                 }
