@@ -206,6 +206,9 @@ size_t shvk_gdn_prefill_workspace_bytes(const shvk_gdn_seq_args* a);
 int shvk_gdn_prefill(const shvk_gdn_seq_args* a, void* workspace, size_t workspace_bytes, void* stream);
 /* Device status word of that call: nonzero after a bounded wait inside a kernel gave up (its outputs are unspecified then). */
 int shvk_gdn_prefill_status(int* status_out);
+/* Test launch (see shvk_gemm_tc_rows_starved): no CTA asks for its first chunk, its roles' waits run out after `polls` polls, the
+ * status word is set and every CTA returns, its outputs unwritten or unspecified.  For calls in chunks of 64 tokens only. */
+int shvk_gdn_prefill_starved(const shvk_gdn_seq_args* a, void* workspace, size_t workspace_bytes, int polls, void* stream);
 
 /* What stands between two blocks, in one pass over rows of D values (1 .. 16384): the norm, gate and scale of a block's output, the
  * residual sum, the norm in front of the next block:

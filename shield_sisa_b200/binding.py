@@ -180,6 +180,7 @@ def load_library(experimental: bool = True) -> C.CDLL:
         "shvk_gdn_step": (i32, [C.POINTER(GdnSeqArgs), vp]),
         "shvk_gdn_prefill_workspace_bytes": (sz, [C.POINTER(GdnSeqArgs)]),
         "shvk_gdn_prefill": (i32, [C.POINTER(GdnSeqArgs), vp, sz, vp]),
+        "shvk_gdn_prefill_starved": (i32, [C.POINTER(GdnSeqArgs), vp, sz, i32, vp]),
         "shvk_gdn_prefill_status": (i32, [C.POINTER(i32)]),
         "shvk_block_norm": (i32, [C.POINTER(BlockNormArgs), vp]),
         "shvk_sisa_attn": (i32, [vp, vp, vp, vp, i32, vp]),

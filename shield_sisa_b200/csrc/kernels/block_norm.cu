@@ -328,7 +328,8 @@ template <typename T, typename TH> int launch_block_norm(const shvk_block_norm_a
     const bool vec = on_group(a.x) && on_group(a.h_in) && on_group(a.h_out) && on_group(a.xn) && (!gate_rows || on_group(a.gate)) &&
                      (!a.h_in || (a.ldh_in & 7) == ld) && (!a.h_out || (a.ldh_out & 7) == ld) && (!a.xn || (a.ldxn & 7) == ld) &&
                      (!gate_rows || (a.ldgate & 7) == ld) && (a.heads == 1 || (ld == 0 && a.D % 8 == 0));
-    const int P = a.rows == 1 ? 1 : ld == 0 ? 1 : ld % 2 ? 8 : ld % 4 ? 4 : 2, nvec = (a.D + (P > 1 ? 7 : 0) + 7) / 8;
+    // (by the pitch alone, for one row too: a row's sums are taken in the same order alone and among others)
+    const int P = ld == 0 ? 1 : ld % 2 ? 8 : ld % 4 ? 4 : 2, nvec = (a.D + (P > 1 ? 7 : 0) + 7) / 8;
     if (!vec || nvec > 2048) {
         const int smem = a.D * int(sizeof(float));
         const cudaError_t e = cudaFuncSetAttribute(block_norm_any_kernel<T, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);

@@ -627,7 +627,8 @@ extern "C" size_t shvk_gdn_prefill_workspace_bytes(const shvk_gdn_seq_args* a) {
     return size_t(prefill_chunks(*a)) * size_t(a->HV) * size_t(PW_BYTES);
 }
 
-extern "C" int shvk_gdn_prefill(const shvk_gdn_seq_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+namespace {
+int prefill(const shvk_gdn_seq_args* a, void* workspace, size_t workspace_bytes, void* stream, int starve_polls) {
     using namespace sb;
     if (const int e = check_gdn_seq(a)) return e;
     if (a->dtype == DT_F32) return int(cudaErrorInvalidValue);
@@ -635,7 +636,17 @@ extern "C" int shvk_gdn_prefill(const shvk_gdn_seq_args* a, void* workspace, siz
     if (!workspace || !aligned16(workspace) || workspace_bytes < shvk_gdn_prefill_workspace_bytes(a)) return int(cudaErrorInvalidValue);
     cudaStream_t s = cudaStream_t(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    if (takes_tc(*a)) return gdn_prefill_tc(*a, ws, s);
+    if (takes_tc(*a)) return gdn_prefill_tc(*a, ws, s, starve_polls);
+    if (starve_polls) return int(cudaErrorInvalidValue);         // the other form waits for nothing that could stay away
     if (a->dtype == DT_BF16) return a->DK == 64 ? launch_prefill<__nv_bfloat16, 64>(*a, ws, s) : launch_prefill<__nv_bfloat16, 128>(*a, ws, s);
     return a->DK == 64 ? launch_prefill<__half, 64>(*a, ws, s) : launch_prefill<__half, 128>(*a, ws, s);
+}
+}  // namespace
+
+extern "C" int shvk_gdn_prefill(const shvk_gdn_seq_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    return prefill(a, workspace, workspace_bytes, stream, 0);
+}
+
+extern "C" int shvk_gdn_prefill_starved(const shvk_gdn_seq_args* a, void* workspace, size_t workspace_bytes, int polls, void* stream) {
+    return prefill(a, workspace, workspace_bytes, stream, polls > 1 ? polls : 1);
 }

@@ -471,7 +471,7 @@ template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setma
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <typename T, int DK, int STAGES>
-__global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(const __grid_constant__ WalkMaps maps, const shvk_gdn_seq_args a, const uint8_t* __restrict__ ws, const WalkSegments seg, uint32_t polls) {
+__global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(const __grid_constant__ WalkMaps maps, const shvk_gdn_seq_args a, const uint8_t* __restrict__ ws, const WalkSegments seg, uint32_t polls, bool starve) {
     constexpr bool FINE = std::is_same<T, __half>::value;
     using W = Ws<FINE>;
     using Sm = WalkSmem<DK, FINE, STAGES>;
@@ -930,7 +930,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 const uint32_t kq = smem_u32(sm.st[s].kq), vt = smem_u32(sm.st[s].v), wt = smem_u32(sm.st[s].w);
                 const int y = start + c * CT;
                 wait(empty(s), sph ^ 1u);
-                if (!dead && lead) {                             // rows past the sequence are another's, past the last zeros: both unused
+                if (!dead && lead && !(starve && c == 0)) {      // rows past the sequence are another's, past the last zeros: both unused
                     mbar_expect_tx(wfull(s), W::BYTES + 2 * CT * DK * 2 + CT * TV * 2);
 #pragma unroll
                     for (int h = 0; h < DK / 64; ++h) {
@@ -1078,7 +1078,7 @@ inline size_t chunk_bytes(const shvk_gdn_seq_args& a) {
     return (size_t(a.n_tokens / CT + a.n_seq + 1) * size_t(a.HV) * each + 15) / 16 * 16;
 }
 
-template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s) {
+template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s, uint32_t polls, bool starve) {
     constexpr bool FINE = std::is_same<T, __half>::value;
     constexpr int STAGES = 3;
     const int chunks = segment_chunks(a);
@@ -1104,19 +1104,19 @@ template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t*
         return int(cudaErrorInvalidValue);
     WalkSegments seg{};
     if (!chunks) {
-        gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(ctas), TC_THREADS, smem, s>>>(maps, a, ws, seg, PREFILL_POLLS);
+        gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(ctas), TC_THREADS, smem, s>>>(maps, a, ws, seg, polls, starve);
         return int(cudaGetLastError());
     }
     seg.chunks = chunks;
     seg.x = reinterpret_cast<float*>(ws + chunk_bytes(a));
     seg.phi = seg.x + segments * a.HV * DK * a.DV;
     seg.pass = 1;
-    gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(ctas), TC_THREADS, smem, s>>>(maps, a, ws, seg, PREFILL_POLLS);
+    gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(ctas), TC_THREADS, smem, s>>>(maps, a, ws, seg, polls, starve);
     if ((e = cudaGetLastError()) != cudaSuccess) return int(e);
     gdn_prefill_tc_join_kernel<DK><<<unsigned((long long)a.n_seq * a.HV * (a.DV / JC)), JOIN_THREADS, 0, s>>>(a, seg);
     if ((e = cudaGetLastError()) != cudaSuccess) return int(e);
     seg.pass = 2;
-    gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(segments * a.HV * splits), TC_THREADS, smem, s>>>(maps, a, ws, seg, PREFILL_POLLS);
+    gdn_prefill_tc_walk_kernel<T, DK, STAGES><<<unsigned(segments * a.HV * splits), TC_THREADS, smem, s>>>(maps, a, ws, seg, polls, starve);
     return int(cudaGetLastError());
 }
 
@@ -1126,9 +1126,11 @@ size_t gdn_prefill_tc_workspace(const shvk_gdn_seq_args& a) {
     const int chunks = segment_chunks(a);
     return chunk_bytes(a) + (chunks ? size_t(segment_count(a, chunks)) * size_t(a.HV) * size_t(a.DK) * size_t(a.DK + a.DV) * sizeof(float) : 0);
 }
-int gdn_prefill_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s) {
-    if (a.dtype == DT_BF16) return a.DK == 64 ? launch_tc<__nv_bfloat16, 64>(a, ws, s) : launch_tc<__nv_bfloat16, 128>(a, ws, s);
-    return a.DK == 64 ? launch_tc<__half, 64>(a, ws, s) : launch_tc<__half, 128>(a, ws, s);
+int gdn_prefill_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s, int starve_polls) {
+    const bool starve = starve_polls > 0;
+    const uint32_t polls = starve ? uint32_t(starve_polls < 256 ? 256 : starve_polls > (1 << 17) ? 1 << 17 : starve_polls) : PREFILL_POLLS;
+    if (a.dtype == DT_BF16) return a.DK == 64 ? launch_tc<__nv_bfloat16, 64>(a, ws, s, polls, starve) : launch_tc<__nv_bfloat16, 128>(a, ws, s, polls, starve);
+    return a.DK == 64 ? launch_tc<__half, 64>(a, ws, s, polls, starve) : launch_tc<__half, 128>(a, ws, s, polls, starve);
 }
 
 }  // namespace sb

@@ -64,6 +64,13 @@ def test_prefill_refuses(L, kw):
         assert L.shvk_gdn_prefill_workspace_bytes(C.byref(a)) == 0
 
 
+def test_starved_launch_refuses_what_waits_for_nothing(L):
+    a = good(DV=64, ldv=256, ldo=256)
+    assert L.shvk_gdn_prefill_starved(C.byref(a), 0x200000, 1 << 40, 256, None) == INVALID
+    assert L.shvk_gdn_prefill_starved(None, 0x200000, 1 << 40, 256, None) == INVALID
+    assert L.shvk_gdn_prefill_status(None) == INVALID
+
+
 def test_prefill_refuses_its_workspace(L):
     a = good()
     need = L.shvk_gdn_prefill_workspace_bytes(C.byref(a))
@@ -598,6 +605,77 @@ def test_captured_replayed_and_on_two_streams(L, form):
         launch(L, form, w)
         torch.cuda.synchronize()
         assert torch.equal(z["o"], w["o"])
+
+
+@gpu
+@pytest.mark.parametrize("layer_type", ["bf16", "fp16"])
+def test_a_layer_in_service(L, layer_type):
+    """The operators as a layer runs them: a prompt by the chunked form, the gated norm over each head's values, then the residual sum and
+    the next block's norm; then two more tokens by the step form and the same norms.  Against the formulas in float64 on the same inputs,
+    each operator's outputs taken as the next one's inputs (its own tests bound it on those)."""
+    import torch
+    t = {"bf16": torch.bfloat16, "fp16": torch.float16}[layer_type]
+    hv, dv, d = 4, 128, 512
+    lens = [70, 200, 1]
+    x = make(layer_type, lens, 2, hv, 128, dv, seed=71, tail=0)
+    gen = torch.Generator(device="cuda").manual_seed(72)
+    rn = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
+    o_w, next_w = 1 + 0.2 * rn(dv), 1 + 0.2 * rn(d)
+    code, s = CODES[layer_type], torch.cuda.current_stream().cuda_stream
+
+    def norms(o, rows):
+        """(gated heads, residual stream, normalised rows) by the calls, and checked."""
+        gate, h = rn(rows, hv * dv).to(t), 3 * rn(rows, d)
+        on, xn, h_out = torch.empty(rows, hv * dv, device="cuda", dtype=t), torch.empty(rows, d, device="cuda", dtype=t), h.clone()
+        a = binding.BlockNormArgs(rows=rows, heads=hv, D=dv, x=o.data_ptr(), ldx=hv * dv, x_dtype=code, post_w=o_w.data_ptr(), gate=gate.data_ptr(),
+                                  ldgate=hv * dv, gate_dtype=code, gate_act=1, scale=1.0, h_out=on.data_ptr(), ldh_out=hv * dv, h_dtype=code, eps=1e-6)
+        assert L.shvk_block_norm(C.byref(a), s) == 0
+        b = binding.BlockNormArgs(rows=rows, heads=1, D=d, x=on.data_ptr(), ldx=d, x_dtype=code, scale=0.7, h_in=h_out.data_ptr(), ldh_in=d,
+                                  h_out=h_out.data_ptr(), ldh_out=d, h_dtype=0, pre_w=next_w.data_ptr(), xn=xn.data_ptr(), ldxn=d, xn_dtype=code, eps=1e-6)
+        assert L.shvk_block_norm(C.byref(b), s) == 0
+        o64, g64 = o.double().view(rows, hv, dv), gate.double().view(rows, hv, dv)
+        want = o64 / (o64.square().mean(-1, keepdim=True) + 1e-6).sqrt() * o_w.double() * g64 * torch.sigmoid(g64)
+        half, err = torch.finfo(t).eps / 2, 128 * 2.0 ** -24
+        assert float(((on.double().view_as(want) - want).abs() - (half + err) * want.abs() - 2.0 ** -25).max()) <= 0
+        want_h = h.double() + on.double() * float(np.float32(0.7))
+        assert float(((h_out.double() - want_h).abs() - err * (h.double().abs() + on.double().abs())).max()) <= 0
+        z = h_out.double()
+        want_n = z / (z.square().mean(-1, keepdim=True) + 1e-6).sqrt() * next_w.double()
+        assert float(((xn.double() - want_n).abs() - (half + 2 * err) * want_n.abs() - err * 4).max()) <= 0
+    check(L, "prefill", x)
+    norms(x["o"], sum(lens))
+    for token in range(2):
+        y = make(layer_type, [1, 1, 1], 2, hv, 128, dv, seed=73 + token, tail=0)
+        y["states"], y["n_slots"], y["slot_in"], y["slot_out"] = x["states"], x["n_slots"], x["slot_out"], x["slot_out"]
+        check(L, "step", y)
+        norms(y["o"], 3)
+
+
+@gpu
+def test_waits_that_run_out_end_the_call(L):
+    """Nothing is copied for the first chunks: every role gives up in turn, the status word says so, and the next call is right."""
+    import subprocess
+    import sys
+    code = """
+import ctypes as C, torch
+from tests import test_gdn_seq as T
+from shield_sisa_b200 import binding
+L = binding.load_library(True)
+x = T.make("bf16", [200, 130], 2, 4, 128, 128, seed=3)
+T.launch(L, "prefill", x)
+torch.cuda.synchronize()
+status = C.c_int(-1)
+assert L.shvk_gdn_prefill_status(C.byref(status)) == 0 and status.value == 0
+a = T.args(x)
+assert L.shvk_gdn_prefill_starved(C.byref(a), x["ws"].data_ptr(), x["ws"].numel(), 256, torch.cuda.current_stream().cuda_stream) == 0
+torch.cuda.synchronize()
+assert L.shvk_gdn_prefill_status(C.byref(status)) == 0 and status.value > 0
+T.check(L, "prefill", T.make("bf16", [200, 130], 2, 4, 128, 128, seed=4))
+print("ended with status", status.value)
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=str(__import__("tests.helpers", fromlist=["ROOT"]).ROOT))
+    assert r.returncode == 0, r.stderr[-2000:]                 # in a process of its own: the word stays set
+    assert "ended with status" in r.stdout
 
 
 @gpu
