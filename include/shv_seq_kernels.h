@@ -196,7 +196,7 @@ typedef struct shvk_gdn_seq_args {
 } shvk_gdn_seq_args;
 /* Token by token in fp32, any storage type: new tokens of live sequences (one, or a few), and the exact tier's form of any length. */
 int shvk_gdn_step(const shvk_gdn_seq_args* a, void* stream);
-/* In chunks of 64 or (DV no multiple of 128, short sequences) 16 tokens on the tensor cores, dtype bf16 or fp16: prompts and histories.  Outputs and states are those of the rule to
+/* In chunks of 64 or (short sequences, most DV that are no multiple of 128) 16 tokens on the tensor cores, dtype bf16 or fp16: prompts and histories.  Outputs and states are those of the rule to
  * float32's accuracy before o is rounded (in a value column, to 2^-32 of the chunk's largest |v - exp(.) S^T k|: what follows a decay
  * to nothing does not show it unless the state before it was some 2^20 times larger).  Two launches; four where long sequences are too few to fill the GPU and are
  * walked in segments (by n_seq, n_tokens and the head sizes: a sequence's bits follow from those too).  `workspace` (device, 16-byte

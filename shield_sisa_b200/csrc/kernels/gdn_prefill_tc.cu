@@ -1,4 +1,4 @@
-// The chunked delta rule with kept states for heads of 128 values (or a multiple): chunks of 64 tokens on tcgen05.  The algebra, the
+// The chunked delta rule with kept states for heads of 128 values (or a multiple of 64): chunks of 64 tokens on tcgen05.  The algebra, the
 // pieces and the scales are those of gdn_prefill.cu, with 64 for 16:
 //
 //     U = T (V - diag(e) K S0),  O = M U + diag(e) Q S0,  S = e_64 S0 + K^T diag(exp(c_64 - c_j)) U
@@ -480,9 +480,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
     extern __shared__ uint8_t walk_raw[];
     Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(walk_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int splits = a.DV / TV, kinds = splits + (seg.pass == 1), split = int(blockIdx.x % unsigned(kinds));
+    const int splits = (a.DV + TV - 1) / TV, kinds = splits + (seg.pass == 1), split = int(blockIdx.x % unsigned(kinds));
     const int nh = int(blockIdx.x / unsigned(kinds)), head = nh % a.HV, khead = head / (a.HV / a.HK);
     const bool phi = split == splits;                            // this CTA makes the segment's Phi
+    const int columns = phi ? DK : min(a.DV - split * TV, TV);   // the lanes behind them walk along, from zero states to nowhere
     int n = nh / a.HV, at = 0, segment = 0;
     if (seg.chunks) {                                            // the last sequence whose first segment is not behind this one
         segment = n;
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         if (out >= 0 && out != in)
             for (int i = tid; i < DK * TV; i += TC_THREADS) {
                 const long long e = (i / TV) * (long long)a.DV + i % TV;
-                to[e] = from ? from[e] : 0.0f;
+                if (i % TV < columns) to[e] = from ? from[e] : 0.0f;
             }
         return;
     }
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             const float* src = from + (long long)(half * KH) * a.DV + row;
 #pragma unroll
             for (int i = 0; i < KH; ++i) {
-                S[i] = from ? src[i * (long long)a.DV] : phi && row == half * KH + i ? 1.0f : 0.0f;
+                S[i] = from && row < columns ? src[i * (long long)a.DV] : phi && row == half * KH + i ? 1.0f : 0.0f;
                 mine = fmaxf(mine, fabsf(S[i]));
             }
             sm.meet1[half][row] = mine;
@@ -740,7 +741,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             inv = pow2_biased(254 - exponent_of(sig));
             if (++s == STAGES) { s = 0; sph ^= 1u; }
         }
-        if (to && !dead && (!phi || row < DK)) {
+        if (to && !dead && row < columns) {
             float* dst = to + (half * KH) * to_k + row * to_c;
 #pragma unroll
             for (int i = 0; i < KH; ++i) dst[i * to_k] = S[i] * inv;
@@ -787,7 +788,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             wait(b_o, ph);
             tc_fence_after();
             const float4 mark = sm.scale[row];
-            const int first = __float_as_int(mark.z), left = dead || !writes ? 0 : len - c * CT;
+            const int first = __float_as_int(mark.z), left = dead || !writes || 32 * quad >= columns ? 0 : len - c * CT;     // (columns: 64 or 128)
             const bool plain = __all_sync(0xffffffffu, left >= CT && first >= CT);
             // sixteen tokens at a time in a loop: the code of a chunk's roles has to fit the instruction cache
 #pragma unroll 1
@@ -1061,7 +1062,7 @@ template <int DK> __global__ void __launch_bounds__(JOIN_THREADS) gdn_prefill_tc
 // a join's segment about 1,000, the two launches more about as much as two chunks) for sequences of the average length; segments are not
 // shorter than 13 chunks, so that their states take less room than their chunks' T and M.
 inline int segment_chunks(const shvk_gdn_seq_args& a) {
-    const long long sms = device_sms(), splits = a.DV / TV, heads = (long long)a.n_seq * a.HV, chunks = a.n_tokens / CT / a.n_seq;
+    const long long sms = device_sms(), splits = (a.DV + TV - 1) / TV, heads = (long long)a.n_seq * a.HV, chunks = a.n_tokens / CT / a.n_seq;
     auto waves = [&](long long ctas) { return (ctas + sms - 1) / sms; };
     double best = 0.9 * double(chunks * waves(heads * splits));
     int found = 0;
@@ -1082,7 +1083,7 @@ template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t*
     constexpr bool FINE = std::is_same<T, __half>::value;
     constexpr int STAGES = 3;
     const int chunks = segment_chunks(a);
-    const long long segments = chunks ? segment_count(a, chunks) : 0, splits = a.DV / TV;
+    const long long segments = chunks ? segment_count(a, chunks) : 0, splits = (a.DV + TV - 1) / TV;
     const long long items = (a.n_tokens / CT + a.n_seq + 1) * a.HV, ctas = (chunks ? segments : a.n_seq) * a.HV * (splits + (chunks ? 1 : 0));
     if (items > 0x7fffffff || ctas > 0x7fffffff) return int(cudaErrorInvalidValue);
     cudaError_t e;

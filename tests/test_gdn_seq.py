@@ -317,6 +317,7 @@ def test_prefill_of_any_size_of_numbers(L, kind, what):
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "fp16"])
 @pytest.mark.parametrize("layout,lens", [((1, 1, 128, 128), [4099]), ((1, 2, 64, 128), [3000, 64 * 13 * 3]), ((1, 1, 128, 256), [2496]),
+                                         ((1, 1, 128, 64), [4000]), ((1, 1, 64, 192), [70, 5100]),
                                          ((1, 1, 64, 128), [0, 5000, 1, 900]), ((1, 1, 64, 128), [0, 9000, 1, 2000])], ids=str)
 def test_few_long_sequences_are_walked_in_segments(L, kind, layout, lens):
     """Segments of at least 13 chunks: whole ones, a last one of a few tokens, sequences of one segment and of none among them; states
