@@ -299,8 +299,10 @@ int launch_rows(const shvk_block_norm_args& a, int P, int threads, cudaStream_t 
     const int groups = ROWT ? threads / ROWT : 1, span = (ROWT ? ROWT : threads) * NV * 8;
     const int smem = 3 * span * int(sizeof(float));
     static_assert(3 * 4 * 512 * 8 * sizeof(float) <= 200 * 1024, "the longest row's weights fit");
-    const cudaError_t e = cudaFuncSetAttribute(block_norm_kernel<T, TH, NV, ROWT, EDGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return int(e);
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(block_norm_kernel<T, TH, NV, ROWT, EDGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return int(e);
+    }
     const long long need = ((a.rows * a.heads + P - 1) / P + groups - 1) / groups * P;     // CTAs of one pass over the rows
     const int resident = ROWT ? 4 : NV == 1 ? 1024 / threads : threads > 256 ? 1 : 512 / threads;      // CTAs of an SM, by registers
     const long long most = (long long)device_sms() * resident / P * P;

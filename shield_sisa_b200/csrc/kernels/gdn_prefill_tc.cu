@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(128, FINE_PREP<T> ? 3 : 4) gdn_prefill_tc_prep
         const float most = warp_max(rk * sqrtf(k2));             // the longest key (of 32 tokens)
         if (lane == 0 && warp < 2) sm.top[warp] = most;
     }
-    // exp(c_i - c_j) of a block below the diagonal is exp(c_i - c_e) exp(c_e - c_j), e the last token of j's block
+    // exp(c_i - c_j) of a block below the diagonal is exp(c_i - c_e) exp(c_e - c_j), e the last token of j's block.
     if (tid < CT) {
         sm.col[tok] = expf(float(sm.cum[tok | 15] - cs));
         sm.row[0][tok] = expf(float(cs - sm.cum[15]));
@@ -392,6 +392,12 @@ struct WalkSegments {
 };
 __device__ __forceinline__ int first_segment(int first_chunk, int n, int chunks) { return first_chunk / chunks + n; }
 
+// (out of line: the waits' own code has to stay short)
+__device__ __noinline__ void give_up(int* abort, int warp) {
+    *abort = 1;
+    atomicCAS(&g_prefill_status, 0, 1 + (warp < COMPUTE ? 0 : warp < WARP_MMA ? 1 : warp - 10));
+}
+
 struct WalkMaps { CUtensorMap q, k, v; };                        // 64 rows x 64 columns swizzled, 64 x 128 columns of V as they are
 
 template <int DK, bool FINE, int STAGES> struct WalkSmem {
@@ -414,13 +420,9 @@ template <int DK> struct Cols {
 };
 
 // D[128 x N] (+)= A (tensor memory, fp16) x B (shared memory)
-// (issued by the lane that `lead` names, without a branch: the operands stay in uniform registers)
-__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 e, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)), "r"(lead) : "memory");
-}
-__device__ __forceinline__ void commit_if(uint32_t lead, uint32_t bar) {
-    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
 }
 // Waits for a phase of a barrier, at most `polls` times the hardware's own patience; a few instructions, for loops that must stay short.
 __device__ __forceinline__ bool mbar_wait_counted(uint32_t bar, uint32_t parity, uint32_t polls) {
@@ -552,8 +554,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         if (__any_sync(0xffffffffu, !mbar_wait_counted(bar, parity & 1u, polls))) {
             dead = true;
             polls = 1;
-            sm.abort = 1;
-            atomicCAS(&g_prefill_status, 0, 1 + (warp < COMPUTE ? 0 : warp < WARP_MMA ? 1 : warp - 10));
+            give_up(&sm.abort, warp);
         }
     };
     constexpr float FINITE = 3.402823466e38f;
@@ -842,7 +843,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
         regs_down<104>();
         if (warp == WARP_MMA) {
             // --------------------------------------------------------------------------------------- the products
-            const uint32_t lead = elect_one();
+            const bool lead = elect_one();
+            // (in loops: unrolled, the products of a chunk take 13 KB of code, for which the other roles' leaves the instruction cache: 8 % slower)
             auto products = [&](int c, int s, uint32_t sph) {
                 const uint32_t ph = uint32_t(c) & 1u;
                 const uint32_t kq = smem_u32(sm.st[s].kq), wt = smem_u32(sm.st[s].w);
@@ -852,74 +854,74 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 wait(b_s, ph);
                 tc_fence_after();
                 const uint32_t qs = C::QS + 64 * ph;             // (read by the outputs of chunk c - 2 before M U of chunk c - 1 was let in)
-                if (!dead) {
+                if (!dead && lead) {
                     const uint64_t b0 = smem_desc_sw128(kq);
-#pragma unroll
+#pragma unroll 1
                     for (int p = 0; p < DK / 16; ++p) {          // (K S0)^T, for which the chain waits
                         const uint64_t b = b0 + uint64_t((p >> 2) * (HALF / 16) + 2 * (p & 3));
-                        mma_ts(lead, C::R, C::S + 8 * p, b, id64, p > 0);
-                        mma_ts(lead, C::R, C::S + DK / 2 + 8 * p, b, id64, true);
+                        mma_ts(C::R, C::S + 8 * p, b, id64, p > 0);
+                        mma_ts(C::R, C::S + DK / 2 + 8 * p, b, id64, true);
                     }
-                    commit_if(lead, b_r);
-#pragma unroll
+                    tc_commit(b_r);
+#pragma unroll 1
                     for (int p = 0; p < DK / 16; ++p) {          // (Q S0)^T
                         const uint64_t b = b0 + uint64_t((p >> 2) * (HALF / 16) + 2 * (p & 3) + CT * 128 / 16);
-                        mma_ts(lead, qs, C::S + 8 * p, b, id64, p > 0);
-                        if (FINE) mma_ts(lead, qs, C::S + DK / 2 + 8 * p, b, id64, true);
+                        mma_ts(qs, C::S + 8 * p, b, id64, p > 0);
+                        if (FINE) mma_ts(qs, C::S + DK / 2 + 8 * p, b, id64, true);
                     }
                 }
                 wait(wfull(s), sph);
                 wait(b_w, ph);
                 tc_fence_after();
-                if (!dead) {
+                if (!dead && lead) {
                     const uint64_t t0 = desc_plain(wt, 128, 256);
-#pragma unroll
+#pragma unroll 1
                     for (int kk = 0; kk < 4; ++kk) {             // T is triangular: tokens 16 kk .. reach columns 16 kk .. 63
                         const uint64_t th = t0 + uint64_t((W::T + tri_step(kk)) / 16), tlo = t0 + uint64_t((W::TL + tri_step(kk)) / 16);
                         const uint32_t id = idesc_f16(64 - 16 * kk, false), d = C::R + 16 * kk;
-                        mma_ts(lead, d, C::P + 8 * kk, th, id, kk > 0);
-                        mma_ts(lead, d, C::P + 8 * kk, tlo, id, true);
-                        mma_ts(lead, d, C::P + 32 + 8 * kk, th, id, true);
+                        mma_ts(d, C::P + 8 * kk, th, id, kk > 0);
+                        mma_ts(d, C::P + 8 * kk, tlo, id, true);
+                        mma_ts(d, C::P + 32 + 8 * kk, th, id, true);
                     }
-                    commit_if(lead, b_u);
+                    tc_commit(b_u);
                 }
                 wait(b_d, ph);
                 tc_fence_after();
-                if (!dead) {
+                if (!dead && lead) {
                     constexpr uint32_t idk = idesc_f16(DK, true);
                     const uint64_t b0 = desc_mn(kq, HALF);
-#pragma unroll
+#pragma unroll 1
                     for (int kk = 0; kk < 4; ++kk) {
-                        mma_ts(lead, C::P, C::S + 8 * kk, b0 + uint64_t(128 * kk), idk, kk > 0);
-                        mma_ts(lead, C::P, C::S + 32 + 8 * kk, b0 + uint64_t(128 * kk), idk, true);
+                        mma_ts(C::P, C::S + 8 * kk, b0 + uint64_t(128 * kk), idk, kk > 0);
+                        mma_ts(C::P, C::S + 32 + 8 * kk, b0 + uint64_t(128 * kk), idk, true);
                     }
-                    commit_if(lead, b_p);
+                    tc_commit(b_p);
                 }
                 wait(b_q, ph ^ 1u);                   // the last chunk's outputs are read
                 tc_fence_after();
-                if (!dead) {
+                if (!dead && lead) {
                     const uint64_t m0 = desc_plain(wt, 128, 256);
-#pragma unroll
+#pragma unroll 1
                     for (int kk = 0; kk < 4; ++kk) {
                         const uint64_t mh = m0 + uint64_t((W::M + tri_step(kk)) / 16);
                         const uint32_t id = idesc_f16(64 - 16 * kk, false), d = C::MU + 16 * kk, u = C::R + 16 * kk;
-                        mma_ts(lead, d, u, mh, id, kk > 0);
+                        mma_ts(d, u, mh, id, kk > 0);
                         if (FINE) {
-                            mma_ts(lead, d, u, m0 + uint64_t((W::ML + tri_step(kk)) / 16), id, true);
-                            mma_ts(lead, d, u + 8, mh, id, true);
+                            mma_ts(d, u, m0 + uint64_t((W::ML + tri_step(kk)) / 16), id, true);
+                            mma_ts(d, u + 8, mh, id, true);
                         }
                     }
-                    commit_if(lead, b_o);
-                    commit_if(lead, empty(s));
+                    tc_commit(b_o);
+                    tc_commit(empty(s));
                 }
             };
-            // (a stage's addresses have to be constants: computed, they cost every product a move to a uniform register, 30 of 65 cycles)
+            int s = 0;
             uint32_t sph = 0;
 #pragma unroll 1
-            for (int c0 = 0; c0 < NB; c0 += STAGES, sph ^= 1u)
-#pragma unroll
-                for (int s = 0; s < STAGES; ++s)
-                    if (c0 + s < NB) products(c0 + s, s, sph);
+            for (int c = 0; c < NB; ++c) {
+                products(c, s, sph);
+                if (++s == STAGES) { s = 0; sph ^= 1u; }
+            }
         } else if (warp == WARP_COPY) {
             // --------------------------------------------------------------------------------------- copies
             const uint8_t* src = ws + ((long long)(first_chunk(rows, n) + c0) * a.HV + head) * W::BYTES;
