@@ -170,7 +170,8 @@ int shvk_gdn_chunked(const void* q, const void* k, const void* v, const float* g
  * may have no rows, and rows behind the last sequence are neither read nor written.  q, k, v, o in `dtype` with row pitches in
  * elements, head h at h * DK (q, k) or h * DV (v, o) of its row; HK query / key heads, HV value heads, value head h uses key head
  * h / (HV / HK).  g (log decay) and beta fp32, row pitch ldgb.  l2norm != 0: q and k are divided by sqrt(x.x + 1e-6) first; q is
- * multiplied by `scale` either way.
+ * multiplied by `scale` either way.  g is meant to be at most 0 (a state grows without bound otherwise, and sums of positive g over 64
+ * tokens past some 80 leave fp32); exp(g) is 0 for g below about -104, -infinity too.
  *     S <- exp(g) S + k u^T,  u = beta (v - exp(g) S^T k),  o = S^T q
  * States are fp32 [n_slots][HV][DK][DV].  Sequence n starts from slot slot_in[n] and leaves its last state in slot slot_out[n]; a
  * value outside [0, n_slots), or a NULL array, means a zero state and a state that is not kept.  The two may name the same slot.  A
@@ -196,16 +197,21 @@ typedef struct shvk_gdn_seq_args {
 } shvk_gdn_seq_args;
 /* Token by token in fp32, any storage type: new tokens of live sequences (one, or a few), and the exact tier's form of any length. */
 int shvk_gdn_step(const shvk_gdn_seq_args* a, void* stream);
-/* In chunks of 64 or (short sequences, most DV that are no multiple of 128) 16 tokens on the tensor cores, dtype bf16 or fp16: prompts and histories.  Outputs and states are those of the rule to
- * float32's accuracy before o is rounded (in a value column, to 2^-32 of the chunk's largest |v - exp(.) S^T k|: what follows a decay
- * to nothing does not show it unless the state before it was some 2^20 times larger).  Two launches; four where long sequences are too few to fill the GPU and are
- * walked in segments (by n_seq, n_tokens and the head sizes: a sequence's bits follow from those too).  `workspace` (device, 16-byte
- * aligned, at least as many bytes as shvk_gdn_prefill_workspace_bytes(a) says, contents irrelevant) holds what they hand on: calls
- * that may overlap need their own.  Its size follows from the counts, sizes and type; it is 0 for arguments that the call refuses. */
+/* In chunks of 64 or (short sequences, most DV that are no multiple of 128) 16 tokens on the tensor cores, dtype bf16 or fp16: prompts
+ * and histories.  Outputs and states are those of the rule to float32's accuracy before o is rounded (in a value column, to 2^-32 of the
+ * chunk's largest |v - exp(.) S^T k|: what follows a decay to nothing does not show it unless the state before it was some 2^20 times
+ * larger).  Two launches; four where long sequences are too few to fill the GPU and are walked in segments (by n_seq, n_tokens and the
+ * head sizes: a sequence's bits follow from those too).  `workspace` (device, 16-byte aligned, at least as many bytes as
+ * shvk_gdn_prefill_workspace_bytes(a) says, contents irrelevant) holds what they hand on: calls that may overlap need their own.  Its
+ * size follows from the counts, sizes and type; it is 0 for arguments that the call refuses. */
 size_t shvk_gdn_prefill_workspace_bytes(const shvk_gdn_seq_args* a);
 int shvk_gdn_prefill(const shvk_gdn_seq_args* a, void* workspace, size_t workspace_bytes, void* stream);
-/* Device status word of that call: nonzero after a bounded wait inside a kernel gave up (its outputs are unspecified then). */
+/* Status word of that call, one per device and process: nonzero after a bounded wait inside a kernel gave up (the call's outputs are
+ * unspecified then), until it is cleared.  The async forms read it into host memory behind the stream's work, and clear it, as
+ * shvk_status_fetch_async and shvk_status_clear_async do with the words of the clips' kernels, of which it is none. */
 int shvk_gdn_prefill_status(int* status_out);
+int shvk_gdn_prefill_status_fetch_async(int* host_word, void* stream);
+int shvk_gdn_prefill_status_clear_async(void* stream);
 /* Test launch (see shvk_gemm_tc_rows_starved): no CTA asks for its first chunk, its roles' waits run out after `polls` polls, the
  * status word is set and every CTA returns, its outputs unwritten or unspecified.  For calls in chunks of 64 tokens only. */
 int shvk_gdn_prefill_starved(const shvk_gdn_seq_args* a, void* workspace, size_t workspace_bytes, int polls, void* stream);

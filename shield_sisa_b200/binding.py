@@ -182,6 +182,8 @@ def load_library(experimental: bool = True) -> C.CDLL:
         "shvk_gdn_prefill": (i32, [C.POINTER(GdnSeqArgs), vp, sz, vp]),
         "shvk_gdn_prefill_starved": (i32, [C.POINTER(GdnSeqArgs), vp, sz, i32, vp]),
         "shvk_gdn_prefill_status": (i32, [C.POINTER(i32)]),
+        "shvk_gdn_prefill_status_fetch_async": (i32, [vp, vp]),
+        "shvk_gdn_prefill_status_clear_async": (i32, [vp]),
         "shvk_block_norm": (i32, [C.POINTER(BlockNormArgs), vp]),
         "shvk_sisa_attn": (i32, [vp, vp, vp, vp, i32, vp]),
         "shvk_sisa_attn_h16": (i32, [vp, vp, vp, vp, vp, i32, vp]),

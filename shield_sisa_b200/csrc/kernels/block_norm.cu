@@ -47,7 +47,7 @@ template <typename T> __device__ __forceinline__ void put8(T* p, const float (&v
 template <typename T> struct Raw { uint4 w[sizeof(T) == 4 ? 2 : 1]; };
 // The values [lo, hi) of a group, the others as it may be: the whole group in one or two accesses where all of it lies in the array
 // (`whole`: everywhere but at an array's end), else value by value.  (Value by value at every row's edges, loads waited for one another:
-// 189 us instead of 58 for 16,384 rows of 2,047.)
+// 189 us for 16,384 rows of 2,047, now 95.)
 template <typename T> __device__ __forceinline__ Raw<T> get_raw(const T* p, int lo, int hi, bool whole) {
     Raw<T> r;
     if (whole) {
@@ -94,8 +94,8 @@ template <typename T> __device__ __forceinline__ void gate8(float (&x)[8], const
     }
 }
 
-// ROWT: threads of a row: 8, 16, 32, or 0 = the whole CTA.  EDGE: a group may reach over a row's ends.  P: classes of rows (1 where every row starts on a group).  The next row's values
-// are asked for before this one's are used (not with four groups a thread: no registers).
+// ROWT: threads of a row: 8, 16, 32, or 0 = the whole CTA.  EDGE: a group may reach over a row's ends.  P: classes of rows (1 where every row
+// starts on a group).  The next row's values are asked for before this one's are used (not with four groups a thread: no registers).
 template <typename T, typename TH, int NV, int ROWT, bool EDGE>
 __global__ void __launch_bounds__(ROWT ? 128 : 512, ROWT ? 4 : NV == 1 ? 2 : 1)
 block_norm_kernel(const shvk_block_norm_args a, int P) {

@@ -14,6 +14,10 @@
 // that the walk keeps or finds anew.  On the output's way, where the caller rounds to 16 bits, one piece is enough for bf16 (its step is
 // 2^-8, a piece's 2^-11); for fp16 outputs there are two here as well.  Sums over tokens that last, S = e S + P, are rounded float32 FMAs
 // and not tensor-core accumulations, whose truncation would lean one way for thousands of chunks.
+//
+// This form takes short sequences and the widths that fill no CTA of gdn_prefill_tc.cu (see takes_tc).  128 sequences of 48 tokens, 6 heads of
+// 128 x 128, bf16: 89 us, for 38 MB of rows and 100 MB of states (21 us).  The walk's chain binds, dependent products and exchanges among
+// lanes: some 2,400 cycles for a chunk of 16 tokens (1.3 us; the 1,024 of one sequence 1.34 ms).
 #include "gdn_pieces.cuh"
 #include "gdn_seq.cuh"
 

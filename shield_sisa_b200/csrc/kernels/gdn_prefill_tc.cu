@@ -3,9 +3,10 @@
 //
 //     U = T (V - diag(e) K S0),  O = M U + diag(e) Q S0,  S = e_64 S0 + K^T diag(exp(c_64 - c_j)) U
 //
-// prep   a CTA per chunk and head: T and M, what needs no state.  Gram products of 16 x 16 blocks on mma.sync, the 64 x 64 triangular
-//        inverse by block columns in float32, one a warp.  Both leave as fp16 pieces in the layout that the tensor core reads, the
-//        blocks above the diagonal left out: 16,912 bytes a chunk (22,032 with the second piece of M).
+// prep   a CTA per chunk and head: T and M, what needs no state.  Gram products of 16 x 16 blocks on mma.sync; of the triangular inverse the
+//        blocks on the diagonal by substitution in float32, those below it as products of blocks on the tensor cores, each factor in two
+//        TF32 pieces.  Both leave as fp16 pieces in the layout that the tensor core reads, the blocks above the diagonal left out: 16,912
+//        bytes a chunk (22,032 with the second piece of M).
 // walk   a CTA per head and 128 value columns.  The values are the 128 lanes of tensor memory: S^T, W^T, U^T and D^T are operands that
 //        lie there as pieces, K, Q, T and M come from shared memory.  The state itself stays in registers: a value column's keys in two
 //        threads (eight warps), rounded by float32 FMAs; per chunk its pieces go to tensor memory and the product K^T D comes back.
@@ -14,6 +15,16 @@
 //
 // A chunk is a chain: pieces of S -> K S0 -> W -> T W -> D -> K^T D -> S.  Q S0 and M U run beside it, and the outputs of a chunk are
 // written while the next one's first product runs.
+//
+// What bounds it.  64 sequences of 2,048 tokens, 6 heads of 128 x 128, bf16: prep 238 us and walk 386, for 862 MB that have to move (131 us
+// at the rate of a plain copy) and 0.16 TFLOP of the walk's products (97 us at cuBLAS's bf16 rate).  The walk is bound by its chain: a
+// chunk takes some 7,200 cycles of an SM (8,000 with all of them at work), of which the three products that it waits for are about 1,700;
+// cutting into pieces, the ways through tensor memory and shared memory and the meetings of threads are the rest.  A head's state and its
+// operands take all registers of an SM, so no second chain fills the gaps (384 chains on 148 SMs: three waves).  An instruction that is not in the cache costs most beside that,
+// which is why the loops below are rolled where they can be.  prep is a row of short phases between barriers, four CTAs of four warps on
+// an SM (issue slots 46 % used, DRAM 20 %): loads 63 us, Gram products 39, scalars and masks 46, the diagonal's inverses 17, the products of
+// blocks 40, T's pieces 22, the copy out 11.
+// One sequence of 16,384 tokens, 6 heads: prep 36 us, the two walks of its segments 173, the join 26.
 #include "gdn_pieces.cuh"
 #include "gdn_seq.cuh"
 #include "tc_ptx.cuh"
@@ -928,8 +939,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             const uint32_t lead = elect_one();
             int s = 0;
             uint32_t sph = 0;
-    #pragma unroll 1
-        for (int c = 0; c < NB; ++c) {
+#pragma unroll 1
+            for (int c = 0; c < NB; ++c) {
                 const uint32_t kq = smem_u32(sm.st[s].kq), vt = smem_u32(sm.st[s].v), wt = smem_u32(sm.st[s].w);
                 const int y = start + c * CT;
                 wait(empty(s), sph ^ 1u);
@@ -963,8 +974,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
             };
             int s = 0;
             uint32_t sph = 0;
-    #pragma unroll 1
-        for (int c = 0; c < NB; ++c) {
+#pragma unroll 1
+            for (int c = 0; c < NB; ++c) {
                 typename Sm::Stage& st = sm.st[s];
                 const int left = len - c * CT;
                 wait(wfull(s), sph);
@@ -1009,7 +1020,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
 
 // X of segment g becomes Phi_g X_(g-1) + X_g, g = 1 .. the last but one, in float32: a CTA takes JC columns of a head through all segments
 // of a sequence, the state so far in shared memory.  A thread has one key of the result and a share of the sum's keys; its part of the
-// next Phi does not depend on the state and is on its way while this one is used.
+// next Phi does not depend on the state and is on its way while this one is used.  (A segment is a chain of a product, two barriers and a
+// sum, about 1,000 cycles; with a whole sum in each thread it took three times that.)
 constexpr int JC = 8, JOIN_THREADS = 512;
 template <int DK> __global__ void __launch_bounds__(JOIN_THREADS) gdn_prefill_tc_join_kernel(const shvk_gdn_seq_args a, const WalkSegments seg) {
     constexpr int SHARES = JOIN_THREADS / DK, KPT = DK / SHARES, EPT = DK * JC / JOIN_THREADS;      // EPT: values of the result a thread adds up
@@ -1141,4 +1153,15 @@ int gdn_prefill_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s, int 
 extern "C" int shvk_gdn_prefill_status(int* status_out) {
     if (!status_out) return int(cudaErrorInvalidValue);
     return int(cudaMemcpyFromSymbol(status_out, sb::g_prefill_status, sizeof(int)));
+}
+
+extern "C" int shvk_gdn_prefill_status_fetch_async(int* host_word, void* stream) {
+    if (!host_word) return int(cudaErrorInvalidValue);
+    return int(cudaMemcpyFromSymbolAsync(host_word, sb::g_prefill_status, sizeof(int), 0, cudaMemcpyDeviceToHost, cudaStream_t(stream)));
+}
+
+extern "C" int shvk_gdn_prefill_status_clear_async(void* stream) {
+    void* word = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&word, sb::g_prefill_status);
+    return int(e != cudaSuccess ? e : cudaMemsetAsync(word, 0, sizeof(int), cudaStream_t(stream)));
 }

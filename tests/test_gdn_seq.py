@@ -679,6 +679,41 @@ print("ended with status", status.value)
     assert "ended with status" in r.stdout
 
 
+def test_status_fetch_refuses_no_place(L):
+    assert L.shvk_gdn_prefill_status_fetch_async(None, None) == INVALID
+
+
+@gpu
+def test_status_word_is_read_and_cleared_behind_the_work(L):
+    """The word of a call whose waits ran out, fetched and cleared on the call's stream; the next call leaves it clear."""
+    import subprocess
+    import sys
+    code = """
+import ctypes as C, torch
+from tests import test_gdn_seq as T
+from shield_sisa_b200 import binding
+L = binding.load_library(True)
+x = T.make("fp16", [200, 130], 2, 4, 64, 128, seed=3)
+T.launch(L, "prefill", x)
+word = torch.full((3,), -1, dtype=torch.int32).pin_memory()
+stream = torch.cuda.Stream()
+torch.cuda.synchronize()
+a = T.args(x)
+assert L.shvk_gdn_prefill_starved(C.byref(a), x["ws"].data_ptr(), x["ws"].numel(), 256, stream.cuda_stream) == 0
+assert L.shvk_gdn_prefill_status_fetch_async(word.data_ptr(), stream.cuda_stream) == 0
+assert L.shvk_gdn_prefill_status_clear_async(stream.cuda_stream) == 0
+assert L.shvk_gdn_prefill_status_fetch_async(word.data_ptr() + 4, stream.cuda_stream) == 0
+stream.synchronize()
+T.check(L, "prefill", T.make("fp16", [200, 130], 2, 4, 64, 128, seed=4))
+assert L.shvk_gdn_prefill_status_fetch_async(word.data_ptr() + 8, stream.cuda_stream) == 0
+stream.synchronize()
+print("words", word[0].item() > 0, word[1].item(), word[2].item())
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=str(__import__("tests.helpers", fromlist=["ROOT"]).ROOT))
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert "words True 0 0" in r.stdout
+
+
 @gpu
 def test_slots_past_two_gigabytes(L):
     """A pool whose last slots lie beyond 2^31 values."""
