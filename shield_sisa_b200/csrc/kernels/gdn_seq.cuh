@@ -45,7 +45,7 @@ inline int check_gdn_seq(const shvk_gdn_seq_args* a) {
     return 0;
 }
 
-// gdn_prefill_tc.cu: the chunked form for DV a multiple of 64 (arguments checked, workspace large enough)
+// gdn_prefill_tc.cu: the chunked form for DV a multiple of 64 (arguments checked, tokens there, workspace large enough)
 size_t gdn_prefill_tc_workspace(const shvk_gdn_seq_args& a);
 int gdn_prefill_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s, int starve_polls = 0);
 
