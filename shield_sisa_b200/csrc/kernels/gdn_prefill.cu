@@ -16,7 +16,7 @@
 // and not tensor-core accumulations, whose truncation would lean one way for thousands of chunks.
 //
 // This form takes short sequences and the widths that fill no CTA of gdn_prefill_tc.cu (see takes_tc).  128 sequences of 48 tokens, 6 heads of
-// 128 x 128, bf16: 89 us, for 38 MB of rows and 100 MB of states (21 us).  The walk's chain binds, dependent products and exchanges among
+// 128 x 128, bf16: 83 us in a graph, for 38 MB of rows and 100 MB of states (21 us).  The walk's chain binds, dependent products and exchanges among
 // lanes: some 2,400 cycles for a chunk of 16 tokens (1.3 us; the 1,024 of one sequence 1.34 ms).
 #include "gdn_pieces.cuh"
 #include "gdn_seq.cuh"
@@ -81,6 +81,7 @@ template <typename T, int DK>
 __global__ void __launch_bounds__(128, 4) gdn_prefill_prep_kernel(const shvk_gdn_seq_args a, uint8_t* __restrict__ ws, long long items) {
     constexpr int ROWB = DK * 2, VPR = DK / 8, KSTEP = DK / 16, VEC = PB * VPR / 32, LP = PB + 4;
     extern __shared__ __align__(16) uint8_t prep_raw[];
+    next_may_start();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     PrepWarp<DK>& sm = reinterpret_cast<PrepWarp<DK>*>(prep_raw)[warp];
     const long long item0 = ((long long)blockIdx.x * 4 + warp) * 2;
@@ -277,7 +278,10 @@ __global__ void __launch_bounds__(NW * 32, MINCTA) gdn_prefill_scan_kernel(const
     const SeqRows rows(a.seq_start, n, int(a.n_tokens));
     const int len = rows.end - rows.start, NB = (len + PB - 1) / PB;
     const long long in = slot_of(a.slot_in, n, a.n_slots), out = slot_of(a.slot_out, n, a.n_slots);
-    if (len == 0 && (out < 0 || out == in)) return;
+    if (len == 0 && (out < 0 || out == in)) {
+        last_is_done();
+        return;
+    }
     const int col0 = split * VC + warp * 16;                     // the warp's first value column
     const T* Q = static_cast<const T*>(a.q) + rows.start * a.ldq + khead * DK;
     const T* K = static_cast<const T*>(a.k) + rows.start * a.ldk + khead * DK;
@@ -338,8 +342,6 @@ __global__ void __launch_bounds__(NW * 32, MINCTA) gdn_prefill_scan_kernel(const
     // S^T in units of 1 / sig: S[nj][0, 1] value column col0 + g, keys 8 nj + 2 t, + 1;  S[nj][2, 3] column + 8.  top: a bound of the
     // largest |S| of the row in these units, kept between 2^9 and 2^15 so that the pieces lose nothing at either end of fp16.
     float S[NJ][4], sig[2], inv[2], top[2];
-#pragma unroll
-    for (int c = 0; c < NSLOT - 1; ++c) issue(c);
     {
         const float* src = a.states + ((in < 0 ? 0 : in) * a.HV + head) * (long long)(DK * a.DV) + col0 + g;
 #pragma unroll
@@ -347,6 +349,9 @@ __global__ void __launch_bounds__(NW * 32, MINCTA) gdn_prefill_scan_kernel(const
 #pragma unroll
             for (int e = 0; e < 4; ++e) S[nj][e] = in < 0 ? 0.0f : src[(8 * nj + 2 * t + (e & 1)) * (long long)a.DV + 8 * (e >> 1)];
     }
+    last_is_done();
+#pragma unroll
+    for (int c = 0; c < NSLOT - 1; ++c) issue(c);
     if (NB == 0) {                                               // nothing to walk: the state as it is
         cp_wait<0>();
         float* dst = a.states + (out * a.HV + head) * (long long)(DK * a.DV) + col0 + g;
@@ -594,7 +599,8 @@ template <typename T, int DK, int NW, int NSLOT, int MINCTA> int launch_scan(con
     if (ctas > 0x7fffffff) return int(cudaErrorInvalidValue);
     const cudaError_t e = cudaFuncSetAttribute(gdn_prefill_scan_kernel<T, DK, NW, NSLOT, MINCTA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return int(e);
-    gdn_prefill_scan_kernel<T, DK, NW, NSLOT, MINCTA><<<unsigned(ctas), NW * 32, smem, s>>>(a, ws);
+    if (a.n_tokens > 0) return int(launch_behind(gdn_prefill_scan_kernel<T, DK, NW, NSLOT, MINCTA>, ctas, NW * 32, smem, s, a, ws));
+    gdn_prefill_scan_kernel<T, DK, NW, NSLOT, MINCTA><<<unsigned(ctas), NW * 32, smem, s>>>(a, ws);      // (behind no preparation)
     return int(cudaGetLastError());
 }
 

@@ -53,13 +53,6 @@ template <bool FINE> struct Ws {
 
 __device__ int g_prefill_status = 0;                             // 1 + role whose wait gave up
 
-// The kernels of a call are launched behind one another with programmatic ordering: one may start when every CTA of the one before has
-// started or left, and waits for its end, with its memory, where that is first needed.  Every thread waits before it returns, so that the
-// end of the last kernel is the end of them all.  (Calls in a graph: 1 x 321 tokens 32.4 us, 34.5 one after the
-// other; 37 of up to 1,021 133.8 and 136.2.)
-__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void last_is_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // 128-byte rows, 16-byte pieces swizzled by the row: what SWIZZLE_128B reads
 __device__ __forceinline__ uint32_t sw128(int row, int piece) { return uint32_t(row * 128 + ((piece ^ (row & 7)) << 4)); }
 
@@ -1106,21 +1099,6 @@ inline long long segment_count(const shvk_gdn_seq_args& a, int chunks) { return 
 inline size_t chunk_bytes(const shvk_gdn_seq_args& a) {
     const size_t each = a.dtype == DT_F16 ? Ws<true>::BYTES : Ws<false>::BYTES;
     return (size_t(a.n_tokens / CT + a.n_seq + 1) * size_t(a.HV) * each + 15) / 16 * 16;
-}
-
-template <typename... P, typename... A>
-cudaError_t launch_behind(void (*kernel)(P...), long long ctas, int threads, int smem, cudaStream_t s, A... args) {
-    cudaLaunchAttribute order{};
-    order.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    order.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t c{};
-    c.gridDim = dim3(unsigned(ctas));
-    c.blockDim = dim3(unsigned(threads));
-    c.dynamicSmemBytes = size_t(smem);
-    c.stream = s;
-    c.attrs = &order;
-    c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, kernel, P(args)...);
 }
 
 template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s, uint32_t polls, bool starve) {

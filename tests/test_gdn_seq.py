@@ -609,6 +609,54 @@ def test_captured_replayed_and_on_two_streams(L, form):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_calls_behind_one_another_share_states_and_workspace(L, kind, dk):
+    """Calls of all forms in turn, each from the states that the one before left and in one workspace: the same bits queued at once,
+    captured and replayed, or with a pause behind each."""
+    import torch
+    hv, dv, n = 4, 128, 3
+    shapes = [[1000, 130, 700], [3, 17, 0], [65, 64, 130], [1, 1, 1], [9000, 20, 3000], [40, 30, 33], [300, 2, 1]]
+    calls = [make(kind, lens, 2, hv, dk, dv, seed=90 + i) for i, lens in enumerate(shapes)]
+    room = max(L.shvk_gdn_prefill_workspace_bytes(C.byref(args(x))) for x in calls)
+    ws = torch.empty(room, dtype=torch.uint8, device="cuda")
+    states = calls[0]["states"][:n].clone()
+    slots = torch.arange(n, device="cuda", dtype=torch.int32)
+    for x in calls:
+        x["states"], x["n_slots"], x["slot_in"], x["slot_out"] = states, n, slots, slots
+    first = states.clone()
+
+    def run(pause, stream):
+        for i, x in enumerate(calls):
+            a = args(x)
+            rc = L.shvk_gdn_step(C.byref(a), stream) if i in (3, 6) else L.shvk_gdn_prefill(C.byref(a), ws.data_ptr(), room, stream)
+            assert rc == 0
+            if pause:
+                torch.cuda.synchronize()
+
+    def result():
+        torch.cuda.synchronize()
+        got = [states.clone()] + [x["o"].clone() for x in calls]
+        states.copy_(first)
+        for x in calls:
+            x["o"].fill_(7.0)
+        torch.cuda.synchronize()
+        return got
+    run(True, torch.cuda.current_stream().cuda_stream)
+    want = result()
+    for _ in range(5):
+        run(False, torch.cuda.current_stream().cuda_stream)
+        assert all(torch.equal(g, w) for g, w in zip(result(), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(False, torch.cuda.current_stream().cuda_stream)
+    result()
+    for _ in range(3):
+        graph.replay()
+        assert all(torch.equal(g, w) for g, w in zip(result(), want))
+
+
+@gpu
 @pytest.mark.parametrize("layer_type", ["bf16", "fp16"])
 def test_a_layer_in_service(L, layer_type):
     """The operators as a layer runs them: a prompt by the chunked form, the gated norm over each head's values, then the residual sum and
