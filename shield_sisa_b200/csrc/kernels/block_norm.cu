@@ -299,7 +299,7 @@ int launch_rows(const shvk_block_norm_args& a, int P, int threads, cudaStream_t 
     const int groups = ROWT ? threads / ROWT : 1, span = (ROWT ? ROWT : threads) * NV * 8;
     const int smem = 3 * span * int(sizeof(float));
     static_assert(3 * 4 * 512 * 8 * sizeof(float) <= 200 * 1024, "the longest row's weights fit");
-    if (smem > 48 * 1024) {
+    if (smem > 47 * 1024) {                                      // (beside the sums of a CTA, which are static)
         const cudaError_t e = cudaFuncSetAttribute(block_norm_kernel<T, TH, NV, ROWT, EDGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return int(e);
     }

@@ -147,6 +147,15 @@ WIDTHS = [1, 7, 8, 33, 120, 128, 129, 255, 256, 384, 505, 512, 513, 960, 1920, 2
 
 
 @gpu
+@pytest.mark.parametrize("kind,res", [("bf16", "fp32"), ("fp32", "fp32"), ("fp16", "fp16")])
+@pytest.mark.parametrize("d", [1536, 1537, 2040, 2048, 3585, 3841, 4088, 4089, 4095, 4096, 4097, 8177, 8191, 8193])
+def test_widths_where_the_shared_memory_changes(L, kind, res, d):
+    """Weights and rows of a CTA around the sizes at which a launch has to ask for more than 48 KB, with and without all of them."""
+    check(L, make(kind, 9, 1, d, res=res, seed=d + 1))
+    check(L, make(kind, 9, 1, d, res=res, seed=d + 2, gate="one"))
+
+
+@gpu
 @pytest.mark.parametrize("kind,res", [("bf16", "fp32"), ("fp16", "fp16"), ("fp32", "fp32"), ("bf16", "bf16"), ("fp16", "fp32")])
 @pytest.mark.parametrize("d", WIDTHS)
 def test_every_width(L, kind, res, d):
