@@ -1026,8 +1026,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
 
 // X of segment g becomes Phi_g X_(g-1) + X_g, g = 1 .. the last but one, in float32: a CTA takes JC columns of a head through all segments
 // of a sequence, the state so far in shared memory.  A thread has one key of the result and a share of the sum's keys; its part of the
-// next Phi does not depend on the state and is on its way while this one is used.  (A segment is a chain of a product, two barriers and a
-// sum, about 1,000 cycles; with a whole sum in each thread it took three times that.)
+// next Phi does not depend on the state and is on its way while this one is used.  (A segment's Phi, 64 KB out of L2, its products, two
+// barriers and a sum are a chain of about 2.3 us; with a whole sum in each thread it took three times that.)
 constexpr int JC = 8, JOIN_THREADS = 512;
 template <int DK> __global__ void __launch_bounds__(JOIN_THREADS) gdn_prefill_tc_join_kernel(const shvk_gdn_seq_args a, const WalkSegments seg) {
     constexpr int SHARES = JOIN_THREADS / DK, KPT = DK / SHARES, EPT = DK * JC / JOIN_THREADS;      // EPT: values of the result a thread adds up
@@ -1080,8 +1080,8 @@ template <int DK> __global__ void __launch_bounds__(JOIN_THREADS) gdn_prefill_tc
     }
 }
 
-// Chunks of a segment, 0 where sequences are walked whole.  Counted in chunks' times of one wave of CTAs (a walk's chunk takes 7,200 cycles,
-// a join's segment about 1,000, the two launches more about as much as two chunks) for sequences of the average length; segments are not
+// Chunks of a segment, 0 where sequences are walked whole.  Counted in chunks' times of one wave of CTAs (a walk's chunk takes 3.8 us, a
+// join's segment 2.3, the two launches more about as much as two chunks) for sequences of the average length; segments are not
 // shorter than 13 chunks, so that their states take less room than their chunks' T and M.
 inline int segment_chunks(const shvk_gdn_seq_args& a) {
     const long long sms = device_sms(), splits = (a.DV + TV - 1) / TV, heads = (long long)a.n_seq * a.HV, chunks = a.n_tokens / CT / a.n_seq;
@@ -1090,7 +1090,7 @@ inline int segment_chunks(const shvk_gdn_seq_args& a) {
     int found = 0;
     for (long long g = 2; g <= 64 && (chunks + g - 1) / g >= 13; ++g) {
         const long long len = (chunks + g - 1) / g;
-        const double t = double(len * (waves(heads * (splits + (g - 2) * (splits + 1))) + waves(heads * splits * (g - 1)))) + 0.15 * double(g - 2) + 2.0;
+        const double t = double(len * (waves(heads * (splits + (g - 2) * (splits + 1))) + waves(heads * splits * (g - 1)))) + 0.6 * double(g - 2) + 2.0;
         if (t < best) { best = t; found = int(len); }
     }
     return found;
