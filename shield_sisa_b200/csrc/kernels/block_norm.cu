@@ -10,6 +10,7 @@
 // cut at the same places, so that its copy of the weights in shared memory, shifted as its rows are, serves them all with 16-byte
 // reads.  A group that reaches over a row's end is read and written value by value.
 #include "device_utils.cuh"
+#include "launch_order.cuh"
 #include "shv_seq_kernels.h"
 
 #include <type_traits>
@@ -156,6 +157,8 @@ block_norm_kernel(const shvk_block_norm_args a, int P) {
     };
     constexpr bool AHEAD = NV < 4;
     Row now;
+    next_may_start();
+    last_is_done();
     fetch(R < total, row, head, now);
     if (ROWT == 0 && tid < 64) (&red[0][0][0])[tid] = 0.0f;
     for (int e = tid; e < span; e += blockDim.x) {               // the weights, behind the first row's loads
@@ -257,6 +260,8 @@ __global__ void __launch_bounds__(256) block_norm_any_kernel(const shvk_block_no
     extern __shared__ float bn_h[];
     __shared__ float red[2][8];
     const int tid = threadIdx.x;
+    next_may_start();
+    last_is_done();
     const long long row = blockIdx.x / a.heads, base = blockIdx.x % a.heads * (long long)a.D;
     const T* x = static_cast<const T*>(a.x) + row * a.ldx + base;
     const T* gate = a.gate ? static_cast<const T*>(a.gate) + row * a.ldgate + base : nullptr;
@@ -307,8 +312,7 @@ int launch_rows(const shvk_block_norm_args& a, int P, int threads, cudaStream_t 
     const int resident = ROWT ? 4 : NV == 1 ? 1024 / threads : threads > 256 ? 1 : 512 / threads;      // CTAs of an SM, by registers
     const long long most = (long long)device_sms() * resident / P * P;
     const long long ctas = need < most ? need : (most > 0 ? most : P);
-    block_norm_kernel<T, TH, NV, ROWT, EDGE><<<unsigned(ctas), threads, smem, s>>>(a, P);
-    return int(cudaGetLastError());
+    return int(launch_behind(block_norm_kernel<T, TH, NV, ROWT, EDGE>, ctas, threads, smem, s, a, P));
 }
 
 template <typename T, typename TH, bool EDGE> int launch_vec(const shvk_block_norm_args& a, int P, int nvec, cudaStream_t s) {
@@ -336,8 +340,7 @@ template <typename T, typename TH> int launch_block_norm(const shvk_block_norm_a
         const int smem = a.D * int(sizeof(float));
         const cudaError_t e = cudaFuncSetAttribute(block_norm_any_kernel<T, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return int(e);
-        block_norm_any_kernel<T, TH><<<unsigned(a.rows * a.heads), 256, smem, s>>>(a);
-        return int(cudaGetLastError());
+        return int(launch_behind(block_norm_any_kernel<T, TH>, a.rows * a.heads, 256, smem, s, a));
     }
     return P == 1 && a.D % 8 == 0 ? launch_vec<T, TH, false>(a, P, nvec, s) : launch_vec<T, TH, true>(a, P, nvec, s);
 }

@@ -81,7 +81,8 @@ template <typename T, int DK>
 __global__ void __launch_bounds__(128, 4) gdn_prefill_prep_kernel(const shvk_gdn_seq_args a, uint8_t* __restrict__ ws, long long items) {
     constexpr int ROWB = DK * 2, VPR = DK / 8, KSTEP = DK / 16, VEC = PB * VPR / 32, LP = PB + 4;
     extern __shared__ __align__(16) uint8_t prep_raw[];
-    next_may_start();
+    last_is_done();
+    next_may_start();                                            // (behind the wait: the walk reads where sequences lie before its own)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     PrepWarp<DK>& sm = reinterpret_cast<PrepWarp<DK>*>(prep_raw)[warp];
     const long long item0 = ((long long)blockIdx.x * 4 + warp) * 2;
@@ -626,8 +627,7 @@ template <typename T, int DK> int launch_prefill(const shvk_gdn_seq_args& a, uin
         constexpr int smem = 4 * int(sizeof(PrepWarp<DK>));
         const cudaError_t e = cudaFuncSetAttribute(gdn_prefill_prep_kernel<T, DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return int(e);
-        gdn_prefill_prep_kernel<T, DK><<<unsigned(ctas), 128, smem, s>>>(a, ws, items);
-        if (const cudaError_t le = cudaGetLastError(); le != cudaSuccess) return int(le);
+        if (const cudaError_t le = launch_behind(gdn_prefill_prep_kernel<T, DK>, ctas, 128, smem, s, a, ws, items); le != cudaSuccess) return int(le);
     }
     const long long heads = (long long)a.n_seq * a.HV;
     if (a.DV % 128 == 0 && heads > device_sms()) return launch_scan<T, DK, 8, 4, 1>(a, ws, s);

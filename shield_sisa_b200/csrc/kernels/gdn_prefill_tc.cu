@@ -129,7 +129,8 @@ __global__ void __launch_bounds__(128, FINE_PREP<T> ? 3 : 4) gdn_prefill_tc_prep
     extern __shared__ uint8_t prep_raw[];
     Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(prep_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    next_may_start();
+    last_is_done();
+    next_may_start();                                            // (behind the wait: the walk reads where sequences lie before its own)
     const int chunk = int(blockIdx.x / unsigned(a.HV)), head = int(blockIdx.x % unsigned(a.HV)), khead = head / (a.HV / a.HK);
     int n = 0;                                                   // the last sequence whose first chunk is not behind this one
     for (int lo = 0, hi = a.n_seq - 1; lo <= hi;) {
@@ -1119,8 +1120,15 @@ template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t*
         !tma::make_map_2d(&maps.k, a.k, 2, a.n_tokens, (long long)a.HK * DK, a.ldk, CT, 64, true) ||
         !tma::make_map_2d(&maps.v, a.v, 2, a.n_tokens, (long long)a.HV * a.DV, a.ldv, CT, TV, false))
         return int(cudaErrorInvalidValue);
-    gdn_prefill_tc_prep_kernel<T, DK><<<unsigned(items), 128, prep_smem, s>>>(a, ws);
-    if ((e = cudaGetLastError()) != cudaSuccess) return int(e);
+    // Ahead of the end of what ran before, but for calls in segments: calls in a row of 321 tokens 36.1 -> 34.0 us, of 64 x 2,048 tokens
+    // 615.6 -> 614.6, but in segments 1 x 16,384 233.7 -> 235.2.
+    if (!chunks) {
+        e = launch_behind(gdn_prefill_tc_prep_kernel<T, DK>, items, 128, prep_smem, s, a, ws);
+    } else {
+        gdn_prefill_tc_prep_kernel<T, DK><<<unsigned(items), 128, prep_smem, s>>>(a, ws);
+        e = cudaGetLastError();
+    }
+    if (e != cudaSuccess) return int(e);
     WalkSegments seg{};
     auto walk = [&](long long n) { return launch_behind(gdn_prefill_tc_walk_kernel<T, DK, STAGES>, n, TC_THREADS, smem, s, maps, a, ws, seg, polls, starve); };
     if (!chunks) return int(walk(ctas));

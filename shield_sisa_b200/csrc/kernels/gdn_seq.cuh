@@ -2,6 +2,7 @@
 // slots lie.
 #pragma once
 #include "device_utils.cuh"
+#include "launch_order.cuh"
 #include "shv_seq_kernels.h"
 
 namespace sb {
@@ -43,28 +44,6 @@ inline int check_gdn_seq(const shvk_gdn_seq_args* a) {
     }
     if (a->n_slots < 0 || ((a->slot_in || a->slot_out) && (!a->states || !aligned16(a->states)))) return bad;
     return 0;
-}
-
-// The kernels of a call are launched behind one another with programmatic ordering: one may start when every CTA of the one before has
-// started or left, and waits for its end, with its memory, where that is first needed.  Every thread waits before it returns, so that the
-// end of the last kernel is the end of them all.  (Calls in a graph: 1 x 321 tokens 32.4 us, 34.5 one after the other; 37 of up to 1,021
-// 133.8 and 136.2.)
-__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void last_is_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-template <typename... P, typename... A>
-inline cudaError_t launch_behind(void (*kernel)(P...), long long ctas, int threads, int smem, cudaStream_t s, A... args) {
-    cudaLaunchAttribute order{};
-    order.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    order.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t c{};
-    c.gridDim = dim3(unsigned(ctas));
-    c.blockDim = dim3(unsigned(threads));
-    c.dynamicSmemBytes = size_t(smem);
-    c.stream = s;
-    c.attrs = &order;
-    c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, kernel, P(args)...);
 }
 
 // gdn_prefill_tc.cu: the chunked form for DV a multiple of 64 (arguments checked, tokens there, workspace large enough)

@@ -40,6 +40,8 @@ gdn_step_kernel(const shvk_gdn_seq_args a) {
     const int splits = a.DV / VC, split = blockIdx.x % splits;
     const int nh = blockIdx.x / splits, n = nh / a.HV, head = nh % a.HV, khead = head / (a.HV / a.HK);
     const int col = split * VC + tid % LPR * 4, row0 = tid / LPR;
+    next_may_start();
+    last_is_done();
     const SeqRows rows(a.seq_start, n, int(a.n_tokens));
     const long long in = slot_of(a.slot_in, n, a.n_slots), out = slot_of(a.slot_out, n, a.n_slots);
     if (rows.start == rows.end && (out < 0 || out == in)) return;
@@ -144,8 +146,7 @@ gdn_step_kernel(const shvk_gdn_seq_args a) {
 template <typename T, int DK, int VC> int launch_step(const shvk_gdn_seq_args& a, cudaStream_t s) {
     const long long ctas = (long long)a.n_seq * a.HV * (a.DV / VC);
     if (ctas > 0x7fffffff) return int(cudaErrorInvalidValue);
-    gdn_step_kernel<T, DK, VC><<<unsigned(ctas), step_threads<DK, VC>(), 0, s>>>(a);
-    return int(cudaGetLastError());
+    return int(launch_behind(gdn_step_kernel<T, DK, VC>, ctas, step_threads<DK, VC>(), 0, s, a));
 }
 
 template <typename T> int dispatch_step(const shvk_gdn_seq_args& a, cudaStream_t s) {

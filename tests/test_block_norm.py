@@ -279,3 +279,29 @@ def test_captured_and_replayed(L):
     launch(L, y)
     torch.cuda.synchronize()
     assert torch.equal(x["h_out"], y["h_out"]) and torch.equal(x["xn"], y["xn"])
+
+
+@gpu
+@pytest.mark.parametrize("d", [128, 384, 2047, 2048, 16377])
+def test_norms_behind_one_another(L, d):
+    """Each call reads what the one before wrote, in place and with nothing between them: the same bits as with a pause behind each."""
+    import torch
+    x = make("bf16", 700, 1, d, res="fp32", gate="none", seed=3 + d)
+    y = dict(x)
+    y["x"], y["xn"] = x["xn"], x["x"]                            # the other way round, h in place
+    x["h_out"] = y["h_out"] = y["h_in"] = x["h_in"]
+    first = [x[name].clone() for name in ("x", "xn", "h_in")]
+
+    def run(pause):
+        for name, v in zip(("x", "xn", "h_in"), first):
+            x[name].copy_(v)
+        for i in range(12):
+            launch(L, (x, y)[i % 2])
+            if pause:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return [x[name].clone() for name in ("x", "xn", "h_in")]
+    want = run(True)
+    assert all(torch.isfinite(w.float()).all() for w in want)
+    for _ in range(5):
+        assert all(torch.equal(g, w) for g, w in zip(run(False), want))

@@ -657,6 +657,76 @@ def test_calls_behind_one_another_share_states_and_workspace(L, kind, dk):
 
 
 @gpu
+@pytest.mark.parametrize("form", ["step", "prefill", "long"])
+@pytest.mark.parametrize("before", ["copy", "fill", "join", "nothing"])
+def test_what_a_call_may_stand_behind(L, form, before):
+    """Behind a copy, a fill, two streams that meet, or first of all; queued and in a graph: its inputs are the ones written there."""
+    import torch
+    lens = [9000, 700] if form == "long" else [70, 0, 130]
+    x = make("bf16", lens, 2, 4, 128, 128, seed=17)
+    form = "prefill" if form == "long" else form
+    launch(L, form, x)
+    torch.cuda.synchronize()
+    states = x["states"].clone()
+    names = ("v", "seq_start", "states") if before != "fill" else ("states",)
+    good = {name: x[name].clone() for name in names}
+    good["states"] = torch.zeros_like(states) if before == "fill" else make("bf16", lens, 2, 4, 128, 128, seed=17)["states"]
+    side, fork, joined = torch.cuda.Stream(), torch.cuda.Event(), torch.cuda.Event()
+
+    def run():
+        main = torch.cuda.current_stream()
+        if before == "join":
+            fork.record(main)
+            side.wait_event(fork)
+            with torch.cuda.stream(side):
+                x["v"].copy_(good["v"])
+                x["states"].copy_(good["states"])
+                joined.record(side)
+            x["seq_start"].copy_(good["seq_start"])
+            main.wait_event(joined)
+        elif before == "fill":
+            x["states"].zero_()
+        elif before == "copy":
+            for name in names:
+                x[name].copy_(good[name])
+        launch(L, form, x, stream=main)
+
+    def spoil():
+        x["o"].fill_(7.0)
+        if before in ("copy", "join"):
+            x["v"].fill_(1.0)
+            x["seq_start"].zero_()
+        if before != "nothing":
+            x["states"].fill_(3.0)
+        else:
+            x["states"].copy_(good["states"])
+        torch.cuda.synchronize()
+    spoil()
+    if before in ("copy", "join"):                              # the answer: everything in its place, with a pause in front
+        for name in names:
+            x[name].copy_(good[name])
+    elif before == "fill":
+        x["states"].zero_()
+    torch.cuda.synchronize()
+    launch(L, form, x)
+    torch.cuda.synchronize()
+    want = (x["o"].clone(), x["states"].clone())
+    for _ in range(3):
+        spoil()
+        run()
+        torch.cuda.synchronize()
+        assert torch.equal(x["o"], want[0]) and torch.equal(x["states"], want[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(3):
+        spoil()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x["o"], want[0]) and torch.equal(x["states"], want[1])
+
+
+@gpu
 @pytest.mark.parametrize("layer_type", ["bf16", "fp16"])
 def test_a_layer_in_service(L, layer_type):
     """The operators as a layer runs them: a prompt by the chunked form, the gated norm over each head's values, then the residual sum and
