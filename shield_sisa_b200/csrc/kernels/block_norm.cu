@@ -8,7 +8,11 @@
 // Rows whose pitch is no multiple of eight start anywhere in such a group.  All arrays of a call then start at the same place of it (or
 // the call goes to block_norm_any_kernel), and the place repeats every eight rows at most: a CTA walks rows of one class, which are
 // cut at the same places, so that its copy of the weights in shared memory, shifted as its rows are, serves them all with 16-byte
-// reads.  A group that reaches over a row's end is read and written value by value.
+// reads.  A group that reaches over a row's end is read whole where that stays in the array, and written value by value.
+//
+// 16-bit rows, one B200: 123,264 heads of 128 with a SiLU gate 20.7 us (95 MB, 0.70 of a plain copy's rate), 20,544 x 384 residual and norm
+// 18.1 us (0.79), four times as many rows of either 5.3 and 6.1 TB/s (0.81, 0.93): ramp up and drain.  16,384 x 2,048 with everything
+// 65 us (4.1 TB/s; two barriers of a CTA a row), x 2,047 95: masks at a row's ends, and sectors that two SMs write.
 #include "device_utils.cuh"
 #include "launch_order.cuh"
 #include "shv_seq_kernels.h"

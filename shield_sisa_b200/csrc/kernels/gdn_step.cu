@@ -7,9 +7,9 @@
 //
 // A token of a sequence moves DK x DV floats in and out for 6 DK DV operations: HBM binds.  A CTA takes VC of a head's value columns, its
 // state in registers from the first token to the last: a thread has four columns (16-byte loads and stores) of every RSTEP-th key.
-// One token for each of 512 sequences, 6 heads of 128 x 128, bf16: 406 MB in 69 us, 5.9 TB/s, 0.90 of what a plain copy reaches.  (32 value
+// One token for each of 512 sequences, 6 heads of 128 x 128, bf16: 406 MB in 68 us, 6.0 TB/s, 0.91 of what a plain copy reaches.  (32 value
 // columns to a CTA, 128 threads: a CTA asks for 16 KB at once and seven of them are resident, enough bytes in flight; a sequence of several
-// tokens pays two barriers of four warps for each.)  128 sequences of float32 values, 6 heads of 64 x 128: 12.3 us, 0.64; below some 50 MB
+// tokens pays two barriers of four warps for each.)  128 sequences of float32 values, 6 heads of 64 x 128: 10.5 us, 0.75; below some 50 MB
 // the launch and the state's one round trip show.
 #include "gdn_seq.cuh"
 
