@@ -146,8 +146,8 @@ def prepare(case, seed):
     s.slot_out = n + torch.randperm(n, device="cuda", generator=gen).to(torch.int32)
     s.workspace = None
     if case["op"] == "prefill":                                  # memory that a program keeps, one piece for all its layers
-        chunks = s.tokens // 64 + n + 1
-        s.workspace = torch.empty(chunks * hv * 40960, dtype=torch.uint8, device="cuda")
+        blocks = s.tokens // 16 + n + 1
+        s.workspace = torch.empty(blocks * hv * 8192, dtype=torch.uint8, device="cuda")
     return s
 
 
