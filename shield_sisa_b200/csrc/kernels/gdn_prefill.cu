@@ -11,9 +11,10 @@
 // hi lo + lo hi, are summed in float32.  K and Q are 16-bit values already: one piece.  fp16 has the bits (bf16 pieces would have to be
 // three) but not the range, so everything is scaled by powers of two, which cost no bits: a token's k and q by their norms, T by its
 // largest entry, rows of M by theirs, and the rows of S^T, W^T, U^T (one value column each; what a chunk does to them is linear) by scales
-// that the walk keeps or finds anew.  On the output's way, where the caller rounds to 16 bits, one piece is enough for bf16 (its step is
-// 2^-8, a piece's 2^-11); for fp16 outputs there are two here as well.  Sums over tokens that last, S = e S + P, are rounded float32 FMAs
-// and not tensor-core accumulations, whose truncation would lean one way for thousands of chunks.
+// that the walk keeps or finds anew.  On the output's way S, M and U are two pieces as well (with one, of eleven bits, 11 % of bf16
+// outputs were not the rounded value of the rule, now 0.03 %, and less than a thousandth of each where terms cancel; it costs 4 % here, 5 %
+// in gdn_prefill_tc.cu).  Sums over tokens that last, S = e S + P, are rounded float32 FMAs and not tensor-core accumulations, whose
+// truncation would lean one way for thousands of chunks.
 //
 // This form takes short sequences and the widths that fill no CTA of gdn_prefill_tc.cu (see takes_tc).  128 sequences of 48 tokens, 6 heads of
 // 128 x 128, bf16: 83 us in a graph, for 38 MB of rows and 100 MB of states (21 us).  The walk's chain binds, dependent products and exchanges among
@@ -268,7 +269,6 @@ template <int DK, int VC, int NSLOT> struct ScanSmem {
 template <typename T, int DK, int NW, int NSLOT, int MINCTA>
 __global__ void __launch_bounds__(NW * 32, MINCTA) gdn_prefill_scan_kernel(const shvk_gdn_seq_args a, const uint8_t* __restrict__ ws) {
     constexpr int VC = 16 * NW, NT = NW * 32, KSTEP = DK / 16, NJ = DK / 8, ROWB = DK * 2, VROWB = VC * 2, VPR = DK / 8, VPV = VC / 8;
-    constexpr bool FINE = std::is_same<T, __half>::value;        // outputs with eleven bits: two pieces on their way as well
     constexpr int KN = PB * VPR, VN = PB * VPV, WN = PW_BYTES / 16;
     extern __shared__ __align__(128) uint8_t scan_raw[];
     ScanSmem<DK, VC, NSLOT>& sm = *reinterpret_cast<ScanSmem<DK, VC, NSLOT>*>(scan_raw);
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(NW * 32, MINCTA) gdn_prefill_scan_kernel(const
                 mma16<__half>(R[ni], sh, bk[2 * ni], bk[2 * ni + 1]);
                 mma16<__half>(RL[ni], sl, bk[2 * ni], bk[2 * ni + 1]);
                 mma16<__half>(QS[ni], sh, bq[2 * ni], bq[2 * ni + 1]);
-                if (FINE) mma16<__half>(QS[ni], sl, bq[2 * ni], bq[2 * ni + 1]);
+                mma16<__half>(QS[ni], sl, bq[2 * ni], bq[2 * ni + 1]);
             }
         }
         // ---------------------------------------------------------------- W = V - e K S0, scaled by row to at most 2^10; U = T W
@@ -516,20 +516,15 @@ __global__ void __launch_bounds__(NW * 32, MINCTA) gdn_prefill_scan_kernel(const
         {
             uint32_t uh[4], ul[4], bm[4], bml[4], ov[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (FINE) split_pair(U[i >> 1][2 * (i & 1)], U[i >> 1][2 * (i & 1) + 1], uh[i], ul[i]);
-                else uh[i] = pack_half(U[i >> 1][2 * (i & 1)], U[i >> 1][2 * (i & 1) + 1]);
-            }
+            for (int i = 0; i < 4; ++i) split_pair(U[i >> 1][2 * (i & 1)], U[i >> 1][2 * (i & 1) + 1], uh[i], ul[i]);
             ldsm4(smem_u32(st.w + PW_M) + toff, bm);
-            if (FINE) ldsm4(smem_u32(st.w + PW_ML) + toff, bml);
+            ldsm4(smem_u32(st.w + PW_ML) + toff, bml);
 #pragma unroll
             for (int ni = 0; ni < 2; ++ni) {
                 float acc[4] = {};
                 mma16<__half>(acc, uh, bm[2 * ni], bm[2 * ni + 1]);
-                if (FINE) {
-                    mma16<__half>(acc, ul, bm[2 * ni], bm[2 * ni + 1]);
-                    mma16<__half>(acc, uh, bml[2 * ni], bml[2 * ni + 1]);
-                }
+                mma16<__half>(acc, ul, bm[2 * ni], bm[2 * ni + 1]);
+                mma16<__half>(acc, uh, bml[2 * ni], bml[2 * ni + 1]);
                 const float2 om = wf(PW_OM, 8 * ni + 2 * t), eq = wf(PW_EQ, 8 * ni + 2 * t);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {

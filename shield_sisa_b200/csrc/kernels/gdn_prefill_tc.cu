@@ -6,7 +6,9 @@
 // prep   a CTA per chunk and head: T and M, what needs no state.  Gram products of 16 x 16 blocks on mma.sync; of the triangular inverse the
 //        blocks on the diagonal by substitution in float32, those below it as products of blocks on the tensor cores, each factor in two
 //        TF32 pieces.  Both leave as fp16 pieces in the layout that the tensor core reads, the blocks above the diagonal left out: 16,912
-//        bytes a chunk (22,032 with the second piece of M).
+//        bytes a chunk (22,032 with the second piece of M, for fp16).  For bf16 the second piece of M's rows waits in the
+//        rows of o that it makes, 128 bytes of each, until the chunk's outputs go there: four CTAs of prep fit an SM so (with it in
+//        the workspace three, as for fp16: 285 us instead of 255 for 64 x 2,048), and walk loads it by TMA.
 // walk   a CTA per head and 128 value columns.  The values are the 128 lanes of tensor memory: S^T, W^T, U^T and D^T are operands that
 //        lie there as pieces, K, Q, T and M come from shared memory.  The state itself stays in registers: a value column's keys in two
 //        threads (eight warps), rounded by float32 FMAs; per chunk its pieces go to tensor memory and the product K^T D comes back.
@@ -45,9 +47,9 @@ constexpr int TV = 128;                                          // value column
 // tri_at(i, j) = tri_step(j / 16) + (r / 8) 256 + (j / 8 % 2) 128 + (r % 8) 16 + (j % 8) 2, r = i - 16 (j / 16).
 constexpr int TRI_BYTES = 5120;
 __host__ __device__ constexpr int tri_step(int kk) { return 32 * (64 * kk - 8 * kk * (kk - 1)); }
-// workspace of a chunk and head: T hi | T lo | M hi | (M lo) | six arrays of 64 floats | e_64, T's scale, the largest ER, DK's scale
-template <bool FINE> struct Ws {
-    static constexpr int T = 0, TL = TRI_BYTES, M = 2 * TRI_BYTES, ML = 3 * TRI_BYTES, SC = (FINE ? 4 : 3) * TRI_BYTES;
+// workspace of a chunk and head: T hi | T lo | M hi | (M lo, fp16 calls) | six arrays of 64 floats | e_64, T's scale, the largest ER, DK's scale
+template <bool LO_WS> struct Ws {
+    static constexpr int T = 0, TL = TRI_BYTES, M = 2 * TRI_BYTES, ML = 3 * TRI_BYTES, SC = (LO_WS ? 4 : 3) * TRI_BYTES;
     static constexpr int ER = SC, EQ = SC + 256, DK = SC + 512, OM = SC + 768, KS = SC + 1024, QS = SC + 1280, E64 = SC + 1536;
     static constexpr int BYTES = SC + 1552;
 };
@@ -74,8 +76,8 @@ template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const
 __device__ __forceinline__ int first_chunk(const SeqRows& r, int n) { return r.start / CT + n; }
 
 // ---------------------------------------------------------------------------------------------------- what needs no state
-template <int DK, bool FINE> struct PrepSmem {
-    static constexpr int TILES = 2 * CT * DK * 2, IMAGES = Ws<FINE>::BYTES, LP = CT + 4;
+template <int DK, bool LO_WS> struct PrepSmem {
+    static constexpr int TILES = 2 * CT * DK * 2, IMAGES = Ws<LO_WS>::BYTES, LP = CT + 4;
     static constexpr int X_AT = (IMAGES + 15) / 16 * 16, BOTH = X_AT + CT * LP * 4;
     __align__(1024) uint8_t a[TILES > BOTH ? TILES : BOTH];      // K and Q as they are, then what leaves and, behind it, X = (I + L)^-1
     __align__(16) float l[CT * LP];
@@ -120,12 +122,12 @@ template <int P> __device__ __forceinline__ void block_store(float* D, const flo
             *reinterpret_cast<float2*>(D + (g + 8 * h) * P + 8 * ni + 2 * t) = make_float2(sign * d[ni][2 * h], sign * d[ni][2 * h + 1]);
 }
 
-template <typename T> constexpr bool FINE_PREP = std::is_same<T, __half>::value;
+template <typename T> constexpr bool M_LO_IN_WS = std::is_same<T, __half>::value;     // M's second piece: in the workspace, or in o's rows
 template <typename T, int DK>
-__global__ void __launch_bounds__(128, FINE_PREP<T> ? 3 : 4) gdn_prefill_tc_prep_kernel(const shvk_gdn_seq_args a, uint8_t* __restrict__ ws) {
-    constexpr bool FINE = std::is_same<T, __half>::value;
-    using W = Ws<FINE>;
-    using Sm = PrepSmem<DK, FINE>;
+__global__ void __launch_bounds__(128, M_LO_IN_WS<T> ? 3 : 4) gdn_prefill_tc_prep_kernel(const shvk_gdn_seq_args a, uint8_t* __restrict__ ws) {
+    constexpr bool LO_WS = M_LO_IN_WS<T>;
+    using W = Ws<LO_WS>;
+    using Sm = PrepSmem<DK, LO_WS>;
     constexpr int LP = Sm::LP;
     extern __shared__ uint8_t prep_raw[];
     Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(prep_raw) + 1023) & ~uintptr_t(1023));
@@ -296,13 +298,9 @@ __global__ void __launch_bounds__(128, FINE_PREP<T> ? 3 : 4) gdn_prefill_tc_prep
                 *reinterpret_cast<float2*>(sm.l + i * LP + j0) = make_float2(l[0], l[1]);
                 uint32_t mh, ml;
                 const int at = tri_step(bj) + (2 * (bi - bj) + h) * 256 + ni * 128 + g * 16 + 4 * t;      // tri_at(i, j0)
-                if (FINE) {
-                    split_pair(m[0], m[1], mh, ml);
-                    *reinterpret_cast<uint32_t*>(out + W::M + at) = mh;
-                    *reinterpret_cast<uint32_t*>(out + W::ML + at) = ml;
-                } else {
-                    *reinterpret_cast<uint32_t*>(out + W::M + at) = pack_half(m[0], m[1]);
-                }
+                split_pair(m[0], m[1], mh, ml);
+                *reinterpret_cast<uint32_t*>(out + W::M + at) = mh;
+                *reinterpret_cast<uint32_t*>(out + (LO_WS ? W::ML + at : W::T + sw128(i, j0 >> 3) + 2 * (j0 & 7))) = ml;
             }
         }
     }
@@ -327,6 +325,15 @@ __global__ void __launch_bounds__(128, FINE_PREP<T> ? 3 : 4) gdn_prefill_tc_prep
         }
     }
     __syncthreads();
+    if (!LO_WS)                                                  // M lo to o's rows, a copy in the columns of each CTA of the walk
+        for (int v = tid; v < CT * 8; v += 128) {
+            const int row = v >> 3, p = v & 7;
+            if (row < left && p < 2 * (row >> 4) + 2) {
+                const uint4 x = *reinterpret_cast<const uint4*>(out + W::T + sw128(row, p));
+                T* o = static_cast<T*>(a.o) + (t0 + row) * a.ldo + head * a.DV + 8 * p;
+                for (int c = 0; c < a.DV; c += TV) *reinterpret_cast<uint4*>(o + c) = x;
+            }
+        }
     // ... then pairs of blocks, X_10 = -X_11 L_10 X_00 and X_32 likewise, then the lower left quarter from the halves on its sides.  A
     // product's result goes through shared memory: over the L that it used up.
     auto L = [&](int i, int j) { return sm.l + 16 * (i * LP + j); };
@@ -412,13 +419,14 @@ __device__ __noinline__ void give_up(int* abort, int warp) {
     atomicCAS(&g_prefill_status, 0, 1 + (warp < COMPUTE ? 0 : warp < WARP_MMA ? 1 : warp - 10));
 }
 
-struct WalkMaps { CUtensorMap q, k, v; };                        // 64 rows x 64 columns swizzled, 64 x 128 columns of V as they are
+struct WalkMaps { CUtensorMap q, k, v, o; };                     // 64 rows x 64 columns swizzled, 64 x 128 columns of V as they are
 
-template <int DK, bool FINE, int STAGES> struct WalkSmem {
+template <int DK, bool LO_WS, int STAGES> struct WalkSmem {
+    static constexpr int M_LO = (Ws<LO_WS>::BYTES + 1023) / 1024 * 1024;      // (not LO_WS) M lo from o's rows: 64 of 128 bytes, swizzled
     struct Stage {
         __align__(1024) uint8_t kq[2 * CT * DK * 2];             // scaled fp16 by halves of 64 keys: 64 rows of K, 64 rows of Q, 128 bytes each, swizzled
         __align__(1024) uint8_t v[CT * TV * 2];                  // [token][value] as it is
-        __align__(1024) uint8_t w[(Ws<FINE>::BYTES + 1023) / 1024 * 1024];
+        __align__(1024) uint8_t w[M_LO + (LO_WS ? 0 : CT * 128)];
     } st[STAGES];
     float vtop[2][TV], meet1[2][TV];                             // the chunk's largest |V| of a column; what its two threads tell each other
     __align__(16) float2 meet2[2][TV];
@@ -488,9 +496,9 @@ template <int N> __device__ __forceinline__ void regs_down() { asm volatile("set
 
 template <typename T, int DK, int STAGES>
 __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(const __grid_constant__ WalkMaps maps, const shvk_gdn_seq_args a, const uint8_t* __restrict__ ws, const WalkSegments seg, uint32_t polls, bool starve) {
-    constexpr bool FINE = std::is_same<T, __half>::value;
-    using W = Ws<FINE>;
-    using Sm = WalkSmem<DK, FINE, STAGES>;
+    constexpr bool LO_WS = M_LO_IN_WS<T>;
+    using W = Ws<LO_WS>;
+    using Sm = WalkSmem<DK, LO_WS, STAGES>;
     using C = Cols<DK>;
     constexpr int HALF = 2 * CT * 128;                           // bytes of 64 keys of K and Q
     extern __shared__ uint8_t walk_raw[];
@@ -696,12 +704,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 tc_wait_ld();
                 clean(x, p);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (FINE) split_pair(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
-                    else hi[i] = pack_half(x[2 * i], x[2 * i + 1]);
-                }
+                for (int i = 0; i < 8; ++i) split_pair(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
                 tc_st8(tl + C::R + 32 * half + 16 * p, hi);      // over the U that this round has read
-                if (FINE) tc_st8(tl + C::R + 32 * half + 16 * p + 8, lo);
+                tc_st8(tl + C::R + 32 * half + 16 * p + 8, lo);
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                     const float4 dk = dk4[i / 4];
@@ -886,7 +891,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                     for (int p = 0; p < DK / 16; ++p) {          // (Q S0)^T
                         const uint64_t b = b0 + uint64_t((p >> 2) * (HALF / 16) + 2 * (p & 3) + CT * 128 / 16);
                         mma_ts(qs, C::S + 8 * p, b, id64, p > 0);
-                        if (FINE) mma_ts(qs, C::S + DK / 2 + 8 * p, b, id64, true);
+                        mma_ts(qs, C::S + DK / 2 + 8 * p, b, id64, true);
                     }
                 }
                 wait(wfull(s), sph);
@@ -919,16 +924,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 wait(b_q, ph ^ 1u);                   // the last chunk's outputs are read
                 tc_fence_after();
                 if (!dead && lead) {
-                    const uint64_t m0 = desc_plain(wt, 128, 256);
+                    const uint64_t m0 = desc_plain(wt, 128, 256), o0 = smem_desc_sw128(wt + Sm::M_LO);
 #pragma unroll 1
                     for (int kk = 0; kk < 4; ++kk) {
                         const uint64_t mh = m0 + uint64_t((W::M + tri_step(kk)) / 16);
                         const uint32_t id = idesc_f16(64 - 16 * kk, false), d = C::MU + 16 * kk, u = C::R + 16 * kk;
                         mma_ts(d, u, mh, id, kk > 0);
-                        if (FINE) {
-                            mma_ts(d, u, m0 + uint64_t((W::ML + tri_step(kk)) / 16), id, true);
-                            mma_ts(d, u + 8, mh, id, true);
-                        }
+                        mma_ts(d, u, LO_WS ? m0 + uint64_t((W::ML + tri_step(kk)) / 16) : o0 + uint64_t(kk * (16 * 128 / 16 + 2)), id, true);
+                        mma_ts(d, u + 8, mh, id, true);
                     }
                     tc_commit(b_o);
                     tc_commit(empty(s));
@@ -953,7 +956,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                 const int y = start + c * CT;
                 wait(empty(s), sph ^ 1u);
                 if (!dead && lead && !(starve && c == 0)) {      // rows past the sequence are another's, past the last zeros: both unused
-                    mbar_expect_tx(wfull(s), W::BYTES + 2 * CT * DK * 2 + CT * TV * 2);
+                    mbar_expect_tx(wfull(s), W::BYTES + 2 * CT * DK * 2 + CT * TV * 2 + (LO_WS ? 0 : CT * 128));
 #pragma unroll
                     for (int h = 0; h < DK / 64; ++h) {
                         tma_load_2d(kq + h * HALF, &maps.k, khead * DK + 64 * h, y, wfull(s));
@@ -961,6 +964,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                     }
                     bulk_load(wt, src + (long long)c * a.HV * W::BYTES, W::BYTES, wfull(s));
                     tma_load_2d(vt, &maps.v, head * a.DV + (phi ? 0 : split * TV), y, wfull(s));
+                    if (!LO_WS) tma_load_2d(wt + Sm::M_LO, &maps.o, head * a.DV + (phi ? 0 : split * TV), y, wfull(s));
                 }
                 __syncwarp();
                 if (++s == STAGES) { s = 0; sph ^= 1u; }
@@ -1104,13 +1108,13 @@ inline size_t chunk_bytes(const shvk_gdn_seq_args& a) {
 }
 
 template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s, uint32_t polls, bool starve) {
-    constexpr bool FINE = std::is_same<T, __half>::value;
+    constexpr bool LO_WS = M_LO_IN_WS<T>;
     constexpr int STAGES = 3;
     const int chunks = segment_chunks(a);
     const long long segments = chunks ? segment_count(a, chunks) : 0, splits = (a.DV + TV - 1) / TV;
     const long long items = (a.n_tokens / CT + a.n_seq + 1) * a.HV, ctas = (chunks ? segments : a.n_seq) * a.HV * (splits + (chunks ? 1 : 0));
     if (items > 0x7fffffff || ctas > 0x7fffffff) return int(cudaErrorInvalidValue);
-    constexpr int prep_smem = int(sizeof(PrepSmem<DK, FINE>)) + 1024, smem = int(sizeof(WalkSmem<DK, FINE, STAGES>)) + 1024;
+    constexpr int prep_smem = int(sizeof(PrepSmem<DK, LO_WS>)) + 1024, smem = int(sizeof(WalkSmem<DK, LO_WS, STAGES>)) + 1024;
     static_assert(smem <= 227 * 1024, "the stages fit");
     cudaError_t e = cudaFuncSetAttribute(gdn_prefill_tc_prep_kernel<T, DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, prep_smem);
     if (e != cudaSuccess) return int(e);
@@ -1119,7 +1123,8 @@ template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t*
     WalkMaps maps;
     if (!tma::make_map_2d(&maps.q, a.q, 2, a.n_tokens, (long long)a.HK * DK, a.ldq, CT, 64, true) ||
         !tma::make_map_2d(&maps.k, a.k, 2, a.n_tokens, (long long)a.HK * DK, a.ldk, CT, 64, true) ||
-        !tma::make_map_2d(&maps.v, a.v, 2, a.n_tokens, (long long)a.HV * a.DV, a.ldv, CT, TV, false))
+        !tma::make_map_2d(&maps.v, a.v, 2, a.n_tokens, (long long)a.HV * a.DV, a.ldv, CT, TV, false) ||
+        !tma::make_map_2d(&maps.o, a.o, 2, a.n_tokens, (long long)a.HV * a.DV, a.ldo, CT, 64, true))
         return int(cudaErrorInvalidValue);
     // Ahead of the end of what ran before, but for calls in segments: calls in a row of 321 tokens 36.1 -> 34.0 us, of 64 x 2,048 tokens
     // 615.6 -> 614.6, but in segments 1 x 16,384 233.7 -> 235.2.

@@ -853,3 +853,44 @@ def test_slots_past_two_gigabytes(L):
     assert torch.equal(x["states"][slots - 2], small[0])
     del x
     torch.cuda.empty_cache()
+
+
+def form_of(L, x):
+    """Chunks of how many tokens the prefill takes this call in: those of 16 need 2,448 bytes for each chunk and value head, those of 64
+    another size."""
+    need = L.shvk_gdn_prefill_workspace_bytes(C.byref(args(x)))
+    return 16 if need == (x["rows"] // 16 + x["n"] + 1) * x["hv"] * 2448 else 64
+
+
+def assert_float32_outputs(x, want):
+    """The outputs are the rule's to float32's accuracy before they are rounded: few of them are another value of the type than the
+    float64 ones' rounding.  An error e moves an output over a tie with a probability of 2 e / step, a step is at least eps / 2 of the
+    value, and the mean of rms / |value| is some 4 (a normal value's, down to a thousandth of the rms).  With e within 2^-19 of the rms
+    (the state's error is held to 1e-6 of its norm, half of that), that is 16 x 2^-19 / eps of the outputs: 0.4 % for bf16, 3 % for fp16.
+    (Pieces of eleven bits, e of 2^-12, move 16 x 2^-12 / 2^-7 = 50 % at most, and some 5 % where they are off by chance.)"""
+    import torch
+    total = sum(x["lens"])
+    wrong = float((x["o"][:total] != want[:total].to(x["o"].dtype)).double().mean())
+    print(f"outputs that are not the float64 ones' rounding: {100 * wrong:.3f} %")
+    assert wrong <= 16 * 2.0 ** -19 / torch.finfo(x["o"].dtype).eps
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("form,layout,lens", [(16, (2, 6, 128, 128), [48, 0, 17, 33] * 5), (16, (6, 6, 64, 64), [100] * 30),
+                                              (16, (3, 3, 64, 32), [300, 129]), (16, (1, 1, 128, 96), [500]),
+                                              (64, (2, 6, 128, 128), [333, 64, 0, 190]), (64, (6, 6, 64, 128), [321]),
+                                              (64, (2, 2, 128, 256), [200, 77]), (64, (2, 4, 64, 192), [140, 300]),
+                                              (64, (1, 4, 64, 64), [150, 260]), (64, (1, 1, 128, 128), [3000])], ids=str)
+def test_prefill_outputs_are_float32_before_they_are_rounded(L, kind, form, layout, lens):
+    import torch
+    x = make(kind, lens, *layout, seed=len(lens) + layout[2])
+    assert form_of(L, x) == form
+    want, _, _ = rule(x, first_states(x))
+    check(L, "prefill", x)
+    assert_float32_outputs(x, want)
+    first, states = x["o"].clone(), x["states"].clone()          # whatever o's rows held before
+    x["o"][:sum(lens)] = torch.nan
+    launch(L, "prefill", x)
+    torch.cuda.synchronize()
+    assert torch.equal(x["o"], first) and torch.equal(x["states"], states)
