@@ -204,7 +204,8 @@ int shvk_gdn_step(const shvk_gdn_seq_args* a, void* stream);
  * larger).  Two launches; four where long sequences are too few to fill the GPU and are walked in segments (by n_seq, n_tokens and the
  * head sizes: a sequence's bits follow from those too).  `workspace` (device, 16-byte aligned, at least as many bytes as
  * shvk_gdn_prefill_workspace_bytes(a) says, contents irrelevant) holds what they hand on: calls that may overlap need their own.  Its
- * size follows from the counts, sizes and type; it is 0 for arguments that the call refuses. */
+ * size follows from the counts, sizes and type; it is 0 for arguments that the call refuses.  One piece of HV (n_tokens / 16 + n_seq + 1)
+ * 8,192 bytes is enough for every call of that many rows and sequences with DV up to 128. */
 size_t shvk_gdn_prefill_workspace_bytes(const shvk_gdn_seq_args* a);
 int shvk_gdn_prefill(const shvk_gdn_seq_args* a, void* workspace, size_t workspace_bytes, void* stream);
 /* Status word of that call, one per device and process: nonzero after a bounded wait inside a kernel gave up (the call's outputs are

@@ -600,15 +600,15 @@ template <typename T, int DK, int NW, int NSLOT, int MINCTA> int launch_scan(con
     return int(cudaGetLastError());
 }
 
-// Whether the chunks of 64 tokens take a call: sequences that on average fill a chunk (with the narrower keys: two).  us, 64 / 16: DK 128,
-// 128 sequences of 6 heads, 48 tokens 109 / 89, 64 111 / 111, 128 154 / 169; 37 of 500 138 / 185; 512 of 32 352 / 247, of 64 362 / 369, of
-// 321 1,098 / 1,324.  DK 64: 128 of 64 84 / 68, of 128 117 / 113; 37 of 500 107 / 122; 1 of 1,000 64 / 91.
+// Whether the chunks of 64 tokens take a call: sequences that on average fill two.  us, 64 / 16: DK 128, 128 sequences of 6 heads, 48 tokens
+// 130 / 85, 64 101 / 105, 72 162 / 119, 112 171 / 155, 128 143 / 169, of none to 256 184 / 189; 512 of 64 344 / 373, of 96 583 / 495, of 128
+// 491 / 610; 37 of 500 138 / 185.  DK 64: 128 of 64 81 / 65, of 128 114 / 112; 37 of 500 107 / 122; 1 of 1,000 64 / 91.
 // Heads that leave half of the 128 lanes idle go there while one wave of CTAs holds them, from two chunks on (DV 64, DK 64, 8 of 256 28 / 32,
 // of 2,048 131 / 186, but 37 of 256 58 / 40; DK 128, 1 of 128 24 / 29), and with the wider keys from eight chunks on (128 of 256 214 / 194, of
 // 512 358 / 366; 64 of 2,048 621 / 734; DK 64 516 / 366).
 inline bool takes_tc(const shvk_gdn_seq_args& a) {
     auto at_least = [&](long long tokens) { return a.n_tokens >= a.n_seq * tokens; };
-    if (a.DV % 128 == 0) return at_least(a.DK == 64 ? 128 : 64);
+    if (a.DV % 128 == 0) return at_least(128);
     if (a.DV % 64) return false;
     return (at_least(128) && (long long)a.n_seq * a.HV * ((a.DV + 127) / 128) <= device_sms()) || (a.DK == 128 && at_least(512));
 }

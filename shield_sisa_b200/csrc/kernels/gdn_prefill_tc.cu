@@ -408,10 +408,13 @@ constexpr uint32_t PREFILL_POLLS = 1u << 17;            // about half a second (
 // from there.  Sequence n's segments stand at first_chunk / chunks + n, as its chunks do.
 struct WalkSegments {
     int chunks, pass;                                            // 0, 0: no segments
-    float* x;                                                    // [segment][head][DK][DV]
-    float* phi;                                                  // [segment][head][column][key]
+    float* x;                                                    // [place][head][DK][DV]
+    float* phi;                                                  // [place][head][column][key]
 };
 __device__ __forceinline__ int first_segment(int first_chunk, int n, int chunks) { return first_chunk / chunks + n; }
+// Place of what a sequence's first segment leaves, the others' behind it.  All but the last leave something, (length - 1) / (64 chunks) of
+// them: never over those of n + 1, and no more than n_tokens / (64 chunks) in all.
+__device__ __forceinline__ int first_place(const SeqRows& r, int chunks) { return int(r.start / (CT * (long long)chunks)); }
 
 // (out of line: the waits' own code has to stay short)
 __device__ __noinline__ void give_up(int* abort, int warp) {
@@ -532,10 +535,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
     const bool writes = seg.pass != 1 || at == 0;                // outputs
     const long long in = at == 0 ? slot_of(a.slot_in, n, a.n_slots) : -1, out = last ? slot_of(a.slot_out, n, a.n_slots) : -1;
     const long long state_of = (long long)a.HV * DK * a.DV, state_at = (long long)head * DK * a.DV + split * TV;
+    const long long place = seg.chunks ? first_place(rows, seg.chunks) + at : 0;
     // where the state comes from and goes to: columns to_c apart, keys to_k
-    const float* from = in >= 0 ? a.states + in * state_of + state_at : seg.pass == 2 ? seg.x + (segment - 1) * state_of + state_at : nullptr;
-    float* to = last ? (out >= 0 ? a.states + out * state_of + state_at : nullptr) : phi ? seg.phi + ((long long)segment * a.HV + head) * DK * DK
-                : seg.pass == 1 ? seg.x + segment * state_of + state_at : nullptr;
+    const float* from = in >= 0 ? a.states + in * state_of + state_at : seg.pass == 2 ? seg.x + (place - 1) * state_of + state_at : nullptr;
+    float* to = last ? (out >= 0 ? a.states + out * state_of + state_at : nullptr) : phi ? seg.phi + (place * a.HV + head) * DK * DK
+                : seg.pass == 1 ? seg.x + place * state_of + state_at : nullptr;
     const long long to_k = phi ? 1 : a.DV, to_c = phi ? DK : 1;
     if (NB <= 0) {                                               // nothing to walk: the state as it is
         last_is_done();
@@ -1047,7 +1051,7 @@ template <int DK> __global__ void __launch_bounds__(JOIN_THREADS) gdn_prefill_tc
     if (segments < 3) return;
     const int key = threadIdx.x % DK, share = threadIdx.x / DK;
     const int k1 = threadIdx.x * EPT / JC, c1 = threadIdx.x * EPT % JC;
-    const long long first = first_segment(first_chunk(rows, n), n, seg.chunks), state_of = (long long)a.HV * DK * a.DV, phi_of = (long long)a.HV * DK * DK;
+    const long long first = first_place(rows, seg.chunks), state_of = (long long)a.HV * DK * a.DV, phi_of = (long long)a.HV * DK * DK;
     float* x = seg.x + first * state_of + ((long long)head * DK + k1) * a.DV + block * JC + c1;
     const float* phi = seg.phi + (first * a.HV + head) * DK * DK + (long long)(share * KPT) * DK + key;
     float p[KPT], y[EPT];
@@ -1102,9 +1106,11 @@ inline int segment_chunks(const shvk_gdn_seq_args& a) {
     return found;
 }
 inline long long segment_count(const shvk_gdn_seq_args& a, int chunks) { return (a.n_tokens / CT + a.n_seq + 1) / chunks + a.n_seq + 1; }
+inline long long place_count(const shvk_gdn_seq_args& a, int chunks) { return a.n_tokens / (CT * (long long)chunks); }
+// The last sequence's chunks end at start / 64 + n_seq - 1 + ceil(length / 64), no more than this.
+inline long long chunk_count(const shvk_gdn_seq_args& a) { return a.n_tokens / CT + a.n_seq; }
 inline size_t chunk_bytes(const shvk_gdn_seq_args& a) {
-    const size_t each = a.dtype == DT_F16 ? Ws<true>::BYTES : Ws<false>::BYTES;
-    return (size_t(a.n_tokens / CT + a.n_seq + 1) * size_t(a.HV) * each + 15) / 16 * 16;
+    return size_t(chunk_count(a)) * size_t(a.HV) * (a.dtype == DT_F16 ? Ws<true>::BYTES : Ws<false>::BYTES);
 }
 
 template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s, uint32_t polls, bool starve) {
@@ -1112,7 +1118,7 @@ template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t*
     constexpr int STAGES = 3;
     const int chunks = segment_chunks(a);
     const long long segments = chunks ? segment_count(a, chunks) : 0, splits = (a.DV + TV - 1) / TV;
-    const long long items = (a.n_tokens / CT + a.n_seq + 1) * a.HV, ctas = (chunks ? segments : a.n_seq) * a.HV * (splits + (chunks ? 1 : 0));
+    const long long items = chunk_count(a) * a.HV, ctas = (chunks ? segments : a.n_seq) * a.HV * (splits + (chunks ? 1 : 0));
     if (items > 0x7fffffff || ctas > 0x7fffffff) return int(cudaErrorInvalidValue);
     constexpr int prep_smem = int(sizeof(PrepSmem<DK, LO_WS>)) + 1024, smem = int(sizeof(WalkSmem<DK, LO_WS, STAGES>)) + 1024;
     static_assert(smem <= 227 * 1024, "the stages fit");
@@ -1140,7 +1146,7 @@ template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t*
     if (!chunks) return int(walk(ctas));
     seg.chunks = chunks;
     seg.x = reinterpret_cast<float*>(ws + chunk_bytes(a));
-    seg.phi = seg.x + segments * a.HV * DK * a.DV;
+    seg.phi = seg.x + place_count(a, chunks) * a.HV * DK * a.DV;
     seg.pass = 1;
     if ((e = walk(ctas)) != cudaSuccess) return int(e);
     if ((e = launch_behind(gdn_prefill_tc_join_kernel<DK>, (long long)a.n_seq * a.HV * (a.DV / JC), JOIN_THREADS, 0, s, a, seg)) != cudaSuccess) return int(e);
@@ -1152,7 +1158,7 @@ template <typename T, int DK> int launch_tc(const shvk_gdn_seq_args& a, uint8_t*
 
 size_t gdn_prefill_tc_workspace(const shvk_gdn_seq_args& a) {
     const int chunks = segment_chunks(a);
-    return chunk_bytes(a) + (chunks ? size_t(segment_count(a, chunks)) * size_t(a.HV) * size_t(a.DK) * size_t(a.DK + a.DV) * sizeof(float) : 0);
+    return chunk_bytes(a) + (chunks ? size_t(place_count(a, chunks)) * size_t(a.HV) * size_t(a.DK) * size_t(a.DK + a.DV) * sizeof(float) : 0);
 }
 int gdn_prefill_tc(const shvk_gdn_seq_args& a, uint8_t* ws, cudaStream_t s, int starve_polls) {
     const bool starve = starve_polls > 0;

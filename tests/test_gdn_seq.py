@@ -82,6 +82,22 @@ def test_prefill_refuses_its_workspace(L):
     assert L.shvk_gdn_prefill_workspace_bytes(None) == 0 and L.shvk_gdn_prefill(None, 0x200000, need, None) == INVALID
 
 
+def test_prefill_needs_no_more_than_a_program_keeps_for_it(L):
+    """One piece for calls of any lengths, as the header promises it: 8,192 bytes of a value head for every 16 rows and every sequence."""
+    import random
+    rng = random.Random(4)
+    log = lambda hi: int(hi ** rng.random())  # noqa: E731
+    segments = False
+    for i in range(20000):
+        n, hk, dk, dv, dtype = log(600), rng.choice([1, 2, 6]), rng.choice([64, 128]), rng.choice([32, 64, 96, 128, 128]), rng.choice([1, 2])
+        tokens, hv = n * log(20000) + rng.choice([0, 0, 3, 63]), hk * rng.choice([1, 2, 3])
+        a = good(n_seq=n, HK=hk, HV=hv, DK=dk, DV=dv, dtype=dtype, n_tokens=tokens, ldq=hk * dk, ldk=hk * dk, ldv=hv * dv, ldo=hv * dv, ldgb=hv)
+        need = L.shvk_gdn_prefill_workspace_bytes(C.byref(a))
+        assert 0 < need <= hv * (tokens // 16 + n + 1) * 8192, (n, hv, dk, dv, dtype, tokens)
+        segments |= need > 22032 * (tokens // 64 + n) * hv and dv > 64
+    assert segments                                             # calls that keep states of segments were among them
+
+
 def test_step_of_nothing_launches_nothing(L):
     assert L.shvk_gdn_step(None, None) == INVALID
     assert call(L, "step", good(n_seq=0)) == 0
