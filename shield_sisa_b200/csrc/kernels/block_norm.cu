@@ -13,6 +13,7 @@
 // 16-bit rows, one B200: 123,264 heads of 128 with a SiLU gate 20.7 us (95 MB, 0.70 of a plain copy's rate), 20,544 x 384 residual and norm
 // 18.1 us (0.79), four times as many rows of either 5.3 and 6.1 TB/s (0.81, 0.93): ramp up and drain.  16,384 x 2,048 with everything
 // 65 us (4.1 TB/s; two barriers of a CTA a row), x 2,047 95: masks at a row's ends, and sectors that two SMs write.
+#include "block_norm_rows.cuh"
 #include "device_utils.cuh"
 #include "launch_order.cuh"
 #include "shv_seq_kernels.h"
@@ -109,7 +110,7 @@ block_norm_kernel(const shvk_block_norm_args a, int P) {
     const int tid = threadIdx.x, rt = ROWT ? ROWT : blockDim.x, span = rt * NV * 8;
     const int groups = ROWT ? blockDim.x / ROWT : 1, grp = ROWT ? tid / ROWT : 0, j = ROWT ? tid % ROWT : tid;
     const int cls = blockIdx.x % P, cta = blockIdx.x / P, total = int(a.rows * a.heads);
-    const int off = int(cls * (a.ldx & 7) & 7);                  // where the class's rows start in a group (0 where P is 1)
+    const int off = row_shift(cls, a.ldx);                       // where the class's rows start in a group (0 where P is 1)
     // this group's rows are R, R + step, ...; as (row, head) they move by (step_row, step_head)
     const int step = int(gridDim.x / P) * groups * P, step_row = step / a.heads, step_head = step % a.heads;
     int R = (cta * groups + grp) * P + cls, row = R / a.heads, head = R % a.heads;
@@ -120,8 +121,14 @@ block_norm_kernel(const shvk_block_norm_args a, int P) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (j + i * rt) * 8 - off;                    // column of the group's first value
-        lo[i] = EDGE && c < 0 ? min(-c, 8) : 0;
-        hi[i] = EDGE ? max(min(a.D - c, 8), 0) : c < a.D ? 8 : 0;
+        lo[i] = EDGE ? group_lo(c) : 0;
+        hi[i] = EDGE ? group_hi(c, a.D) : c < a.D ? 8 : 0;
+    }
+    int whole = 0;                                               // rows in which a group over the row's end is read whole
+    if (EDGE) {
+        whole = whole_rows(int(a.rows), a.ldx);
+        if (a.h_in) whole = min(whole, whole_rows(int(a.rows), a.ldh_in));
+        if (row_gate) whole = min(whole, whole_rows(int(a.rows), a.ldgate));
     }
     auto full = [&](int i) { return !EDGE || hi[i] - lo[i] == 8; };
     struct Row {
@@ -143,10 +150,10 @@ block_norm_kernel(const shvk_block_norm_args a, int P) {
             if constexpr (sizeof(TH) == 4) r.h[i].w[1] = z;
             if (on && hi[i] > lo[i]) {
                 const int c = i * rt * 8;
-                const bool fits = !EDGE || base + c + 8 <= width, before = row + 1 < a.rows;
-                r.x[i] = get_raw(px + c, lo[i], hi[i], fits || (before && a.ldx >= width));
-                if (a.h_in) r.h[i] = get_raw(ph + c, lo[i], hi[i], fits || (before && a.ldh_in >= width));
-                if (row_gate) r.g[i] = get_raw(pg + c, lo[i], hi[i], fits || (before && a.ldgate >= width));
+                const bool all = !EDGE || reads_whole(base + c + 8, width, row, whole);
+                r.x[i] = get_raw(px + c, lo[i], hi[i], all);
+                if (a.h_in) r.h[i] = get_raw(ph + c, lo[i], hi[i], all);
+                if (row_gate) r.g[i] = get_raw(pg + c, lo[i], hi[i], all);
             }
         }
     };

@@ -305,3 +305,63 @@ def test_norms_behind_one_another(L, d):
     assert all(torch.isfinite(w.float()).all() for w in want)
     for _ in range(5):
         assert all(torch.equal(g, w) for g, w in zip(run(False), want))
+
+
+GROUPS = r"""
+#include <cuda_runtime.h>
+#include "block_norm_rows.cuh"
+#include <cstdio>
+// every group that a row of the kernel takes, for rows, pitch and width: reads outside the array, whole groups over a row's end
+int main() {
+    long long outside = 0, over = 0, groups = 0;
+    for (int D = 1; D <= 40; ++D)
+        for (long long ld = 0; ld <= 3 * D + 17; ++ld)
+            for (int rows = 1; rows <= 40; ++rows) {
+                const int P = ld % 8 == 0 ? 1 : ld % 2 ? 8 : ld % 4 ? 4 : 2, whole = sb::whole_rows(rows, ld);
+                const long long size = (rows - 1) * ld + D;
+                for (int row = 0; row < rows; ++row) {
+                    const int off = sb::row_shift(row % P, ld);
+                    if ((row * ld - off) % 8) return 1;          // a group starts where the loads do
+                    int seen = 0;
+                    for (int c = -off; c < D; c += 8) {
+                        const int lo = sb::group_lo(c), hi = sb::group_hi(c, D);
+                        if (hi <= lo) continue;
+                        const bool all = sb::reads_whole(c + 8, D, row, whole);
+                        const long long first = row * ld + c + (all ? 0 : lo), last = row * ld + c + (all ? 8 : hi);
+                        outside += first < 0 || last > size;
+                        over += all && hi < 8;
+                        seen += hi - lo;
+                        ++groups;
+                    }
+                    if (seen != D) return 2;
+                }
+            }
+    printf("%lld %lld %lld\n", groups, outside, over);
+}
+"""
+
+
+def test_no_group_is_read_past_its_array(tmp_path):
+    """The kernel's own rules for groups of eight, compiled for the host, over all small widths, pitches and numbers of rows."""
+    import subprocess
+
+    from shield_sisa_b200 import build
+    src, exe = tmp_path / "groups.cu", tmp_path / "groups"
+    src.write_text(GROUPS)
+    subprocess.run([build.NVCC, *build.NVCC_FLAGS, str(src), "-o", str(exe)], check=True, capture_output=True)
+    groups, outside, over = (int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split())
+    assert outside == 0 and groups > 1 << 20 and over > 1 << 18
+
+
+@gpu
+@pytest.mark.parametrize("kind,res", [("bf16", "fp32"), ("fp32", "fp32"), ("fp16", "fp16")])
+@pytest.mark.parametrize("d", [1, 2, 3, 4, 5, 6, 7, 9, 11, 13])
+def test_small_widths_in_arrays_without_a_tail(L, kind, res, d):
+    import torch
+    for rows in (1, 2, 3, 6, 9, 25):
+        x = make(kind, rows, 1, d, res=res, seed=d)
+        for name in ("x", "gate", "h_in", "h_out", "xn"):
+            x[name] = x[name].clone()
+        x["h_flat"] = x["n_flat"] = None
+        assert x["x"].untyped_storage().nbytes() == rows * d * x["x"].element_size()
+        check(L, x)
