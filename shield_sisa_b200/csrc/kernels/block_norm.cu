@@ -314,9 +314,11 @@ template <typename T, typename TH, int NV, int ROWT, bool EDGE>
 int launch_rows(const shvk_block_norm_args& a, int P, int threads, cudaStream_t s) {
     const int groups = ROWT ? threads / ROWT : 1, span = (ROWT ? ROWT : threads) * NV * 8;
     const int smem = 3 * span * int(sizeof(float));
-    static_assert(3 * 4 * 512 * 8 * sizeof(float) <= 200 * 1024, "the longest row's weights fit");
+    // (the kernel's limit is one for all callers: always the most that any of them needs, so that none lowers it under another's launch)
+    constexpr int most_smem = 3 * (ROWT ? ROWT : 512) * NV * 8 * int(sizeof(float));
+    static_assert(most_smem <= 200 * 1024, "the longest row's weights fit");
     if (smem > 47 * 1024) {                                      // (beside the sums of a CTA, which are static)
-        const cudaError_t e = cudaFuncSetAttribute(block_norm_kernel<T, TH, NV, ROWT, EDGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        const cudaError_t e = cudaFuncSetAttribute(block_norm_kernel<T, TH, NV, ROWT, EDGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);
         if (e != cudaSuccess) return int(e);
     }
     const long long need = ((a.rows * a.heads + P - 1) / P + groups - 1) / groups * P;     // CTAs of one pass over the rows
@@ -349,7 +351,7 @@ template <typename T, typename TH> int launch_block_norm(const shvk_block_norm_a
     const int P = ld == 0 ? 1 : ld % 2 ? 8 : ld % 4 ? 4 : 2, nvec = (a.D + (P > 1 ? 7 : 0) + 7) / 8;
     if (!vec || nvec > 2048) {
         const int smem = a.D * int(sizeof(float));
-        const cudaError_t e = cudaFuncSetAttribute(block_norm_any_kernel<T, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        const cudaError_t e = cudaFuncSetAttribute(block_norm_any_kernel<T, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize, BN_MAXD * int(sizeof(float)));
         if (e != cudaSuccess) return int(e);
         return int(launch_behind(block_norm_any_kernel<T, TH>, a.rows * a.heads, 256, smem, s, a));
     }

@@ -365,3 +365,55 @@ def test_small_widths_in_arrays_without_a_tail(L, kind, res, d):
         x["h_flat"] = x["n_flat"] = None
         assert x["x"].untyped_storage().nbytes() == rows * d * x["x"].element_size()
         check(L, x)
+
+
+@gpu
+def test_calls_of_two_threads_do_not_take_each_others_shared_memory(L):
+    """Widths that ask for little and for much shared memory, launched by two host threads at once: no call may refuse or change for the
+    other's sake.  (The limit of a kernel is one for all of its callers.)"""
+    import threading
+
+    import torch
+    wide = [make("bf16", 2, 1, 16384, res="fp32", seed=1, pad=8), make("bf16", 2, 1, 16380, res="fp32", seed=2, shift=1),
+            make("bf16", 2, 1, 6000, res="fp32", seed=3), make("bf16", 2, 1, 4095, res="fp32", seed=3)]
+    small = [make("bf16", 2, 1, 8200, res="fp32", seed=4, pad=8), make("bf16", 2, 1, 100, res="fp32", seed=5, shift=1),
+             make("bf16", 2, 1, 4160, res="fp32", seed=6), make("bf16", 2, 1, 521, res="fp32", seed=3)]
+    torch.cuda.synchronize()
+    streams, codes = [torch.cuda.Stream(), torch.cuda.Stream()], [set(), set()]
+
+    def work(i, calls):
+        torch.cuda.set_device(0)
+        packed = [args(x) for x in calls]
+        for _ in range(3000):
+            for a in packed:
+                codes[i].add(L.shvk_block_norm(C.byref(a), streams[i].cuda_stream))
+    threads = [threading.Thread(target=work, args=(i, calls)) for i, calls in enumerate((wide, small))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [{0}, {0}], codes
+    for x in wide + small:
+        check(L, x)
+
+
+@gpu
+def test_a_small_call_behind_a_large_one_in_a_graph(L):
+    """Both captured before the graph is made."""
+    import torch
+    calls = [make("bf16", 3, 1, d, res="fp32", seed=d, shift=s) for d, s in ((16384, 1), (100, 1), (8200, 0), (4160, 0))]
+    for x in calls:
+        launch(L, x)
+    torch.cuda.synchronize()
+    want = [(x["h_out"].clone(), x["xn"].clone()) for x in calls]
+    for order in (calls, calls[::-1]):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for x in order:
+                launch(L, x)
+        for x in calls:
+            x["h_out"].zero_(), x["xn"].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x["h_out"], w[0]) and torch.equal(x["xn"], w[1]) for x, w in zip(calls, want))
