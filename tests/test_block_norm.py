@@ -417,3 +417,38 @@ def test_a_small_call_behind_a_large_one_in_a_graph(L):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x["h_out"], w[0]) and torch.equal(x["xn"], w[1]) for x, w in zip(calls, want))
+
+
+@gpu
+@pytest.mark.parametrize("kind,res,h", [("bf16", "none", "fp32"), ("fp16", "none", "fp32"), ("bf16", "fp32", "fp32"), ("fp32", "none", "fp32"),
+                                        ("bf16", "none", "bf16"), ("fp16", "fp16", "fp16")])
+@pytest.mark.parametrize("act", [1, 2])
+@pytest.mark.parametrize("d", [384, 61, 2048, 12001])
+@pytest.mark.parametrize("gate", ["rows", "one"])
+def test_gates_far_from_zero(L, kind, res, h, act, d, gate):
+    """Gates of -100 to 100: float32 outputs are float32's although the gate has 16 bits, and a gate that is nearly closed is not taken for
+    a closed one (x of up to 2^100 behind it: values far above a type's smallest).  exp and the quotient stay within the half steps that
+    stand above; where exp's own result is subnormal it is off by 2^-149.  16-bit outputs come from a shorter exponential, whose argument
+    of up to 145 is rounded to 24 bits: 145 x 2^-24 and 2^-22, 2^-16 of the value in all, on top of their own rounding."""
+    import torch
+    x = make(kind, 9, 1, d, post=False, gate=gate, act=act, res=res, pre=False, seed=d, scale=1.0)
+    t, th = types(kind), types(h)
+    x["gate"][:, :d] = (200 * torch.rand(x["gate"].shape[0], d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(d)) - 100).to(t)
+    if kind != "fp16":
+        x["x"][::2, :d] = (x["x"][::2, :d].float() * 2.0 ** 100).to(t)
+    if res == "none":
+        x["h_flat"], x["h_out"] = None, torch.full((9, d), 5.0, device="cuda", dtype=th)
+    a = args(x)
+    a.h_dtype = CODES[h]
+    assert L.shvk_block_norm(C.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    y, g = x["x"][:, :d].double(), x["gate"][:, :d].double()
+    want = y * torch.sigmoid(g) * (g if act == 1 else 1)
+    off = (ERR + (0.0 if h == "fp32" else 2.0 ** -16)) * want.abs() + (y * (g if act == 1 else 1)).abs() * 2.0 ** -148
+    if res != "none":
+        r = x["h_in"][:, :d].double()
+        want, off = want + r, off + ERR * r.abs()
+    got = x["h_out"][:, :d].double()
+    half = torch.finfo(th).eps / 2
+    tiny = 2.0 ** -25 if h == "fp16" else 2.0 ** -149 if h == "fp32" else 2.0 ** -134
+    assert float(((got - want).abs() - half * want.abs() - off - tiny).max()) <= 0
