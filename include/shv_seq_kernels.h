@@ -177,7 +177,7 @@ int shvk_gdn_chunked(const void* q, const void* k, const void* v, const float* g
  * value outside [0, n_slots), or a NULL array, means a zero state and a state that is not kept.  The two may name the same slot.  A
  * slot is written by one sequence of a call at most, and read by no other sequence of that call then (what is left there or read
  * from there is unspecified otherwise).  A sequence without rows copies its state.  DK 64 or 128; DV a multiple of 32, 32 .. 256;
- * q, k, v, o and states 16-byte aligned, row pitches of q, k, v, o multiples of 16 bytes, none below its
+ * q, k, v, o and states 16-byte aligned, the other arrays 4-byte; row pitches of q, k, v, o multiples of 16 bytes, none below its
  * rows' width.  o and the states written overlap no other array of the call; the rows of o that a call writes may hold intermediate
  * values until it ends.  Launched on the current device.
  * Extends the reference's recurrence (engine/cuda/seq.cu:107-195: one sequence length, a zero initial state, none left). */

@@ -23,6 +23,7 @@ __device__ __forceinline__ long long slot_of(const int32_t* __restrict__ slots, 
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 // 0, or the error of arguments that no kernel may see.  Rows are read and written in 16-byte pieces.
 inline int check_gdn_seq(const shvk_gdn_seq_args* a) {
@@ -32,14 +33,15 @@ inline int check_gdn_seq(const shvk_gdn_seq_args* a) {
     if ((a->DK != 64 && a->DK != 128) || a->DV < 32 || a->DV > 256 || a->DV % 32) return bad;
     if (a->HK < 1 || a->HV < 1 || a->HV > 4096 || a->HV % a->HK) return bad;
     if (a->n_seq == 0) return 0;
-    if (!a->seq_start) return bad;
+    if (!a->seq_start || !aligned4(a->seq_start) || !aligned4(a->slot_in) || !aligned4(a->slot_out)) return bad;
     if (a->n_tokens > 0) {
         if (!a->q || !a->k || !a->v || !a->g || !a->beta || !a->o) return bad;
         if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o)) return bad;
+        if (!aligned4(a->g) || !aligned4(a->beta)) return bad;
         const long long vec = a->dtype == DT_F32 ? 4 : 8;
         const long long kw = (long long)a->HK * a->DK, vw = (long long)a->HV * a->DV, most = 1ll << 32;
         if (a->ldq < kw || a->ldk < kw || a->ldv < vw || a->ldgb < a->HV || a->ldo < vw) return bad;
-        if (a->ldq > most || a->ldk > most || a->ldv > most || a->ldo > most) return bad;
+        if (a->ldq > most || a->ldk > most || a->ldv > most || a->ldo > most || a->ldgb > most) return bad;
         if ((a->ldq | a->ldk | a->ldv | a->ldo) % vec) return bad;
     }
     if (a->n_slots < 0 || ((a->slot_in || a->slot_out) && (!a->states || !aligned16(a->states)))) return bad;

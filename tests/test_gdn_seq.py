@@ -64,6 +64,16 @@ def test_prefill_refuses(L, kw):
         assert L.shvk_gdn_prefill_workspace_bytes(C.byref(a)) == 0
 
 
+@pytest.mark.parametrize("form", ["step", "prefill"])
+@pytest.mark.parametrize("kw", [{name: 0x100000 + off} for name in ("g", "beta", "seq_start", "slot_in", "slot_out") for off in (1, 2, 3)] + [dict(ldgb=1 << 33)], ids=str)
+def test_refuses_arrays_that_no_word_is_read_from(L, form, kw):
+    """Float32 and int32 arrays that do not start on four bytes: a read would fault."""
+    a = good(**kw)
+    ws = 0x200000
+    assert (L.shvk_gdn_step(C.byref(a), None) if form == "step" else L.shvk_gdn_prefill(C.byref(a), ws, 1 << 40, None)) == INVALID
+    assert L.shvk_gdn_prefill_workspace_bytes(C.byref(a)) == 0
+
+
 def test_starved_launch_refuses_what_waits_for_nothing(L):
     a = good(DV=64, ldv=256, ldo=256)
     assert L.shvk_gdn_prefill_starved(C.byref(a), 0x200000, 1 << 40, 256, None) == INVALID
