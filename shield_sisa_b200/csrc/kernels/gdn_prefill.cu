@@ -635,7 +635,7 @@ template <typename T, int DK> int launch_prefill(const shvk_gdn_seq_args& a, uin
 
 extern "C" size_t shvk_gdn_prefill_workspace_bytes(const shvk_gdn_seq_args* a) {
     using namespace sb;
-    if (check_gdn_seq(a) || a->n_seq == 0) return 0;
+    if (check_gdn_seq(a) || a->n_seq == 0 || a->dtype == DT_F32) return 0;
     if (takes_tc(*a)) return gdn_prefill_tc_workspace(*a);
     return size_t(prefill_chunks(*a)) * size_t(a->HV) * size_t(PW_BYTES);
 }

@@ -108,6 +108,11 @@ def test_prefill_needs_no_more_than_a_program_keeps_for_it(L):
     assert segments                                             # calls that keep states of segments were among them
 
 
+def test_prefill_needs_nothing_for_a_type_that_it_refuses(L):
+    a = good(dtype=0)
+    assert L.shvk_gdn_prefill_workspace_bytes(C.byref(a)) == 0 and L.shvk_gdn_prefill(C.byref(a), 0x200000, 1 << 40, None) == INVALID
+
+
 def test_step_of_nothing_launches_nothing(L):
     assert L.shvk_gdn_step(None, None) == INVALID
     assert call(L, "step", good(n_seq=0)) == 0
