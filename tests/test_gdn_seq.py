@@ -925,3 +925,251 @@ def test_prefill_outputs_are_float32_before_they_are_rounded(L, kind, form, layo
     launch(L, "prefill", x)
     torch.cuda.synchronize()
     assert torch.equal(x["o"], first) and torch.equal(x["states"], states)
+
+
+# ---------------------------------------------------------------------------------------------- each form of the prefill at its edges
+SHORT = [(16, (2, 4, 64, 128), [20, 0, 33]), (16, (2, 4, 128, 128), [70, 0, 26])]
+FULL = [(64, (2, 4, 128, 128), [200, 0, 330]), (64, (2, 4, 64, 128), [300, 0, 260])]
+SEGMENTS = (64, (1, 2, 128, 128), [3900, 0, 5000])
+
+
+def of_form(L, case, kind="bf16", **kw):
+    form, layout, lens = case
+    x = make(kind, lens, *layout, **kw)
+    assert form_of(L, x) == form
+    return x
+
+
+@gpu
+@pytest.mark.parametrize("case", SHORT + FULL, ids=str)
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("name", list(slot_cases()))
+def test_slots_in_each_form(L, case, kind, name):
+    import torch
+    s = tuple(None if v is None else torch.tensor(v, device="cuda", dtype=torch.int32) for v in slot_cases()[name])
+    x = of_form(L, case, kind, seed=3, slots=s)
+    want, _, _ = rule(x, first_states(x))
+    check(L, "prefill", x)
+    assert_float32_outputs(x, want)
+    if name == "none":                                          # no pool at all
+        got, a = x["o"].clone(), args(x)
+        a.states, a.n_slots = None, 0
+        assert call(L, "prefill", a, x["ws"].data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(x["o"], got)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["in_place", "new", "not_kept", "outside"])
+def test_slots_of_sequences_in_segments(L, name):
+    import torch
+    s = tuple(torch.tensor(v, device="cuda", dtype=torch.int32) for v in slot_cases()[name])
+    x = of_form(L, SEGMENTS, seed=4, slots=s)
+    x["g"] *= 0.1
+    assert L.shvk_gdn_prefill_workspace_bytes(C.byref(args(x))) > 16912 * (x["rows"] // 64 + x["n"]) * x["hv"]      # states of segments
+    check(L, "prefill", x)
+
+
+@gpu
+@pytest.mark.parametrize("case", FULL, ids=str)
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+def test_bounds_that_are_no_bounds_in_chunks_of_64(L, case, kind):
+    """The first sequence is well described, the others have starts outside the rows."""
+    import torch
+    x, y = (of_form(L, case, kind, seed=9, tail=0) for _ in range(2))
+    rows, first = x["rows"], case[2][0]
+    x["seq_start"] = torch.tensor([0, first, -9, 1 << 30], device="cuda", dtype=torch.int32)      # its rows; none; all
+    y["seq_start"] = torch.tensor([0, first, first, first], device="cuda", dtype=torch.int32)
+    guards = [torch.full((rows + 256,) + x["o"].shape[1:], 7.0, device="cuda").to(x["o"].dtype) for _ in range(2)]
+    for z, g in zip((x, y), guards):
+        z["o"] = g[:rows]
+    pool = x["states"].clone()
+    launch(L, "prefill", x)
+    launch(L, "prefill", y)
+    torch.cuda.synchronize()
+    slot = int(x["slot_out"][0])
+    assert torch.equal(x["states"][slot], y["states"][slot]) and not torch.equal(pool[slot], x["states"][slot])
+    assert torch.equal(x["states"][2 * x["n"]], pool[2 * x["n"]]) and torch.equal(x["states"][:x["n"]], pool[:x["n"]])
+    assert all(torch.equal(g[rows:], torch.full_like(g[rows:], 7.0)) for g in guards)
+
+
+@gpu
+@pytest.mark.parametrize("form,layout,lens,at,lost", [(16, (2, 4, 64, 128), [40, 17], 7, 2.0 ** -24), (64, (2, 4, 64, 128), [160, 150], 70, 2.0 ** -17),
+                                                      (64, (2, 4, 128, 128), [160, 150], 70, 2.0 ** -16)], ids=str)
+@pytest.mark.parametrize("low", [-float("inf"), -3.4028234663852886e38])
+def test_a_decay_to_nothing_in_each_form(L, form, layout, lens, at, lost, low):
+    """As test_a_decay_to_nothing_forgets_everything has it, with each form's bound: chunks of 16 hold W to 2^-35 of a column's largest, so
+    16 x 8 x 2^-35 x 16 = 2^-24 of the fill; of 64, 64 x 8 x 2^-32 x 64 = 2^-17, with 128 keys (|k|_1 <= 11.4) 2^-16 at most."""
+    import torch
+    outs = []
+    for fill in (0.0, 1e3, 1e30):
+        x = of_form(L, (form, layout, lens), seed=11)
+        x["g"][at] = low
+        x["g"][lens[0] + 2] = low
+        x["states"][:2] = fill if fill else x["states"][:2]
+        launch(L, "prefill", x)
+        torch.cuda.synchronize()
+        outs.append((fill, x["o"][at:lens[0]].clone(), x["o"][lens[0] + 2:sum(lens)].clone(), x["states"][x["slot_out"].long()].clone()))
+    for fill, *got in outs:
+        for a, b in zip(outs[0][1:], got):
+            assert torch.isfinite(b).all()
+            step = 0.0 if a.dtype == torch.float32 else 2.0 ** -7
+            assert float((a.double() - b.double()).abs().max()) <= lost * fill + (step + 1e-5) * float(a.abs().max())
+    x = of_form(L, (form, layout, lens), seed=11)
+    x["g"][at] = low
+    x["g"][lens[0] + 2] = low
+    want, _, _ = rule(x, first_states(x))
+    check(L, "prefill", x)
+    assert_float32_outputs(x, want)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_not_a_number_stays_in_its_sequence_and_head_in_chunks_of_64(L, kind, dk):
+    """In one head's values of a sequence, in rows behind the last sequence (which a chunk's copies may bring in), and all over a sequence
+    beside others."""
+    import torch
+    case = (64, (2, 4, dk, 128), [150, 200, 130])
+    x, y = (of_form(L, case, kind, seed=13, tail=70) for _ in range(2))
+    x["v"][170, 128:256] = float("nan")                         # sequence 1, value head 1
+    for name in ("q", "k", "v", "g", "beta"):
+        x[name][480:] = float("nan")
+    launch(L, "prefill", x)
+    launch(L, "prefill", y)
+    torch.cuda.synchronize()
+    bad = torch.zeros(x["rows"], 4, dtype=torch.bool, device="cuda")
+    bad[170:350, 1] = True
+    assert torch.isnan(x["o"][bad].float()).all()
+    near = torch.zeros_like(bad)
+    near[150:170, 1] = True                                     # the bad token's own chunk (see the test of bad tokens)
+    assert torch.equal(x["o"][~bad & ~near], y["o"][~bad & ~near])
+    assert torch.isfinite(x["o"][near].float()).all()
+    sx, sy = (z["states"][z["slot_out"].long()] for z in (x, y))
+    keep = torch.ones(3, 4, dtype=torch.bool, device="cuda")
+    keep[1, 1] = False
+    assert torch.equal(sx[keep], sy[keep]) and torch.isnan(sx[1, 1]).all()
+    for name in ("q", "k", "v", "g", "beta"):                   # a whole sequence
+        x[name][150:350] = float("nan")
+    launch(L, "prefill", x)
+    torch.cuda.synchronize()
+    keep = torch.ones(x["rows"], dtype=torch.bool, device="cuda")
+    keep[150:350] = False
+    assert torch.equal(x["o"][keep], y["o"][keep]) and torch.isnan(x["o"][150:350].float()).all()
+    sx = x["states"][x["slot_out"].long()]
+    assert torch.equal(sx[[0, 2]], sy[[0, 2]]) and torch.isnan(sx[1]).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("case,bad_at", [((16, (2, 4, 64, 128), [20, 45, 21]), 23), ((64, (2, 4, 64, 128), [150, 200, 130]), 100),
+                                         ((64, (2, 4, 128, 128), [150, 200, 130]), 100)], ids=str)
+@pytest.mark.parametrize("name", ["q", "k", "v", "g", "beta"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_bad_token_in_each_form(L, kind, case, bad_at, name, bad):
+    """As test_a_bad_token_does_not_reach_the_tokens_before_it has it: other bits in the bad token's own chunk alone, and there by 2^-20 of
+    what enters an output and one step of its type."""
+    import torch
+    x, y = (of_form(L, case, kind, seed=13) for _ in range(2))
+    (a0, a1, _), chunk = case[2], case[0]
+    token, begin, end = a0 + bad_at, a0 + bad_at // chunk * chunk, a0 + a1
+    x[name][token] = bad
+    launch(L, "prefill", x)
+    launch(L, "prefill", y)
+    torch.cuda.synchronize()
+    keep = torch.ones(x["rows"], dtype=torch.bool, device="cuda")
+    keep[begin:end] = False
+    assert torch.equal(x["o"][keep], y["o"][keep])
+    a, b = x["o"][begin:token].double(), y["o"][begin:token].double()
+    assert token > begin and float(((a - b).abs() - torch.finfo(x["o"].dtype).eps * b.abs()).max()) <= 2.0 ** -20 * float(y["o"][a0:end].double().abs().max())
+    assert not torch.isfinite(x["o"][token].float()).all()
+    if name == "q":                                             # nothing but its own output
+        assert torch.equal(x["o"][token + 1:end], y["o"][token + 1:end])
+    sx, sy = (z["states"][z["slot_out"].long()] for z in (x, y))
+    assert torch.equal(sx[[0, 2]], sy[[0, 2]]) and (name == "q") == bool(torch.equal(sx[1], sy[1]))
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("unit", [False, True])
+def test_chunks_of_64_on_slices_of_one_row(L, kind, dk, unit):
+    """q, k and v side by side in rows that are wider than they are, outputs in rows with room between them."""
+    import torch
+    x = of_form(L, (64, (2, 4, dk, 128), [300, 5, 130]), kind, seed=5, fused=True, unit=unit)
+    wide = torch.full((x["rows"], 6, 128), 7.0, device="cuda").to(x["o"].dtype)
+    x["o"] = wide[:, 1:5]
+    want, _, _ = rule(x, first_states(x))
+    check(L, "prefill", x)
+    assert_float32_outputs(x, want)
+    assert torch.equal(wide[:, [0, 5]], torch.full_like(wide[:, [0, 5]], 7.0))
+
+
+@gpu
+@pytest.mark.parametrize("case", FULL + [SEGMENTS], ids=str)
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+def test_chunks_of_64_captured_replayed_and_on_two_streams(L, case, kind):
+    import torch
+    x, y = of_form(L, case, kind, seed=31), of_form(L, case, kind, seed=32)
+    launch(L, "prefill", x)                                     # sizes the workspace outside the capture
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        launch(L, "prefill", x)
+    for name in ("q", "k", "v", "g", "beta", "states", "slot_out"):
+        x[name].copy_(y[name])
+    graph.replay()
+    launch(L, "prefill", y)
+    torch.cuda.synchronize()
+    assert torch.equal(x["o"], y["o"]) and torch.equal(x["states"], y["states"])
+    calls = [of_form(L, case, kind, seed=41 + i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(3):
+        for z, s in zip(calls, streams):
+            launch(L, "prefill", z, stream=s)
+    torch.cuda.synchronize()
+    for i, z in enumerate(calls):
+        w = of_form(L, case, kind, seed=41 + i)
+        launch(L, "prefill", w)
+        torch.cuda.synchronize()
+        assert torch.equal(z["o"], w["o"]) and torch.equal(z["states"], w["states"])
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_steps_continue_what_chunks_of_64_left(L, kind, dk):
+    """A prompt in two calls of the chunked form, the second from where the first stopped, then tokens in place, against one walk of all."""
+    import torch
+    layout, cuts = (2, 4, dk, 128), [(200, 130), (150, 140), (141, 300)]
+    new = 3
+    lens = [a + b + new for a, b in cuts]
+    whole = make(kind, lens, *layout, seed=23, tail=0)
+    want, states, _ = rule(whole, first_states(whole))
+    starts = np.concatenate([[0], np.cumsum(lens)])
+    half = torch.finfo(whole["o"].dtype).eps / 2
+    factor = (dk + 24 * max(lens)) * 2.0 ** -24
+    big = max(float(s.norm(dim=1).max()) for s in states) + float(want.abs().max()) + float(whole["states"].norm(dim=2).max())
+    done = [0, 0, 0]
+    for step, size in enumerate([[a for a, _ in cuts], [b for _, b in cuts]] + [[1, 1, 1]] * new):
+        pick = torch.tensor([starts[i] + done[i] + j for i in range(3) for j in range(size[i])], device="cuda")
+        x = dict(whole)
+        x.pop("ws", None)
+        for name in ("q", "k", "v", "g", "beta"):
+            x[name] = whole[name][pick].contiguous()
+        x["rows"], x["lens"] = len(pick), size
+        x["o"] = torch.full((len(pick), 4, 128), 7.0, device="cuda").to(whole["o"].dtype)
+        x["seq_start"] = torch.from_numpy(np.concatenate([[0], np.cumsum(size)]).astype(np.int32)).cuda()
+        if step:
+            x["slot_in"] = whole["slot_out"]
+        if step < 2:
+            assert form_of(L, x) == 64
+        launch(L, "prefill" if step < 2 else "step", x)
+        torch.cuda.synchronize()
+        ref = want[pick]
+        assert float(((x["o"].double() - ref).abs() - half * ref.abs()).max()) <= factor * big + (2.0 ** -25 if kind == "fp16" else 0.0)
+        done = [d + s for d, s in zip(done, size)]
+    for i in range(3):
+        got = whole["states"][int(whole["slot_out"][i])].double()
+        assert float((got - states[i]).abs().max()) <= factor * max(float(states[i].norm(dim=1).max()), big)
