@@ -414,7 +414,7 @@ struct WalkSegments {
 __device__ __forceinline__ int first_segment(int first_chunk, int n, int chunks) { return first_chunk / chunks + n; }
 // Place of what a sequence's first segment leaves, the others' behind it.  All but the last leave something, (length - 1) / (64 chunks) of
 // them: never over those of n + 1, and no more than n_tokens / (64 chunks) in all.
-__device__ __forceinline__ int first_place(const SeqRows& r, int chunks) { return int(r.start / (CT * (long long)chunks)); }
+__device__ __forceinline__ int first_place(const SeqRows& r, int chunks) { return r.start / (CT * chunks); }
 
 // (out of line: the waits' own code has to stay short)
 __device__ __noinline__ void give_up(int* abort, int warp) {
@@ -535,10 +535,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
     const bool writes = seg.pass != 1 || at == 0;                // outputs
     const long long in = at == 0 ? slot_of(a.slot_in, n, a.n_slots) : -1, out = last ? slot_of(a.slot_out, n, a.n_slots) : -1;
     const long long state_of = (long long)a.HV * DK * a.DV, state_at = (long long)head * DK * a.DV + split * TV;
-    const long long place = seg.chunks ? first_place(rows, seg.chunks) + at : 0;
+    const int place = seg.chunks ? first_place(rows, seg.chunks) + at : 0;
     // where the state comes from and goes to: columns to_c apart, keys to_k
     const float* from = in >= 0 ? a.states + in * state_of + state_at : seg.pass == 2 ? seg.x + (place - 1) * state_of + state_at : nullptr;
-    float* to = last ? (out >= 0 ? a.states + out * state_of + state_at : nullptr) : phi ? seg.phi + (place * a.HV + head) * DK * DK
+    float* to = last ? (out >= 0 ? a.states + out * state_of + state_at : nullptr) : phi ? seg.phi + ((long long)place * a.HV + head) * DK * DK
                 : seg.pass == 1 ? seg.x + place * state_of + state_at : nullptr;
     const long long to_k = phi ? 1 : a.DV, to_c = phi ? DK : 1;
     if (NB <= 0) {                                               // nothing to walk: the state as it is
