@@ -59,18 +59,6 @@ __device__ int g_prefill_status = 0;                             // 1 + role who
 // 128-byte rows, 16-byte pieces swizzled by the row: what SWIZZLE_128B reads
 __device__ __forceinline__ uint32_t sw128(int row, int piece) { return uint32_t(row * 128 + ((piece ^ (row & 7)) << 4)); }
 
-__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 // Chunks of sequence n stand at [start / 64 + n, .. + ceil(length / 64)) of the workspace: never over those of n + 1, for any lengths.
 __device__ __forceinline__ int first_chunk(const SeqRows& r, int n) { return r.start / CT + n; }
@@ -488,10 +476,6 @@ __device__ __forceinline__ void tc_st8(uint32_t t, const uint32_t* r) {
                  ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar) : "memory");
-}
 __device__ __forceinline__ void pair_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); }
 // registers of a warp group: 512 threads start with 128 each; 2 x 152 + 2 x 104 = 4 x 128
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -966,7 +950,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gdn_prefill_tc_walk_kernel(cons
                         tma_load_2d(kq + h * HALF, &maps.k, khead * DK + 64 * h, y, wfull(s));
                         tma_load_2d(kq + h * HALF + CT * 128, &maps.q, khead * DK + 64 * h, y, wfull(s));
                     }
-                    bulk_load(wt, src + (long long)c * a.HV * W::BYTES, W::BYTES, wfull(s));
+                    tma::load_bulk(wt, src + (long long)c * a.HV * W::BYTES, W::BYTES, wfull(s));
                     tma_load_2d(vt, &maps.v, head * a.DV + (phi ? 0 : split * TV), y, wfull(s));
                     if (!LO_WS) tma_load_2d(wt + Sm::M_LO, &maps.o, head * a.DV + (phi ? 0 : split * TV), y, wfull(s));
                 }
