@@ -452,3 +452,47 @@ def test_gates_far_from_zero(L, kind, res, h, act, d, gate):
     half = torch.finfo(th).eps / 2
     tiny = 2.0 ** -25 if h == "fp16" else 2.0 ** -149 if h == "fp32" else 2.0 ** -134
     assert float(((got - want).abs() - half * want.abs() - off - tiny).max()) <= 0
+
+
+@gpu
+@pytest.mark.parametrize("d", [5, 128, 384, 2047, 2048, 12001])
+def test_the_next_norm_over_the_input(L, d):
+    """xn over x and h over the residual, at once: the same bits as into arrays of their own."""
+    import torch
+    x, y = make("bf16", 301, 1, d, seed=d), make("bf16", 301, 1, d, seed=d)
+    launch(L, x)
+    y["xn"], y["h_out"] = y["x"], y["h_in"]
+    launch(L, y)
+    torch.cuda.synchronize()
+    assert torch.equal(x["xn"], y["x"]) and torch.equal(x["h_out"], y["h_in"])
+
+
+@gpu
+@pytest.mark.parametrize("d,pad", [(384, 0), (381, 0), (384, 3)])
+def test_rows_past_two_gigabytes(L, d, pad):
+    """More than 2^31 values in an array: the last rows as they come out alone."""
+    import torch
+    rows = (1 << 31) // (d + pad) + 100
+    rows += -rows % 8                                            # (the last eight rows start at the places that eight rows alone have)
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    flat = torch.zeros(rows * (d + pad) + 16, device="cuda", dtype=torch.bfloat16)
+    shift = 1 if pad else 0
+    big = flat[shift:shift + rows * (d + pad)].view(rows, d + pad)
+    last = torch.randn(8, d, device="cuda", generator=gen).bfloat16()
+    big[-8:, :d] = last
+    w = 1 + 0.3 * torch.randn(d, device="cuda", generator=gen)
+
+    def norm(x, n):
+        a = binding.BlockNormArgs(rows=n, heads=1, D=d, x=x.data_ptr(), ldx=d + pad, x_dtype=1, post_w=w.data_ptr(), scale=0.5, h_out=x.data_ptr(),
+                                  ldh_out=d + pad, h_dtype=1, eps=1e-6)
+        assert L.shvk_block_norm(C.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    small_flat = torch.zeros(8 * (d + pad) + 16, device="cuda", dtype=torch.bfloat16)
+    small = small_flat[shift:shift + 8 * (d + pad)].view(8, d + pad)
+    small[:, :d] = last
+    norm(big, rows)
+    norm(small, 8)
+    torch.cuda.synchronize()
+    assert torch.equal(big[-8:], small) and not flat[:(rows - 8) * (d + pad)].any()
+    assert torch.isfinite(small.float()).all() and small[:, :d].any(dim=1).all()
+    del big, flat
+    torch.cuda.empty_cache()

@@ -1173,3 +1173,55 @@ def test_steps_continue_what_chunks_of_64_left(L, kind, dk):
     for i in range(3):
         got = whole["states"][int(whole["slot_out"][i])].double()
         assert float((got - states[i]).abs().max()) <= factor * max(float(states[i].norm(dim=1).max()), big)
+
+
+@gpu
+@pytest.mark.parametrize("form", ["step", "prefill"])
+def test_no_rows_at_all_copy_the_states(L, form):
+    """Sequences in a call without a single row: states go from slot to slot, or start from zero; no array of rows is there."""
+    import torch
+    for dk, slots in ((64, ([2, 0, -1], [4, 5, 6])), (128, ([1, 1, 0], [3, -1, 0])), (64, (None, [0, 1, 2]))):
+        s = tuple(None if v is None else torch.tensor(v, device="cuda", dtype=torch.int32) for v in slots)
+        x = make("bf16", [0, 0, 0], 2, 4, dk, 128, seed=5, tail=0, slots=s)
+        first, pool = first_states(x), x["states"].clone()
+        a = args(x)
+        a.q = a.k = a.v = a.g = a.beta = a.o = None
+        need = L.shvk_gdn_prefill_workspace_bytes(C.byref(a))
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+        assert call(L, form, a, ws.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        for n, out in enumerate(slots[1]):
+            if out >= 0:
+                pool[out] = first[n]
+        assert torch.equal(x["states"], pool)
+
+
+@gpu
+@pytest.mark.parametrize("form,layout,lens", [("step", (2, 4, 64, 128), [3, 0, 2]), (16, (2, 4, 128, 128), [40, 0, 26]), (64, (2, 4, 128, 128), [200, 0, 330])], ids=str)
+def test_rows_past_two_gigabytes(L, form, layout, lens):
+    """Rows so far apart that the last ones lie beyond 2^31 values of their arrays."""
+    import torch
+    x = make("bf16", lens, *layout, seed=53)
+    y = dict(x)
+    y["states"] = x["states"].clone()
+    rows = x["rows"]
+    pitch = ((1 << 31) // (rows - 5) // 8 + 1) * 8
+    flat = torch.empty(rows * pitch, device="cuda", dtype=torch.bfloat16)
+    big = flat.view(rows, pitch)
+    at = 0
+    for name in ("q", "k", "v"):                                # one behind the other in rows of one array
+        w = x[name].shape[1]
+        big[:, at:at + w] = x[name]
+        y[name] = big[:, at:at + w]
+        at += w
+    y["o"] = big[:, at:at + layout[1] * layout[3]].unflatten(1, (layout[1], layout[3]))
+    y["o"].fill_(7.0)
+    assert (rows - 4) * pitch > 1 << 31
+    if form != "step":
+        assert form_of(L, x) == form and form_of(L, y) == form
+    for z in (x, y):
+        launch(L, "step" if form == "step" else "prefill", z)
+    torch.cuda.synchronize()
+    assert torch.equal(x["o"], y["o"]) and torch.equal(x["states"], y["states"]) and torch.isfinite(x["o"].float()).all()
+    del x, y, big, flat
+    torch.cuda.empty_cache()
