@@ -12,13 +12,12 @@
 // three) but not the range, so everything is scaled by powers of two, which cost no bits: a token's k and q by their norms, T by its
 // largest entry, rows of M by theirs, and the rows of S^T, W^T, U^T (one value column each; what a chunk does to them is linear) by scales
 // that the walk keeps or finds anew.  On the output's way S, M and U are two pieces as well (with one, of eleven bits, 11 % of bf16
-// outputs were not the rounded value of the rule, now 0.03 %, and less than a thousandth of each where terms cancel; it costs 4 % here, 5 %
-// in gdn_prefill_tc.cu).  Sums over tokens that last, S = e S + P, are rounded float32 FMAs and not tensor-core accumulations, whose
+// outputs were not the rule's value rounded, now 0.03 %, in gdn_prefill_tc.cu 0.12 %; it costs 4 % of the time here, 6 % there).  Sums over tokens that last, S = e S + P, are rounded float32 FMAs and not tensor-core accumulations, whose
 // truncation would lean one way for thousands of chunks.
 //
 // This form takes short sequences and the widths that fill no CTA of gdn_prefill_tc.cu (see takes_tc).  128 sequences of 48 tokens, 6 heads of
-// 128 x 128, bf16: 83 us in a graph, for 38 MB of rows and 100 MB of states (21 us).  The walk's chain binds, dependent products and exchanges among
-// lanes: some 2,400 cycles for a chunk of 16 tokens (1.3 us; the 1,024 of one sequence 1.34 ms).
+// 128 x 128, bf16: 80 us, for 38 MB of rows and 100 MB of states (21 us).  The walk's chain binds, dependent products and exchanges among
+// lanes: some 2,300 cycles for a chunk of 16 tokens (1.2 us; the 1,024 of one sequence 1.25 ms).
 #include "gdn_pieces.cuh"
 #include "gdn_seq.cuh"
 
@@ -254,8 +253,8 @@ template <int DK, int VC, int NSLOT> struct ScanSmem {
 
 // NW warps, 16 value columns each: a CTA has VC = 16 NW of the head's DV.  The values are the rows of the products (S^T, U^T: M = 16),
 // so that what one product leaves in registers is the next one's operand as it lies.
-template <typename T, int DK, int NW, int NSLOT, int MINCTA>
-__global__ void __launch_bounds__(NW * 32, MINCTA) gdn_prefill_scan_kernel(const shvk_gdn_seq_args a, const uint8_t* __restrict__ ws) {
+template <typename T, int DK, int NW, int NSLOT>
+__global__ void __launch_bounds__(NW * 32, 1) gdn_prefill_scan_kernel(const shvk_gdn_seq_args a, const uint8_t* __restrict__ ws) {
     constexpr int VC = 16 * NW, NT = NW * 32, KSTEP = DK / 16, NJ = DK / 8, ROWB = DK * 2, VROWB = VC * 2, VPR = DK / 8, VPV = VC / 8;
     constexpr int KN = PB * VPR, VN = PB * VPV, WN = PW_BYTES / 16;
     extern __shared__ __align__(128) uint8_t scan_raw[];
@@ -577,23 +576,23 @@ __global__ void __launch_bounds__(NW * 32, MINCTA) gdn_prefill_scan_kernel(const
     }
 }
 
-template <typename T, int DK, int NW, int NSLOT, int MINCTA> int launch_scan(const shvk_gdn_seq_args& a, const uint8_t* ws, cudaStream_t s) {
+template <typename T, int DK, int NW, int NSLOT> int launch_scan(const shvk_gdn_seq_args& a, const uint8_t* ws, cudaStream_t s) {
     constexpr int smem = int(sizeof(ScanSmem<DK, 16 * NW, NSLOT>));
     const long long ctas = (long long)a.n_seq * a.HV * (a.DV / (16 * NW));
     if (ctas > 0x7fffffff) return int(cudaErrorInvalidValue);
-    const cudaError_t e = cudaFuncSetAttribute(gdn_prefill_scan_kernel<T, DK, NW, NSLOT, MINCTA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(gdn_prefill_scan_kernel<T, DK, NW, NSLOT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return int(e);
-    if (a.n_tokens > 0) return int(launch_behind(gdn_prefill_scan_kernel<T, DK, NW, NSLOT, MINCTA>, ctas, NW * 32, smem, s, a, ws));
-    gdn_prefill_scan_kernel<T, DK, NW, NSLOT, MINCTA><<<unsigned(ctas), NW * 32, smem, s>>>(a, ws);      // (behind no preparation)
+    if (a.n_tokens > 0) return int(launch_behind(gdn_prefill_scan_kernel<T, DK, NW, NSLOT>, ctas, NW * 32, smem, s, a, ws));
+    gdn_prefill_scan_kernel<T, DK, NW, NSLOT><<<unsigned(ctas), NW * 32, smem, s>>>(a, ws);      // (behind no preparation)
     return int(cudaGetLastError());
 }
 
-// Whether the chunks of 64 tokens take a call: sequences that on average fill two.  us, 64 / 16: DK 128, 128 sequences of 6 heads, 48 tokens
-// 130 / 85, 64 101 / 105, 72 162 / 119, 112 171 / 155, 128 143 / 169, of none to 256 184 / 189; 512 of 64 344 / 373, of 96 583 / 495, of 128
-// 491 / 610; 37 of 500 138 / 185.  DK 64: 128 of 64 81 / 65, of 128 114 / 112; 37 of 500 107 / 122; 1 of 1,000 64 / 91.
-// Heads that leave half of the 128 lanes idle go there while one wave of CTAs holds them, from two chunks on (DV 64, DK 64, 8 of 256 28 / 32,
-// of 2,048 131 / 186, but 37 of 256 58 / 40; DK 128, 1 of 128 24 / 29), and with the wider keys from eight chunks on (128 of 256 214 / 194, of
-// 512 358 / 366; 64 of 2,048 621 / 734; DK 64 516 / 366).
+// Whether the chunks of 64 tokens take a call: sequences that on average fill two.  us, 64 / 16, bf16, 6 heads: DK 128, 128 sequences of 48
+// tokens 130 / 80, 64 101 / 99, 72 162 / 113, 112 171 / 147, 128 143 / 160, of none to 256 184 / 187; 512 of 64 345 / 360, of 96 584 / 489, of
+// 128 492 / 606, of 321 1,140 / 1,418; 37 of 500 136 / 171.  DK 64: 128 of 64 81 / 58, of 128 114 / 102; 37 of 500 111 / 120; 1 of 1,000 65 / 79.
+// Heads that leave half of the 128 lanes idle go there while one wave of CTAs holds them, from two chunks on (DV 64, DK 64, 8 of 256 29 / 27,
+// of 2,048 133 / 205, but 37 of 256 58 / 38; DK 128, 1 of 128 21 / 24), and with the wider keys from eight chunks on (128 of 256 210 / 198, of
+// 512 357 / 378; 64 of 2,048 625 / 746; DK 64 537 / 441).
 inline bool takes_tc(const shvk_gdn_seq_args& a) {
     auto at_least = [&](long long tokens) { return a.n_tokens >= a.n_seq * tokens; };
     if (a.DV % 128 == 0) return at_least(128);
@@ -612,10 +611,10 @@ template <typename T, int DK> int launch_prefill(const shvk_gdn_seq_args& a, uin
         if (e != cudaSuccess) return int(e);
         if (const cudaError_t le = launch_behind(gdn_prefill_prep_kernel<T, DK>, ctas, 128, smem, s, a, ws, items); le != cudaSuccess) return int(le);
     }
-    const long long heads = (long long)a.n_seq * a.HV;
-    if (a.DV % 128 == 0 && heads > device_sms()) return launch_scan<T, DK, 8, 4, 1>(a, ws, s);
-    if (a.DV % 64 == 0 && heads * (a.DV / 64) > device_sms()) return launch_scan<T, DK, 4, 4, 1>(a, ws, s);
-    return launch_scan<T, DK, 2, 4, 1>(a, ws, s);
+    // Four warps wherever they divide the columns.  us with two, four and eight warps a CTA, DV 128, sequences of 48 tokens, 6 heads: DK 128, 8 of
+    // them 19.0, 17.9, -; 50 41.3, 38.3, 41.0; 128 82.8, 79.5, 84.7; DK 64, 128 50.3, 48.4, 52.9 (two CTAs of four warps and 220 registers stand
+    // on an SM, one of eight; two warps bring K and Q in twice as often).
+    return a.DV % 64 == 0 ? launch_scan<T, DK, 4, 4>(a, ws, s) : launch_scan<T, DK, 2, 4>(a, ws, s);
 }
 
 }  // namespace
