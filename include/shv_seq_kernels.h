@@ -167,7 +167,7 @@ int shvk_gdn_chunked(const void* q, const void* k, const void* v, const float* g
 
 /* The gated delta rule with states that are kept between calls, over packed sequences.  Rows of all sequences lie one behind the
  * other: sequence n has the rows seq_start[n] .. seq_start[n + 1] - 1 (device, [n_seq + 1], not falling, at most n_tokens); a sequence
- * may have no rows, and rows behind the last sequence are neither read nor written.  q, k, v, o in `dtype` with row pitches in
+ * may have no rows; rows behind the last sequence are not written, and what stands in them has no influence.  q, k, v, o in `dtype` with row pitches in
  * elements, head h at h * DK (q, k) or h * DV (v, o) of its row; HK query / key heads, HV value heads, value head h uses key head
  * h / (HV / HK).  g (log decay) and beta fp32, row pitch ldgb.  l2norm != 0: q and k are divided by sqrt(x.x + 1e-6) first; q is
  * multiplied by `scale` either way.  g is meant to be at most 0 (a state grows without bound otherwise, and sums of positive g over 64
@@ -180,6 +180,9 @@ int shvk_gdn_chunked(const void* q, const void* k, const void* v, const float* g
  * q, k, v, o and states 16-byte aligned, the other arrays 4-byte; row pitches of q, k, v, o multiples of 16 bytes, none below its
  * rows' width.  o and the states written overlap no other array of the call; the rows of o that a call writes may hold intermediate
  * values until it ends.  Launched on the current device.
+ * This call and the next ones (shvk_gdn_step, shvk_gdn_prefill, shvk_block_norm) let a kernel that a caller launches behind them with
+ * programmatic ordering start early, while kernels in front of the call may still run: such a kernel waits for its predecessor
+ * (griddepcontrol.wait) before it reads anything that any earlier work of the stream writes.  Other launches are not concerned.
  * Extends the reference's recurrence (engine/cuda/seq.cu:107-195: one sequence length, a zero initial state, none left). */
 typedef struct shvk_gdn_seq_args {
     int n_seq, HK, HV, DK, DV;

@@ -10,9 +10,9 @@
 // cut at the same places, so that its copy of the weights in shared memory, shifted as its rows are, serves them all with 16-byte
 // reads.  A group that reaches over a row's end is read whole where that stays in the array, and written value by value.
 //
-// 16-bit rows, one B200: 123,264 heads of 128 with a SiLU gate 20.7 us (95 MB, 0.70 of a plain copy's rate), 20,544 x 384 residual and norm
-// 18.1 us (0.79), four times as many rows of either 5.3 and 6.1 TB/s (0.81, 0.93): ramp up and drain.  16,384 x 2,048 with everything
-// 65 us (4.1 TB/s; two barriers of a CTA a row), x 2,047 95: masks at a row's ends, and sectors that two SMs write.
+// 16-bit rows, one B200: 123,264 heads of 128 with a SiLU gate 20.2 us (95 MB, 0.71 of a plain copy's rate), 20,544 x 384 residual and norm
+// 18.2 us (0.79), four times as many rows of either 5.4 and 6.1 TB/s (0.82, 0.93): ramp up and drain.  16,384 x 2,048 with everything
+// 65 us (4.1 TB/s; two barriers of a CTA a row), x 2,047 93: masks at a row's ends, and sectors that two SMs write.
 #include "block_norm_rows.cuh"
 #include "device_utils.cuh"
 #include "launch_order.cuh"
@@ -53,7 +53,7 @@ template <typename T> __device__ __forceinline__ void put8(T* p, const float (&v
 template <typename T> struct Raw { uint4 w[sizeof(T) == 4 ? 2 : 1]; };
 // The values [lo, hi) of a group, the others as it may be: the whole group in one or two accesses where all of it lies in the array
 // (`whole`: everywhere but at an array's end), else value by value.  (Value by value at every row's edges, loads waited for one another:
-// 189 us for 16,384 rows of 2,047, now 95.)
+// 189 us for 16,384 rows of 2,047, now 93.)
 template <typename T> __device__ __forceinline__ Raw<T> get_raw(const T* p, int lo, int hi, bool whole) {
     Raw<T> r;
     if (whole) {
@@ -346,7 +346,7 @@ template <typename T, typename TH, bool EDGE> int launch_vec(const shvk_block_no
     if (nvec <= 16) return launch_rows<T, TH, 2, 8, EDGE>(a, P, 128, s);
     if (nvec <= 32) return launch_rows<T, TH, 2, 16, EDGE>(a, P, 128, s);
     if (nvec <= 64) return launch_rows<T, TH, 2, 32, EDGE>(a, P, 128, s);
-    // one group a thread while a CTA may hold the row so (16,384 rows of 2,048: 65 us, two groups 71; of 2,047, with edges: 100 and 94)
+    // one group a thread while a CTA may hold the row so (16,384 rows of 2,048: 65 us, two groups 71; of 2,047, with edges: 100 and 93)
     if (!EDGE && nvec <= 512) return launch_rows<T, TH, 1, 0, false>(a, P, (nvec + 31) / 32 * 32, s);
     if (nvec <= 1024) return launch_rows<T, TH, 2, 0, EDGE>(a, P, ((nvec + 1) / 2 + 31) / 32 * 32, s);
     return launch_rows<T, TH, 4, 0, EDGE>(a, P, ((nvec + 3) / 4 + 31) / 32 * 32, s);

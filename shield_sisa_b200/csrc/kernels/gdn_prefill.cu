@@ -12,12 +12,13 @@
 // three) but not the range, so everything is scaled by powers of two, which cost no bits: a token's k and q by their norms, T by its
 // largest entry, rows of M by theirs, and the rows of S^T, W^T, U^T (one value column each; what a chunk does to them is linear) by scales
 // that the walk keeps or finds anew.  On the output's way S, M and U are two pieces as well (with one, of eleven bits, 11 % of bf16
-// outputs were not the rule's value rounded, now 0.03 %, in gdn_prefill_tc.cu 0.12 %; it costs 4 % of the time here, 6 % there).  Sums over tokens that last, S = e S + P, are rounded float32 FMAs and not tensor-core accumulations, whose
-// truncation would lean one way for thousands of chunks.
+// outputs were not the rule's value rounded, now 0.03 %, in gdn_prefill_tc.cu 0.12 %; it costs 4 % of the time here, 6 % there).  Sums over
+// tokens that last, S = e S + P, are rounded float32 FMAs and not tensor-core accumulations, whose truncation would lean one way for
+// thousands of chunks.
 //
 // This form takes short sequences and the widths that fill no CTA of gdn_prefill_tc.cu (see takes_tc).  128 sequences of 48 tokens, 6 heads of
 // 128 x 128, bf16: 80 us, for 38 MB of rows and 100 MB of states (21 us).  The walk's chain binds, dependent products and exchanges among
-// lanes: some 2,300 cycles for a chunk of 16 tokens (1.2 us; the 1,024 of one sequence 1.25 ms).
+// lanes: a chunk of 16 tokens takes 1.2 to 1.6 us (8 sequences of 2,048 tokens, DK 64, DV 64: 205 us).
 #include "gdn_pieces.cuh"
 #include "gdn_seq.cuh"
 

@@ -8,7 +8,7 @@
 //        TF32 pieces.  Both leave as fp16 pieces in the layout that the tensor core reads, the blocks above the diagonal left out: 16,912
 //        bytes a chunk (22,032 with the second piece of M, for fp16).  For bf16 the second piece of M's rows waits in the
 //        rows of o that it makes, 128 bytes of each, until the chunk's outputs go there: four CTAs of prep fit an SM so (with it in
-//        the workspace three, as for fp16: 285 us instead of 255 for 64 x 2,048), and walk loads it by TMA.
+//        the workspace three, as for fp16: 285 us for 64 x 2,048 tokens instead of 265), and walk loads it by TMA.
 // walk   a CTA per head and 128 value columns.  The values are the 128 lanes of tensor memory: S^T, W^T, U^T and D^T are operands that
 //        lie there as pieces, K, Q, T and M come from shared memory.  The state itself stays in registers: a value column's keys in two
 //        threads (eight warps), rounded by float32 FMAs; per chunk its pieces go to tensor memory and the product K^T D comes back.
@@ -18,16 +18,16 @@
 // A chunk is a chain: pieces of S -> K S0 -> W -> T W -> D -> K^T D -> S.  Q S0 and M U run beside it, and the outputs of a chunk are
 // written while the next one's first product runs.
 //
-// What bounds it.  64 sequences of 2,048 tokens, 6 heads of 128 x 128, bf16: prep 238 us and walk 386, for 862 MB that have to move (131 us
-// at the rate of a plain copy) and 0.16 TFLOP of the walk's products (97 us at cuBLAS's bf16 rate).  The walk is bound by its chain: a
-// chunk takes some 7,200 cycles of an SM (8,000 with all of them at work), of which the three products that it waits for are about 1,700;
-// cutting into pieces, the ways through tensor memory and shared memory and the meetings of threads are the rest.  A head's state and its
-// operands take all registers of an SM, so no second chain fills the gaps (384 chains on 148 SMs: three waves).  An instruction that is not in the cache costs most beside that,
-// which is why the loops below are rolled where they can be.  prep is a row of short phases between barriers, four CTAs of four warps on
+// What bounds it.  64 sequences of 2,048 tokens, 6 heads of 128 x 128, bf16: prep 265 us and walk 420 by themselves, 648 for the call, for
+// 862 MB that have to move (131 us at the rate of a plain copy) and 0.16 TFLOP of the walk's products (97 us at cuBLAS's bf16 rate).  The
+// walk is bound by its chain: a chunk takes 2.8 us (4.2 with all SMs at work), of which the three products that it waits for are about 0.9;
+// cutting into pieces, the ways through tensor memory and shared memory and the meetings of threads are the rest.  A CTA takes all columns of
+// tensor memory and nearly all shared memory of an SM, so no second chain fills the gaps (384 chains on 148 SMs: three waves).  An
+// instruction that is not in the cache costs most beside that, which is why the loops below are rolled where they can be.  prep is a row of short phases between barriers, four CTAs of four warps on
 // an SM (issue slots 46 % used, DRAM 20 %): loads 63 us, Gram products 39, scalars and masks 46, the diagonal's inverses 17, the products of
-// blocks 40, T's pieces 22, the copy out 11.
-// One sequence of 16,384 tokens, 6 heads: prep 36 us, the two walks of its segments 173, the join 26.  The kernels overlap where one drains:
-// 614 us and 233 for the two calls, 32 for one of 321 tokens with heads of 64 x 128.
+// blocks 40, T's pieces 22, the copy out 11, M's second piece 20.
+// One sequence of 16,384 tokens, 6 heads: prep 38 us, the two walks of its segments 99 and 89, the join 30, by themselves; the kernels overlap
+// where one drains: 241 us for the call, 34 for one of 321 tokens with heads of 64 x 128.
 #include "gdn_pieces.cuh"
 #include "gdn_seq.cuh"
 #include "tc_ptx.cuh"
@@ -1076,7 +1076,9 @@ template <int DK> __global__ void __launch_bounds__(JOIN_THREADS) gdn_prefill_tc
 
 // Chunks of a segment, 0 where sequences are walked whole.  Counted in chunks' times of one wave of CTAs (a walk's chunk takes 3.8 us, a
 // join's segment 2.3, the two launches more about as much as two chunks) for sequences of the average length; segments are not
-// shorter than 13 chunks, so that their states take less room than their chunks' T and M.
+// shorter than 13 chunks, so that their states take less room than their chunks' T and M.  us, 6 heads of 128 x 128, in segments / whole: 1
+// sequence of 2,600 141 / 174, of 16,384 242 / 996; 4 of 3,000 184 / 216; 8 of 4,000 290 / 317; 16 of 8,000, which stay whole, 725.  What
+// a join's segment is counted as hardly matters: at 0.15 chunks 1 of 16,384 241, 8 of 4,000 288, but one head of 50,000 275 instead of 271.
 inline int segment_chunks(const shvk_gdn_seq_args& a) {
     const long long sms = device_sms(), splits = (a.DV + TV - 1) / TV, heads = (long long)a.n_seq * a.HV, chunks = a.n_tokens / CT / a.n_seq;
     auto waves = [&](long long ctas) { return (ctas + sms - 1) / sms; };

@@ -894,7 +894,8 @@ def form_of(L, x):
 
 
 def assert_float32_outputs(x, want):
-    """The outputs are the rule's to float32's accuracy before they are rounded: few of them are another value of the type than the
+    """The outputs are the rule's to float32's accuracy before they are rounded, in either type (check allows bf16 outputs single pieces of
+    eleven bits on their way, which they no longer come from): few of them are another value of the type than the
     float64 ones' rounding.  An error e moves an output over a tie with a probability of 2 e / step, a step is at least eps / 2 of the
     value, and the mean of rms / |value| is some 4 (a normal value's, down to a thousandth of the rms).  With e within 2^-19 of the rms
     (the state's error is held to 1e-6 of its norm, half of that), that is 16 x 2^-19 / eps of the outputs: 0.4 % for bf16, 3 % for fp16.
